@@ -228,7 +228,7 @@ def _run_own(case, state):
         return llk.window_attention(state["q"], state["k"], state["v"], window=case["window"], sinks=case["sinks"],
                                     q_lens=state["q_lens"], kv_lens=state["kv_lens"])
     if "cache" not in state:  # the handle on the pool's tensors that a program keeps
-        state["cache"] = llk.QuantizedKVCache(*state["pool"])
+        state["cache"] = llk.QuantizedKVCache(*state["pool"], bits=case["bits"])
     cache = state["cache"]
     if case["op"] == "cache":
         return cache.attention(state["q"], state["table"], state["lens"], window=case["window"], sinks=case["sinks"])
