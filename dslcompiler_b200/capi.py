@@ -105,6 +105,19 @@ class LaunchPlan(ctypes.Structure):
                                             "threads", "smem_bytes", "sched")]
 
 
+class Tensor4D(ctypes.Structure):
+    """llk_tensor4d: [B, H, L, D], strides in elements."""
+    _fields_ = [("data", ctypes.c_void_p), ("dim", ctypes.c_int64 * 4), ("stride", ctypes.c_int64 * 4)]
+
+
+class KvCache(ctypes.Structure):
+    """llk_kv_cache: the quantised paged cache's arrays and geometry."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("k_params", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("v_params", ctypes.c_void_p), ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("bits", ctypes.c_int32),
+                ("group_size", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3)]
+
+
 # Every exported symbol with its prototype: (restype, argtypes).
 _P = ctypes.POINTER
 _vp, _i, _i64, _u64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64
@@ -116,6 +129,14 @@ PROTOTYPES = {
     "llk_matmul": (_i, [_P(Tensor2D), _P(Tensor2D), _P(Tensor2D), _i, _P(KernelContext), _P(GpuContext)]),
     "llk_rope": (_i, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_double, _P(GpuContext)]),
     "llk_attention": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _i, _P(GpuContext)]),
+    "llk_window_attention": (_i, [_P(Tensor4D), _P(Tensor4D), _P(Tensor4D), _P(Tensor4D), _i, _vp, _vp, _i64, _i64,
+                                 ctypes.c_float, _P(KernelContext), _P(GpuContext)]),
+    "llk_window_attention_scratch": (_i, [_P(Tensor4D), _P(Tensor4D), _i, _i64, _i64, _P(GpuContext), _P(_i64)]),
+    "llk_kv_cache_write": (_i, [_P(KvCache), _P(Tensor4D), _P(Tensor4D), _i, _vp, _P(GpuContext)]),
+    "llk_kv_cache_read": (_i, [_P(KvCache), _P(Tensor4D), _P(Tensor4D), _i, _vp, _P(GpuContext)]),
+    "llk_kv_cache_attention": (_i, [_P(Tensor4D), _P(KvCache), _vp, _i64, _i64, _vp, _vp, _P(Tensor4D), _i, _i64, _i64,
+                                   ctypes.c_float, _P(KernelContext), _P(GpuContext)]),
+    "llk_kv_cache_attention_scratch": (_i, [_P(Tensor4D), _P(KvCache), _i64, _i64, _i64, _P(GpuContext), _P(_i64)]),
     "llk_last_status": (_i, []),
     "llk_status_string": (ctypes.c_char_p, [_i]),
     "llk_synchronize": (_i, [_i, _vp]),

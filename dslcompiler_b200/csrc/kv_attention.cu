@@ -1,0 +1,90 @@
+// kv_attention.cu -- attention over the quantised paged cache, and the plan
+// of the split kernels (kv_attention.cuh).
+#include <type_traits>
+
+#include "kv_attention.cuh"
+
+namespace llk_b200 {
+
+using namespace split_attn;
+
+namespace {
+
+template <int BITS, int D, int G>
+cudaError_t launch_nt(const Params &a, cudaStream_t stream) {
+  if constexpr (row_tiles(16, D) == 2)
+    if (row_tiles(a.p.H / a.p.Hkv * a.p.mask.Lq, D) == 2) return launch_split<BITS, D, G, false, 2>(a, stream);
+  return launch_split<BITS, D, G, false, 1>(a, stream);
+}
+
+template <int BITS>
+cudaError_t launch_bits(const Params &a, cudaStream_t stream) {
+  const int groups = a.p.D / a.pool.group;
+  if (a.p.D == 64) return groups == 1 ? launch_nt<BITS, 64, 1>(a, stream) : launch_nt<BITS, 64, 2>(a, stream);
+  if (a.p.D == 128)
+    return groups == 1   ? launch_nt<BITS, 128, 1>(a, stream)
+           : groups == 2 ? launch_nt<BITS, 128, 2>(a, stream)
+                         : launch_nt<BITS, 128, 4>(a, stream);
+  return groups == 2   ? launch_nt<BITS, 256, 2>(a, stream)
+         : groups == 4 ? launch_nt<BITS, 256, 4>(a, stream)
+                       : launch_nt<BITS, 256, 8>(a, stream);
+}
+
+}  // namespace
+
+bool split_supported(const AttnProblem &p, const KvPool *pool) {
+  const int64_t g = p.Hkv > 0 ? p.H / p.Hkv : 0, rows = g * p.mask.Lq;
+  if (p.dtype != LLK_DTYPE_BF16 && p.dtype != LLK_DTYPE_FP16) return false;
+  if (p.B > 65535 || (rows + 7) / 8 * p.Hkv > 65535) return false;
+  if (pool) return kv_pool_supported(*pool);
+  const auto on16 = [](const View4 &v) {
+    return (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % 8 == 0 && v.sh % 8 == 0 && v.sl % 8 == 0;
+  };
+  return (p.D == 64 || p.D == 80 || p.D == 96 || p.D == 128 || p.D == 256) && on16(p.k) && on16(p.v);
+}
+
+// As many splits as fill the GPU's resident CTAs once (4 a SM), but at least
+// two blocks of 16 tokens for every warp of a CTA.  The lengths are on the
+// device, so the plan goes by the most keys a sequence can have.
+SplitPlan split_plan(const AttnProblem &p, const KvPool *pool, int sm_count) {
+  (void)pool;
+  SplitPlan s;
+  const int rows = p.H / p.Hkv * p.mask.Lq, nt = row_tiles(rows, p.D);
+  s.row_blocks = (rows + 8 * nt - 1) / (8 * nt);
+  int64_t keys = p.mask.Lk;
+  if (p.mask.window > 0) {
+    const int64_t seen = static_cast<int64_t>(p.mask.window) + p.mask.Lq + p.mask.sinks;
+    if (seen < keys) keys = seen;
+  }
+  const int64_t base = static_cast<int64_t>(p.B) * p.Hkv * s.row_blocks;
+  const int64_t room = 4 * static_cast<int64_t>(sm_count) / (base > 0 ? base : 1);
+  const int64_t most = (keys + 2 * kWarps * kTok - 1) / (2 * kWarps * kTok);
+  int64_t n = room < most ? room : most;
+  s.splits = static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
+  s.ws_bytes = 0;
+  if (s.splits > 1) {
+    const size_t cols = static_cast<size_t>(base) * s.splits * 8 * nt;
+    s.ws_bytes = cols * (static_cast<size_t>(p.D) * 4 + sizeof(float2));
+  }
+  return s;
+}
+
+cudaError_t split_launch(const AttnProblem &p, const KvPool *pool, const int *block_table, int64_t table_width,
+                         const SplitPlan &plan, void *workspace, cudaStream_t stream) {
+  if (p.B == 0 || p.H == 0 || p.mask.Lq == 0) return cudaSuccess;
+  Params a = {};
+  a.p = p;
+  if (pool) a.pool = *pool;
+  a.table = block_table;
+  a.table_width = table_width;
+  a.splits = plan.splits;
+  a.row_blocks = plan.row_blocks;
+  const int nt = row_tiles(p.H / p.Hkv * p.mask.Lq, p.D);
+  const size_t cols = static_cast<size_t>(p.B) * p.Hkv * plan.row_blocks * plan.splits * 8 * nt;
+  a.part_ml = static_cast<float2 *>(workspace);
+  a.part_o = reinterpret_cast<float *>(a.part_ml + cols);
+  if (!pool) return launch_dense(a, stream);
+  return pool->bits == 4 ? launch_bits<4>(a, stream) : launch_bits<8>(a, stream);
+}
+
+}  // namespace llk_b200

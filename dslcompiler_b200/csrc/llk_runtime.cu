@@ -23,6 +23,7 @@
 
 #include "attention_kernels.h"
 #include "decode_kernels.h"
+#include "kv_kernels.h"
 #include "llk_b200.h"
 #include "tc_kernels.h"
 #include "workspace.h"
@@ -62,6 +63,7 @@ struct DeviceState {
   int *status = nullptr;       // device error word written by the kernels
   DeviceBuffer stage[4];       // host-staging buffers: x, wg, wu, y
   DeviceBuffer workspace;      // split-K partials when the caller gives no scratch
+  DeviceBuffer attn_ws;        // serving attention's split partials likewise (never used by a captured call)
   // Pipelined host-buffer SwiGLU: double-buffered weight / Y column chunks,
   // a copy-in and a copy-out stream, and their events.
   DeviceBuffer chunk_w[2][2];  // [buffer][gate, up]
@@ -1043,6 +1045,291 @@ int llk_attention(const float *q, const float *k, const float *v, float *o, int6
                             static_cast<const float *>(p[2]), static_cast<float *>(p[3]), B, H, Lq, Lk, D, scale,
                             causal ? 1 : 0, fast ? 1 : 0, s);
   });
+}
+
+// ------------------------------------------------- attention for serving
+namespace {
+
+constexpr int64_t kMaxLen = int64_t(1) << 30;
+
+// [B, H, L, D] with unit stride along D, as the kernels take it; a dimension
+// of size 1 gets stride 0, so that its stride does not decide the alignment.
+int view4(const llk_tensor4d &t, View4 *out) {
+  for (int i = 0; i < 4; ++i)
+    if (t.dim[i] < 0) return LLK_ERR_SHAPE;
+  if (t.dim[3] > 1 && t.stride[3] != 1) return LLK_ERR_ALIGN;
+  int64_t s[3];
+  for (int i = 0; i < 3; ++i) {
+    if (t.dim[i] > 1 && t.stride[i] < 0) return LLK_ERR_ALIGN;
+    s[i] = t.dim[i] > 1 ? t.stride[i] : 0;
+  }
+  *out = {t.data, s[0], s[1], s[2]};
+  return LLK_OK;
+}
+
+// An output's rows may not lie on one another.
+bool rows_apart(const llk_tensor4d &t) {
+  for (int i = 0; i < 3; ++i)
+    if (t.dim[i] > 1 && t.stride[i] < t.dim[3]) return false;
+  return true;
+}
+
+int dtype_bytes(int dtype) {
+  return dtype == LLK_DTYPE_FP32 ? 4 : (dtype == LLK_DTYPE_BF16 || dtype == LLK_DTYPE_FP16) ? 2 : 0;
+}
+
+bool aligned_to(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Shape rules of both attentions; k's shape is (Hkv, Lk).
+int attn_problem(const llk_tensor4d *q, int64_t Hkv, int64_t Lk, int dtype, int64_t window, int64_t sinks,
+                 float scale, AttnProblem *P) {
+  *P = AttnProblem{};
+  int rc = view4(*q, &P->q);
+  if (rc != LLK_OK) return rc;
+  if (!dtype_bytes(dtype) || window < 0 || sinks < 0) return LLK_ERR_ARG;
+  const int64_t B = q->dim[0], H = q->dim[1], Lq = q->dim[2], D = q->dim[3];
+  if (Hkv < 0 || (Hkv == 0 && H > 0) || (Hkv > 0 && H % Hkv != 0)) return LLK_ERR_SHAPE;
+  if (B > kMaxLen || H > kMaxLen || B * H > kMaxLen || Lq > kMaxLen || Lk > kMaxLen || D > 256 ||
+      (Hkv > 0 && H / Hkv * Lq > kMaxLen))
+    return LLK_ERR_UNSUPPORTED;
+  P->B = static_cast<int>(B);
+  P->H = static_cast<int>(H);
+  P->Hkv = static_cast<int>(Hkv);
+  P->D = static_cast<int>(D);
+  P->dtype = dtype;
+  P->scale = scale;
+  P->mask.Lq = static_cast<int>(Lq);
+  P->mask.Lk = static_cast<int>(Lk);
+  P->mask.window = window > Lk ? 0 : static_cast<int>(window);  // a window over every key is none
+  P->mask.sinks = static_cast<int>(sinks < Lk ? sinks : Lk);
+  return LLK_OK;
+}
+
+// Few query rows take the kernels that split the keys.
+bool use_split(const AttnProblem &P) {
+  return split_supported(P, nullptr) && static_cast<int64_t>(P.H / P.Hkv) * P.mask.Lq <= 64;
+}
+
+int window_problem(const llk_tensor4d *q, const llk_tensor4d *k, int dtype, int64_t window, int64_t sinks, float scale,
+                   AttnProblem *P) {
+  int rc = attn_problem(q, k->dim[1], k->dim[2], dtype, window, sinks, scale, P);
+  if (rc != LLK_OK || (rc = view4(*k, &P->k)) != LLK_OK) return rc;
+  return k->dim[0] == q->dim[0] && k->dim[3] == q->dim[3] ? LLK_OK : LLK_ERR_SHAPE;
+}
+
+int kv_pool(const llk_kv_cache *c, KvPool *out) {
+  if (!c || c->reserved[0] || c->reserved[1] || c->reserved[2]) return LLK_ERR_ARG;
+  if (c->num_pages < 0 || c->page_size < 1 || c->kv_heads < 1 || c->head_dim < 1 || c->bits < 1 || c->group_size < 1 ||
+      c->head_dim % c->group_size != 0)
+    return LLK_ERR_SHAPE;
+  *out = {c->k_codes,   c->k_params,    c->v_codes, c->v_params,  c->num_pages,
+          c->page_size, c->kv_heads, c->head_dim, c->bits, c->group_size};
+  if (!kv_pool_supported(*out)) return LLK_ERR_UNSUPPORTED;
+  if (c->num_pages > 0 && (!c->k_codes || !c->k_params || !c->v_codes || !c->v_params)) return LLK_ERR_ARG;
+  if (!aligned16(c->k_codes) || !aligned16(c->k_params) || !aligned16(c->v_codes) || !aligned16(c->v_params))
+    return LLK_ERR_ALIGN;
+  return LLK_OK;
+}
+
+// Device memory for the parts of a split launch: the caller's scratch, or
+// the library's buffer when the call is not being captured.
+int split_workspace(DeviceState &ds, size_t need, const KernelContext *ctx, cudaStream_t stream, void **out) {
+  *out = nullptr;
+  if (need == 0) return LLK_OK;
+  if (ctx && ctx->scratch && ctx->scratch_size >= need && aligned16(ctx->scratch)) {
+    *out = ctx->scratch;
+    return LLK_OK;
+  }
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &cap) != cudaSuccess) {
+    cudaGetLastError();
+    return LLK_ERR_CUDA;
+  }
+  if (cap != cudaStreamCaptureStatusNone) return LLK_ERR_NOMEM;
+  if (ds.attn_ws.ensure(need) != cudaSuccess) {
+    cudaGetLastError();
+    return LLK_ERR_NOMEM;
+  }
+  *out = ds.attn_ws.ptr;
+  return LLK_OK;
+}
+
+// The call's device, its state, and a check that every pointer is its memory.
+int enter(const llk_gpu_context *gpu, const void *const *ptrs, int n, DeviceState **ds, cudaStream_t *stream) {
+  int dev, rc;
+  if ((rc = resolve_device(gpu, &dev)) != LLK_OK) return rc;
+  if ((rc = device_init(dev, ds)) != LLK_OK) return rc;
+  *stream = gpu ? static_cast<cudaStream_t>(gpu->stream) : nullptr;
+  for (int i = 0; i < n; ++i)
+    if (ptrs[i] && locate_ptr(ptrs[i], dev) != 1) return LLK_ERR_ARG;
+  return LLK_OK;
+}
+
+int launched(cudaError_t e) {
+  if (e == cudaSuccess) return LLK_OK;
+  cudaGetLastError();
+  return LLK_ERR_CUDA;
+}
+
+}  // namespace
+
+int llk_window_attention_scratch(const llk_tensor4d *q, const llk_tensor4d *k, int dtype, int64_t window, int64_t sinks,
+                                 const llk_gpu_context *gpu, int64_t *bytes) {
+  if (!q || !k || !bytes) return LLK_ERR_ARG;
+  DeviceRestore restore;
+  AttnProblem P;
+  int rc = window_problem(q, k, dtype, window, sinks, 1.f, &P);
+  if (rc != LLK_OK) return rc;
+  *bytes = 0;
+  if (P.B == 0 || P.H == 0 || P.mask.Lq == 0 || P.D == 0) return LLK_OK;
+  P.v = P.k;
+  DeviceState *ds;
+  cudaStream_t stream;
+  if ((rc = enter(gpu, nullptr, 0, &ds, &stream)) != LLK_OK) return rc;
+  if (use_split(P)) *bytes = static_cast<int64_t>(split_plan(P, nullptr, ds->sm_count).ws_bytes);
+  return LLK_OK;
+}
+
+int llk_window_attention(const llk_tensor4d *q, const llk_tensor4d *k, const llk_tensor4d *v, llk_tensor4d *o,
+                         int dtype, const int32_t *q_lens, const int32_t *kv_lens, int64_t window, int64_t sinks,
+                         float scale, KernelContext *ctx, const llk_gpu_context *gpu) {
+  if (!q || !k || !v || !o) return LLK_ERR_ARG;
+  AttnProblem P;
+  int rc = window_problem(q, k, dtype, window, sinks, scale, &P);
+  if (rc != LLK_OK || (rc = view4(*v, &P.v)) != LLK_OK || (rc = view4(*o, &P.o)) != LLK_OK) return rc;
+  for (int i = 0; i < 4; ++i)
+    if (v->dim[i] != k->dim[i] || o->dim[i] != q->dim[i]) return LLK_ERR_SHAPE;
+  if (P.B == 0 || P.H == 0 || P.mask.Lq == 0 || P.D == 0) return LLK_OK;
+  if (!rows_apart(*o)) return LLK_ERR_ALIGN;
+  const int el = dtype_bytes(dtype);
+  if (!q->data || !o->data || (P.mask.Lk > 0 && (!k->data || !v->data))) return LLK_ERR_ARG;
+  if (!aligned_to(q->data, el) || !aligned_to(k->data, el) || !aligned_to(v->data, el) || !aligned_to(o->data, el) ||
+      !aligned_to(q_lens, 4) || !aligned_to(kv_lens, 4))
+    return LLK_ERR_ALIGN;
+  if (o->data == q->data || (P.mask.Lk > 0 && (o->data == k->data || o->data == v->data))) return LLK_ERR_ARG;
+  P.mask.q_lens = q_lens;
+  P.mask.kv_lens = kv_lens;
+  DeviceRestore restore;
+  DeviceState *ds;
+  cudaStream_t stream;
+  const bool keys = P.mask.Lk > 0;
+  const void *ptrs[6] = {q->data, o->data, keys ? k->data : nullptr, keys ? v->data : nullptr, q_lens, kv_lens};
+  if ((rc = enter(gpu, ptrs, 6, &ds, &stream)) != LLK_OK) return rc;
+  if (use_split(P)) {
+    std::lock_guard<std::mutex> lk(ds->mu);
+    const SplitPlan plan = split_plan(P, nullptr, ds->sm_count);
+    void *ws;
+    if ((rc = split_workspace(*ds, plan.ws_bytes, ctx, stream, &ws)) != LLK_OK) return rc;
+    return launched(split_launch(P, nullptr, nullptr, 0, plan, ws, stream));
+  }
+  if (!window_simt_supported(P)) return LLK_ERR_UNSUPPORTED;
+  return launched(window_simt_launch(P, stream));
+}
+
+namespace {
+int kv_move(const llk_kv_cache *cache, const llk_tensor4d *k, const llk_tensor4d *v, int dtype, const int64_t *slots,
+            const llk_gpu_context *gpu, bool write) {
+  if (!cache || !k || !v) return LLK_ERR_ARG;
+  KvPool pool;
+  View4 vk, vv;
+  int rc = kv_pool(cache, &pool);
+  if (rc != LLK_OK || (rc = view4(*k, &vk)) != LLK_OK || (rc = view4(*v, &vv)) != LLK_OK) return rc;
+  const int el = dtype_bytes(dtype);
+  if (!el) return LLK_ERR_ARG;
+  for (int i = 0; i < 4; ++i)
+    if (v->dim[i] != k->dim[i]) return LLK_ERR_SHAPE;
+  if (k->dim[1] != pool.Hkv || k->dim[3] != pool.D) return LLK_ERR_SHAPE;
+  const int64_t B = k->dim[0], L = k->dim[2];
+  if (B == 0 || L == 0) return LLK_OK;
+  // rows of both tensors are counted in 32 bits
+  if (B > kMaxLen || L > kMaxLen || B * L > kMaxLen || B * L * pool.Hkv > kMaxLen) return LLK_ERR_UNSUPPORTED;
+  if (!slots || !k->data || !v->data || (!write && k->data == v->data)) return LLK_ERR_ARG;
+  if (!aligned_to(k->data, el) || !aligned_to(v->data, el) || !aligned_to(slots, 8)) return LLK_ERR_ALIGN;
+  if (!write && (!rows_apart(*k) || !rows_apart(*v))) return LLK_ERR_ALIGN;
+  DeviceRestore restore;
+  DeviceState *ds;
+  cudaStream_t stream;
+  const void *ptrs[7] = {k->data, v->data, slots, pool.k_codes, pool.k_params, pool.v_codes, pool.v_params};
+  if ((rc = enter(gpu, ptrs, pool.num_pages > 0 ? 7 : 3, &ds, &stream)) != LLK_OK) return rc;
+  return launched(write ? kv_write_launch(pool, vk, vv, dtype, B, L, slots, ds->sm_count, stream)
+                        : kv_read_launch(pool, vk, vv, dtype, B, L, slots, ds->sm_count, stream));
+}
+}  // namespace
+
+int llk_kv_cache_write(const llk_kv_cache *cache, const llk_tensor4d *k, const llk_tensor4d *v, int dtype,
+                       const int64_t *slots, const llk_gpu_context *gpu) {
+  return kv_move(cache, k, v, dtype, slots, gpu, true);
+}
+
+int llk_kv_cache_read(const llk_kv_cache *cache, const llk_tensor4d *k, const llk_tensor4d *v, int dtype,
+                      const int64_t *slots, const llk_gpu_context *gpu) {
+  return kv_move(cache, k, v, dtype, slots, gpu, false);
+}
+
+namespace {
+int cache_problem(const llk_tensor4d *q, const KvPool &pool, int64_t table_width, int dtype, int64_t window,
+                  int64_t sinks, float scale, AttnProblem *P) {
+  if (table_width < 0) return LLK_ERR_SHAPE;
+  if (table_width > kMaxLen / pool.page) return LLK_ERR_UNSUPPORTED;
+  const int rc = attn_problem(q, pool.Hkv, table_width * pool.page, dtype, window, sinks, scale, P);
+  if (rc != LLK_OK) return rc;
+  if (q->dim[3] != pool.D) return LLK_ERR_SHAPE;
+  return dtype == LLK_DTYPE_FP32 || !split_supported(*P, &pool) ? LLK_ERR_UNSUPPORTED : LLK_OK;
+}
+}  // namespace
+
+int llk_kv_cache_attention_scratch(const llk_tensor4d *q, const llk_kv_cache *cache, int64_t table_width,
+                                   int64_t window, int64_t sinks, const llk_gpu_context *gpu, int64_t *bytes) {
+  if (!q || !cache || !bytes) return LLK_ERR_ARG;
+  DeviceRestore restore;
+  KvPool pool;
+  AttnProblem P;
+  int rc = kv_pool(cache, &pool);
+  if (rc != LLK_OK || (rc = cache_problem(q, pool, table_width, LLK_DTYPE_BF16, window, sinks, 1.f, &P)) != LLK_OK)
+    return rc;
+  *bytes = 0;
+  if (P.B == 0 || P.H == 0 || P.mask.Lq == 0) return LLK_OK;
+  DeviceState *ds;
+  cudaStream_t stream;
+  if ((rc = enter(gpu, nullptr, 0, &ds, &stream)) != LLK_OK) return rc;
+  *bytes = static_cast<int64_t>(split_plan(P, &pool, ds->sm_count).ws_bytes);
+  return LLK_OK;
+}
+
+int llk_kv_cache_attention(const llk_tensor4d *q, const llk_kv_cache *cache, const int32_t *block_table,
+                           int64_t table_width, int64_t table_stride, const int32_t *q_lens, const int32_t *kv_lens,
+                           llk_tensor4d *o, int dtype, int64_t window, int64_t sinks, float scale, KernelContext *ctx,
+                           const llk_gpu_context *gpu) {
+  if (!q || !cache || !o) return LLK_ERR_ARG;
+  KvPool pool;
+  AttnProblem P;
+  int rc = kv_pool(cache, &pool);
+  if (rc != LLK_OK || (rc = cache_problem(q, pool, table_width, dtype, window, sinks, scale, &P)) != LLK_OK ||
+      (rc = view4(*o, &P.o)) != LLK_OK)
+    return rc;
+  for (int i = 0; i < 4; ++i)
+    if (o->dim[i] != q->dim[i]) return LLK_ERR_SHAPE;
+  if (P.B == 0 || P.H == 0 || P.mask.Lq == 0) return LLK_OK;
+  if (P.B > 1 && table_stride < table_width) return LLK_ERR_SHAPE;
+  if (!rows_apart(*o)) return LLK_ERR_ALIGN;
+  if (!q->data || !o->data || !kv_lens || (table_width > 0 && !block_table)) return LLK_ERR_ARG;
+  if (!aligned_to(q->data, 2) || !aligned_to(o->data, 2) || !aligned_to(block_table, 4) || !aligned_to(q_lens, 4) ||
+      !aligned_to(kv_lens, 4))
+    return LLK_ERR_ALIGN;
+  if (o->data == q->data) return LLK_ERR_ARG;
+  P.mask.q_lens = q_lens;
+  P.mask.kv_lens = kv_lens;
+  DeviceRestore restore;
+  DeviceState *ds;
+  cudaStream_t stream;
+  const void *ptrs[9] = {q->data,     o->data,      table_width > 0 ? block_table : nullptr, q_lens, kv_lens,
+                         pool.k_codes, pool.k_params, pool.v_codes, pool.v_params};
+  if ((rc = enter(gpu, ptrs, pool.num_pages > 0 ? 9 : 5, &ds, &stream)) != LLK_OK) return rc;
+  std::lock_guard<std::mutex> lk(ds->mu);
+  const SplitPlan plan = split_plan(P, &pool, ds->sm_count);
+  void *ws;
+  if ((rc = split_workspace(*ds, plan.ws_bytes, ctx, stream, &ws)) != LLK_OK) return rc;
+  return launched(split_launch(P, &pool, block_table, table_width > 0 ? table_stride : 0, plan, ws, stream));
 }
 
 int llk_synchronize(int device, void *stream) {

@@ -174,6 +174,96 @@ int llk_rope(const float *x, const int64_t *position_ids, float *y, int64_t B, i
 int llk_attention(const float *q, const float *k, const float *v, float *o, int64_t B, int64_t H, int64_t Lq,
                   int64_t Lk, int64_t D, float scale, int causal, const llk_gpu_context *gpu);
 
+/* ---- attention for serving ----------------------------------------------
+ * Attention in the serving types with grouped heads, a sliding window and
+ * sinks, over dense keys and values or over a quantised paged KV cache, and
+ * the cache's writer and reader.  No counterpart in the reference.
+ *
+ * All data is DEVICE memory of the call's device (or managed memory): host
+ * buffers and other GPUs' buffers are refused with LLK_ERR_ARG.  Calls are
+ * asynchronous on gpu->stream; gpu->math_mode and variant are ignored (the
+ * 16-bit kernels use the hardware's exp2, 2 ulp, whose error a 16-bit result
+ * does not show; f32 uses exp2f).
+ *
+ * What a query sees: sequence b has n = kv_lens[b] keys and m = q_lens[b]
+ * queries (NULL: as many as the tensors hold; values outside the tensors are
+ * clamped), query i < m is the token at position p = n - m + i, and
+ *   o[b,h,i,:] = sum_j softmax_j(scale * q[b,h,i,:] . k[b,h',j,:]) v[b,h',j,:]
+ * over the keys j <= p with window == 0 or j > p - window or j < sinks
+ * (h' = h / (H / Hkv)).  A query that sees no key gives zeros; rows i >= m of
+ * O are left as they were.  Keys and values that a query does not see do not
+ * affect it, whatever they hold (infinities and NaN included).  O must not
+ * overlap q, k or v. */
+
+/* [B, H, L, D]: strides in elements, stride[3] must be 1, none negative. */
+typedef struct llk_tensor4d {
+  void *data;
+  int64_t dim[4];
+  int64_t stride[4];
+} llk_tensor4d;
+
+/* q, o: [B, H, Lq, D]; k, v: [B, Hkv, Lk, D], Hkv dividing H (else
+ * LLK_ERR_SHAPE); dtype (enum llk_dtype) is that of all four: BF16, FP16 or
+ * FP32.  q_lens, kv_lens: [B] or NULL.  D <= 256, Lq and Lk <= 2^30 (else
+ * LLK_ERR_UNSUPPORTED).
+ *
+ * Scratch: few queries over many keys are split along the keys and joined
+ * through llk_window_attention_scratch() bytes of device memory, taken from
+ * ctx->scratch (16-byte aligned) when it is large enough, else from a buffer
+ * of the library (one a device, grown with cudaMalloc).  Calls that share
+ * either buffer must not overlap on the GPU.  A call that is being captured
+ * into a CUDA graph does not use the library's buffer, which a later call may
+ * move: without enough ctx->scratch it returns LLK_ERR_NOMEM. */
+int llk_window_attention(const llk_tensor4d *q, const llk_tensor4d *k, const llk_tensor4d *v, llk_tensor4d *o,
+                         int dtype, const int32_t *q_lens, const int32_t *kv_lens, int64_t window, int64_t sinks,
+                         float scale, KernelContext *ctx, const llk_gpu_context *gpu);
+int llk_window_attention_scratch(const llk_tensor4d *q, const llk_tensor4d *k, int dtype, int64_t window,
+                                 int64_t sinks, const llk_gpu_context *gpu, int64_t *bytes);
+
+/* A paged cache of keys and values in 4 or 8 bits, owned by the caller:
+ *   k_codes, v_codes   [num_pages, kv_heads, page_size, head_dim * bits / 8] bytes
+ *                      (4 bits: element 2j in the low nibble of byte j);
+ *   k_params, v_params [num_pages, kv_heads, page_size, head_dim / group_size]
+ *                      pairs (scale, min) of bf16, scale first.
+ * An element stands for scale * code + min.  head_dim 64, 128 or 256; bits 4
+ * or 8; group_size 32, 64 or 128, dividing head_dim; page_size a multiple of
+ * 16; all four pointers 16-byte aligned.  Token t of a sequence lies in page
+ * block_table[b][t / page_size] at offset t % page_size; slot number = page *
+ * page_size + offset. */
+typedef struct llk_kv_cache {
+  void *k_codes, *k_params, *v_codes, *v_params;
+  int64_t num_pages;
+  int32_t page_size, kv_heads, head_dim, bits, group_size;
+  int32_t reserved[3]; /* must be zero */
+} llk_kv_cache;
+
+/* Quantises k, v [B, kv_heads, L, head_dim] (BF16, FP16 or FP32) into the
+ * slots [B, L].  x is saturated to +-65504 and NaN counts as 0; per group
+ *   min = bf16(smallest x), scale = bf16(max((largest x - min) / (2^bits - 1), 2^-30)),
+ *   code = (x - min) / scale rounded to nearest even, within [0, 2^bits - 1].
+ * A slot outside the cache (such as -1, padding) is not written; when a slot
+ * is named more than once, its last token in [B, L] order stands. */
+int llk_kv_cache_write(const llk_kv_cache *cache, const llk_tensor4d *k, const llk_tensor4d *v, int dtype,
+                       const int64_t *slots, const llk_gpu_context *gpu);
+
+/* Reads slots [B, L] back into k, v [B, kv_heads, L, head_dim]; a slot
+ * outside the cache reads as zeros. */
+int llk_kv_cache_read(const llk_kv_cache *cache, const llk_tensor4d *k, const llk_tensor4d *v, int dtype,
+                      const int64_t *slots, const llk_gpu_context *gpu);
+
+/* Attention of q [B, H, Lq, head_dim] (BF16 or FP16) over the cache:
+ * sequence b's keys are the first kv_lens[b] tokens of its pages, row b of
+ * block_table (table_width entries, table_stride apart).  The new tokens are
+ * written to the cache before the call, so kv_lens counts them.  An entry
+ * outside the pool holds tokens that no query sees.  Scratch as for
+ * llk_window_attention. */
+int llk_kv_cache_attention(const llk_tensor4d *q, const llk_kv_cache *cache, const int32_t *block_table,
+                           int64_t table_width, int64_t table_stride, const int32_t *q_lens, const int32_t *kv_lens,
+                           llk_tensor4d *o, int dtype, int64_t window, int64_t sinks, float scale, KernelContext *ctx,
+                           const llk_gpu_context *gpu);
+int llk_kv_cache_attention_scratch(const llk_tensor4d *q, const llk_kv_cache *cache, int64_t table_width,
+                                   int64_t window, int64_t sinks, const llk_gpu_context *gpu, int64_t *bytes);
+
 /* Status of the last call on this host thread (llk_swiglu, _memref). */
 int llk_last_status(void);
 const char *llk_status_string(int status);
