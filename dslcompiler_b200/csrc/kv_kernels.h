@@ -50,6 +50,12 @@ struct KvPool {
 bool window_simt_supported(const AttnProblem &p);
 cudaError_t window_simt_launch(const AttnProblem &p, cudaStream_t stream);
 
+// Tensor-core kernel for prompts: bf16 / f16, D <= 128, rows on 16 bytes.
+// encode_fn: cuTensorMapEncodeTiled; status: the device's error word (a
+// bounded wait that gave up).
+bool window_tc_supported(const AttnProblem &p);
+cudaError_t window_tc_launch(void *encode_fn, const AttnProblem &p, int *status, cudaStream_t stream);
+
 bool kv_pool_supported(const KvPool &p);
 // k, v: [B, Hkv, L, D] views of type dtype; slots [B, L].
 cudaError_t kv_write_launch(const KvPool &p, const View4 &k, const View4 &v, int dtype, int64_t B, int64_t L,

@@ -1,0 +1,572 @@
+// window_attention_tc.cu -- llk.window_attention for prompts in bf16 / f16 on
+// the tensor cores (tcgen05, TMEM, TMA).
+//
+//   S = Q K^T,  P = 2^(scale log2 e S - m),  O = O + P V,  l = l + sum P
+// per key tile, with the running reference m of the softmax (a row's maximum,
+// or up to 2^8 below it: see kSlack) and O / l at the end.
+//
+// A CTA owns 256 query rows of one head as two tiles of 128, and sweeps the
+// key tiles that any of its rows sees: the sinks' tiles, then the window's.
+// A query tile skips the key tiles that none of its own rows sees.
+//   warps 0-3, 4-7  softmax of query tile 0 / 1, one thread a row: S from
+//                   TMEM to registers, P back to TMEM in 16 bits, O's rescale
+//                   when the reference moves, the output
+//   warp 8          TMA: Q once, K and V tiles through one ring of stages
+//   warp 9          tcgen05.mma: S = Q K^T (both operands in shared memory),
+//                   O += P V (P from TMEM)
+// TMEM columns: O0, O1, S0, S1, P0, P1.  S and P do not share columns, so
+// the next S of a query tile is computed while its softmax runs on the
+// registers, and the softmax warps never wait for the tensor core; that, and
+// 512 columns, make the key tile 80 wide at D = 128 (80 + 40 + 128 columns a
+// query tile) and 96 at D = 64.
+//
+// 4 D FLOP and one exponential a pair: at D = 128 the tensor core (8192 FLOP
+// a clock and SM) and the exponential unit (16 a clock and SM) need the same
+// 512 clocks for 128 x 64 pairs.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "attn_common.cuh"
+
+namespace llk_b200 {
+
+namespace {
+
+constexpr int kBM = 128;                // rows of a query tile
+constexpr int kThreads = 320;
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+// The reference m may lag a row's maximum by up to this power of two before O
+// is rescaled: P stays below 2^8, far inside f16, its relative rounding is
+// the same, and the f32 sums do not mind.
+constexpr float kSlack = 8.f;
+
+struct TcMaps {
+  CUtensorMap q, k, v;
+};
+
+struct TcArgs {
+  AttnProblem p;
+  int q_blocks;
+  // 0 for a broadcast dimension of the maps, else 1
+  int qb, qh, kb, kh, vb, vh;
+  int vec_o;  // output rows start on 16 bytes
+  int *status;
+};
+
+template <int D>
+struct Cfg {
+  static constexpr int kKT = D == 128 ? 80 : 96;       // keys of a tile
+  static constexpr int kSlabs = D / 64;
+  static constexpr int kQBytes = kBM * D * 2;          // one query tile
+  static constexpr int kStageBytes = kKT * D * 2;      // one K or V tile
+  static constexpr int kStages = D == 128 ? 7 : 8;
+  static constexpr int kColO = 0, kColS = 2 * D, kColP = kColS + 2 * kKT, kCols = 512;
+  static_assert(kColP + kKT <= kCols, "TMEM columns");
+};
+
+struct Tail {
+  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], mma_done;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem, 16-bit pairs along K in a column] * B[smem].
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x8(uint32_t t, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__host__ __device__ constexpr uint32_t idesc_16(bool bf16, uint32_t m, uint32_t n, bool b_mn_major) {
+  const uint32_t t = bf16 ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if constexpr (kBf16) {
+    asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
+  }
+  return r;
+}
+
+// The key tiles of a CTA: s_tiles of sinks, then from the window's first.
+struct Sweep {
+  int n, m, p0, hi, lo, s_keys, s_tiles, w_first, tiles, sinks, window;
+  __device__ __forceinline__ int key0(int j, int kt) const { return (j < s_tiles ? j : w_first + j - s_tiles) * kt; }
+  // does any row of query tile t (rows p0 + 128 t ..) see a key of the tile at k0?
+  __device__ __forceinline__ bool active(int t, int k0, int kt) const {
+    const int first = p0 + kBM * t;
+    int last = first + kBM - 1;
+    last = last < hi - 1 ? last : hi - 1;
+    if (last < first || last < k0) return false;
+    const int flo = window > 0 && first >= window ? first - window + 1 : 0;
+    return k0 + kt > flo || k0 < sinks;
+  }
+};
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+    window_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs A) {
+  using C = Cfg<D>;
+  constexpr int KT = C::kKT, ST = C::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *smem_kv = smem + 2 * C::kQBytes;
+  Tail *st = reinterpret_cast<Tail *>(smem_kv + ST * C::kStageBytes);
+  const AttnProblem &P = A.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int BH = P.B * P.H;
+  // the last query blocks first: under the causal mask they have the most keys
+  const int b = static_cast<int>(blockIdx.x % BH) / P.H, h = static_cast<int>(blockIdx.x % BH) % P.H;
+  const int q0 = (A.q_blocks - 1 - static_cast<int>(blockIdx.x / BH)) * 2 * kBM;
+  const int hk = h / (P.H / P.Hkv);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&st->q_full[i], 1);
+      mbar_init(&st->s_full[i], 1);
+      mbar_init(&st->s_empty[i], kBM);
+      mbar_init(&st->p_ready[i], kBM);
+      mbar_init(&st->pv_done[i], 1);
+    }
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&st->kv_full[i], 1);
+      mbar_init(&st->kv_empty[i], 1);
+    }
+    mbar_init(&st->mma_done, 1);
+    st->abort = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&maps.q);
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
+  }
+  if (warp == 9) {
+    tmem_alloc(&st->tmem, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t tmem = st->tmem;
+  volatile int *abort = &st->abort;
+
+  Sweep w;
+  seq_lens(P.mask, b, w.n, w.m);
+  w.sinks = P.mask.sinks;
+  w.window = P.mask.window;
+  const int rows = w.m - q0;  // of this CTA (may be <= 0 or > 256)
+  w.p0 = w.n - w.m + q0;
+  w.hi = w.p0 + (rows < 2 * kBM ? rows : 2 * kBM);
+  w.lo = window_lo(P.mask, w.p0);
+  w.s_keys = w.sinks < w.lo ? w.sinks : w.lo;
+  w.w_first = w.lo / KT;
+  const int s_all = (w.s_keys + KT - 1) / KT;
+  w.s_tiles = s_all < w.w_first ? s_all : w.w_first;
+  const int end_tile = w.hi > 0 ? (w.hi + KT - 1) / KT : 0;
+  w.tiles = rows > 0 && end_tile > w.w_first ? w.s_tiles + end_tile - w.w_first : 0;
+  const int n = w.tiles;
+  // K and V tiles share the ring in the order K0, K1, V0, K2, V1, ..
+  auto idx_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
+  auto idx_v = [&](int j) { return j < n - 1 ? 2 * j + 2 : 2 * n - 1; };
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0 && n > 0) {
+      bool ok = true;
+      const int q_tiles = rows > kBM ? 2 : 1;
+      for (int t = 0; t < q_tiles; ++t) {
+        mbar_arrive_expect_tx(&st->q_full[t], C::kQBytes);
+        for (int s = 0; s < C::kSlabs; ++s)
+          tma_load_4d(smem + t * C::kQBytes + s * kBM * 128, &maps.q, &st->q_full[t], 64 * s, q0 + kBM * t, h * A.qh,
+                      b * A.qb);
+      }
+      int issued = 0;
+      auto load = [&](const CUtensorMap *map, int j, int ch, int cb) {
+        const int stage = issued % ST;
+        if (issued >= ST && !mbar_wait_bounded(&st->kv_empty[stage], ((issued / ST) - 1) & 1, abort, LLK_ERR_TIMEOUT,
+                                               kWaitLimitNs))
+          return false;
+        uint8_t *dst = smem_kv + stage * C::kStageBytes;
+        mbar_arrive_expect_tx(&st->kv_full[stage], C::kStageBytes);
+        for (int s = 0; s < C::kSlabs; ++s)
+          tma_load_4d(dst + s * KT * 128, map, &st->kv_full[stage], 64 * s, w.key0(j, KT), ch, cb);
+        ++issued;
+        return true;
+      };
+      ok = load(&maps.k, 0, hk * A.kh, b * A.kb);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) ok = load(&maps.k, j + 1, hk * A.kh, b * A.kb);
+        if (ok) ok = load(&maps.v, j, hk * A.vh, b * A.vb);
+      }
+      if (!ok) {
+        // the copies in flight land before the CTA's shared memory goes
+        int dummy = 0;
+        for (int t = 0; t < q_tiles; ++t) mbar_wait_bounded(&st->q_full[t], 0, &dummy, 1, 100000000ull);
+        for (int i = issued > ST ? issued - ST : 0; i < issued; ++i)
+          mbar_wait_bounded(&st->kv_full[i % ST], (i / ST) & 1, &dummy, 1, 100000000ull);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ----------------------------------------------------------------- MMA
+    // (the whole warp follows; lane 0 issues)
+    if (n > 0) {
+      const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem_kv);
+      constexpr uint32_t idesc_s = idesc_16(kBf16, kBM, KT, false), idesc_o = idesc_16(kBf16, kBM, D, true);
+      int cnt_s[2] = {0, 0}, cnt_o[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, int phase) {
+        const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+        ok = __all_sync(0xffffffffu, r);
+        tc_fence_after();
+        return ok;
+      };
+      auto scores = [&](int j) {
+        const int i = idx_k(j), k0 = w.key0(j, KT);
+        const uint32_t k_addr = kv_addr + (i % ST) * C::kStageBytes;
+        if (!wait(&st->kv_full[i % ST], i / ST)) return;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!w.active(t, k0, KT)) continue;
+          if (cnt_s[t] == 0 && !wait(&st->q_full[t], 0)) return;
+          if (cnt_s[t] > 0 && !wait(&st->s_empty[t], cnt_s[t] - 1)) return;
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk & 3) * 32;
+              tc_mma_bf16(tmem + C::kColS + t * KT,
+                          make_smem_desc_sw128(q_addr + t * C::kQBytes + (kk >> 2) * kBM * 128 + off, 16, 1024),
+                          make_smem_desc_sw128(k_addr + (kk >> 2) * KT * 128 + off, 16, 1024), idesc_s, kk > 0);
+            }
+            tc_commit(&st->s_full[t]);
+          }
+          ++cnt_s[t];
+        }
+        if (lane == 0) tc_commit(&st->kv_empty[i % ST]);
+      };
+      scores(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) scores(j + 1);
+        if (!ok) break;
+        const int i = idx_v(j), k0 = w.key0(j, KT);
+        const uint32_t v_addr = kv_addr + (i % ST) * C::kStageBytes;
+        if (!wait(&st->kv_full[i % ST], i / ST)) break;
+        // rows of V that no row of the CTA sees may hold anything: they become
+        // zero before the product (a weight of 0 does not undo a NaN)
+        if (k0 + KT > w.hi || (k0 < w.lo && k0 + KT > w.s_keys)) {
+          uint8_t *v = smem_kv + (i % ST) * C::kStageBytes;
+          for (int e = lane; e < KT * C::kSlabs * 8; e += 32) {
+            const int key = k0 + (e >> 3) % KT;
+            if (key >= w.hi || (key < w.lo && key >= w.s_keys))
+              *reinterpret_cast<uint4 *>(v + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || !w.active(t, k0, KT)) continue;
+          if (!wait(&st->p_ready[t], cnt_o[t])) continue;
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk)
+              mma_ts(tmem + C::kColO + t * D, tmem + C::kColP + t * (KT / 2) + kk * 8,
+                     make_smem_desc_sw128(v_addr + kk * 2048, KT * 128, 1024), idesc_o, cnt_o[t] > 0 || kk > 0);
+            tc_commit(&st->pv_done[t]);
+          }
+          ++cnt_o[t];
+        }
+        if (ok && lane == 0) tc_commit(&st->kv_empty[i % ST]);
+      }
+      // every MMA of this CTA has finished before TMEM is released
+      if (lane == 0) {
+        tc_commit(&st->mma_done);
+        int dummy = 0;
+        mbar_wait_bounded(&st->mma_done, 0, &dummy, 1, 100000000ull);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------- softmax
+    const int t = warp >> 2, quarter = warp & 3;
+    const int row_in = quarter * 32 + lane;
+    const int row = q0 + kBM * t + row_in, pos = w.p0 + kBM * t + row_in;
+    const int row_lo = window_lo(P.mask, pos);
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t ts = t_lane + C::kColS + t * KT, tp = t_lane + C::kColP + t * (KT / 2),
+                   to = t_lane + C::kColO + t * D;
+    const float sc = P.scale * kLog2e;
+    float m = -INFINITY;
+    uint64_t l2 = 0;  // two partial sums
+    int cnt = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, int phase) {
+      const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+      ok = __all_sync(0xffffffffu, r);
+      tc_fence_after();
+      return ok;
+    };
+    const int first = w.p0 + kBM * t;  // of the tile's rows that exist, the first and the last position
+    const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
+    const int last_lo = window_lo(P.mask, last);
+    for (int j = 0; j < n; ++j) {
+      const int k0 = w.key0(j, KT);
+      if (!w.active(t, k0, KT)) continue;
+      if (!wait(&st->s_full[t], cnt)) break;
+      uint32_t sb[KT];
+#pragma unroll
+      for (int c = 0; c < KT; c += 16)
+        tmem_ld_32x32b_x16(ts + c, *reinterpret_cast<uint32_t(*)[16]>(&sb[c]));
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&st->s_empty[t]);
+      float s[KT];
+#pragma unroll
+      for (int i = 0; i < KT; ++i) s[i] = __uint_as_float(sb[i]);
+      // every row of the tile sees every key of it, or the rows look key by key
+      const bool full = k0 + KT - 1 <= first && (k0 >= last_lo || k0 + KT <= w.sinks);
+      if (!full) {
+        const int hi_c = pos - k0, lo_c = row_lo - k0, s_c = w.sinks - k0;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+          if (i > hi_c || (i < lo_c && i >= s_c)) s[i] = -INFINITY;
+      }
+      float mx0 = s[0], mx1 = s[1];
+#pragma unroll
+      for (int i = 2; i < KT; i += 2) {
+        mx0 = fmaxf(mx0, s[i]);
+        mx1 = fmaxf(mx1, s[i + 1]);
+      }
+      const float top = fmaxf(mx0, mx1) * sc;  // scale > 0
+      float corr = 1.f;
+      bool move = false;
+      if (cnt == 0) {
+        m = top;
+      } else {
+        move = __any_sync(0xffffffffu, top > m + kSlack);
+        if (move) {
+          const float m_new = fmaxf(m, top);
+          corr = m_new == -INFINITY ? 1.f : exp2_approx(m - m_new);
+          m = m_new;
+          float a, c;
+          unpack_f32x2(l2, a, c);
+          l2 = pack_f32x2(a * corr, c * corr);
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      const uint64_t sc2 = pack_f32x2(sc, sc), ref2 = pack_f32x2(-ref, -ref);
+      uint32_t pk[KT / 2];
+#pragma unroll
+      for (int i = 0; i < KT; i += 2) {
+        float a, c;
+        unpack_f32x2(fma_f32x2(pack_f32x2(s[i], s[i + 1]), sc2, ref2), a, c);
+        a = exp2_approx(a);
+        c = exp2_approx(c);
+        l2 = add_f32x2(l2, pack_f32x2(a, c));
+        pk[i / 2] = pack16<kBf16>(a, c);
+      }
+      if (cnt > 0) {
+        // P's columns are free and O is whole
+        if (!wait(&st->pv_done[t], cnt - 1)) break;
+        if (move) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t x[16];
+            tmem_ld_32x32b_x16(to + c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
+            tmem_st_x8(to + c, x);
+            tmem_st_x8(to + c + 8, x + 8);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < KT / 2; c += 8) tmem_st_x8(tp + c, pk + c);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&st->p_ready[t]);
+      ++cnt;
+    }
+    // ------------------------------------------------------------- output
+    if (ok && cnt > 0) wait(&st->pv_done[t], cnt - 1);
+    if (ok && rows > kBM * t) {
+      using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+      float l0, l1;
+      unpack_f32x2(l2, l0, l1);
+      const float l = l0 + l1;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const bool mine = row < w.m;
+      T *orow = static_cast<T *>(P.o.p) + b * P.o.sb + h * P.o.sh + static_cast<int64_t>(row) * P.o.sl;
+      bool bad = false;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t x[32];
+        if (cnt > 0) {
+          tmem_ld_32x32b_x32(to + c, x);
+          tmem_ld_wait();
+        }
+        float y[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          y[i] = cnt > 0 ? __uint_as_float(x[i]) * inv : 0.f;
+          bad |= !(fabsf(y[i]) < INFINITY);
+        }
+        if (mine) {
+          if (A.vec_o && c + 32 <= P.D) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4 *>(orow + c + i) =
+                  make_uint4(pack16<kBf16>(y[i], y[i + 1]), pack16<kBf16>(y[i + 2], y[i + 3]),
+                             pack16<kBf16>(y[i + 4], y[i + 5]), pack16<kBf16>(y[i + 6], y[i + 7]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i < P.D) orow[c + i] = from_f32<T>(y[i]);
+          }
+        }
+      }
+      // a non-finite row: redone from the definition, by the whole warp
+      unsigned todo = __ballot_sync(0xffffffffu, mine && bad);
+      while (todo) {
+        const int r = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int rr = row - lane + r, pp = pos - lane + r;
+        __syncwarp();
+        attention_row<T>(static_cast<const T *>(P.q.p) + b * P.q.sb + h * P.q.sh + static_cast<int64_t>(rr) * P.q.sl,
+                         static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh,
+                         static_cast<const T *>(P.v.p) + b * P.v.sb + hk * P.v.sh,
+                         static_cast<T *>(P.o.p) + b * P.o.sb + h * P.o.sh + static_cast<int64_t>(rr) * P.o.sl, P.k.sl,
+                         P.v.sl, P.D, pp, window_lo(P.mask, pp), w.sinks, sc);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+  if (threadIdx.x == 0 && st->abort != 0) atomicExch(A.status, st->abort);
+}
+
+// {D, L, H, B} map of a view with a box of 64 x rows; a broadcast or size-1
+// dimension becomes one of size 1 (*f = 0: its coordinate is always 0).
+bool encode(PFN_cuTensorMapEncodeTiled_v12000 enc, CUtensorMap *map, bool bf16, const View4 &v, int64_t D, int64_t L,
+            int64_t H, int64_t B, int rows, int *fh, int *fb) {
+  *fh = H > 1 && v.sh != 0;
+  *fb = B > 1 && v.sb != 0;
+  const int64_t some = (D * 2 + 15) / 16 * 16;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(L), static_cast<cuuint64_t>(*fh ? H : 1),
+                        static_cast<cuuint64_t>(*fb ? B : 1)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(L > 1 ? v.sl * 2 : some),
+                           static_cast<cuuint64_t>(*fh ? v.sh * 2 : some),
+                           static_cast<cuuint64_t>(*fb ? v.sb * 2 : some)};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, es[4] = {1, 1, 1, 1};
+  return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, v.p, dims, strides, box,
+             es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool kBf16>
+cudaError_t launch_tc(PFN_cuTensorMapEncodeTiled_v12000 enc, const AttnProblem &p, int *status, cudaStream_t stream) {
+  using C = Cfg<D>;
+  TcMaps maps;
+  TcArgs a = {};
+  a.p = p;
+  a.q_blocks = (p.mask.Lq + 2 * kBM - 1) / (2 * kBM);
+  a.status = status;
+  a.vec_o = (reinterpret_cast<uintptr_t>(p.o.p) & 15) == 0 && p.o.sb % 8 == 0 && p.o.sh % 8 == 0 && p.o.sl % 8 == 0;
+  if (!encode(enc, &maps.q, kBf16, p.q, p.D, p.mask.Lq, p.H, p.B, kBM, &a.qh, &a.qb) ||
+      !encode(enc, &maps.k, kBf16, p.k, p.D, p.mask.Lk, p.Hkv, p.B, C::kKT, &a.kh, &a.kb) ||
+      !encode(enc, &maps.v, kBf16, p.v, p.D, p.mask.Lk, p.Hkv, p.B, C::kKT, &a.vh, &a.vb))
+    return cudaErrorInvalidValue;
+  const int smem = 2 * C::kQBytes + C::kStages * C::kStageBytes + static_cast<int>(sizeof(Tail)) + 1024;
+  auto kern = window_tc_kernel<D, kBf16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.q_blocks) * p.B * p.H));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, maps, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace
+
+// What TMA can describe: 16-bit rows on 16 bytes (a row's start needs it, D
+// a multiple of 8 with it), D <= 128; a scale that keeps the order of scores (and
+// -inf).
+bool window_tc_supported(const AttnProblem &p) {
+  const auto rows16 = [&](const View4 &v, int64_t L) {
+    return (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % 8 == 0 && v.sh % 8 == 0 && v.sl % 8 == 0 &&
+           (L <= 1 || v.sl > 0) && v.sl < (int64_t(1) << 38) && v.sh < (int64_t(1) << 38) && v.sb < (int64_t(1) << 38);
+  };
+  return (p.dtype == LLK_DTYPE_BF16 || p.dtype == LLK_DTYPE_FP16) && p.D % 8 == 0 && p.D <= 128 && p.mask.Lk > 0 &&
+         p.scale > 0.f && rows16(p.q, p.mask.Lq) && rows16(p.k, p.mask.Lk) && rows16(p.v, p.mask.Lk) &&
+         (static_cast<int64_t>(p.mask.Lq) + 255) / 256 * p.B * p.H <= INT32_MAX;
+}
+
+cudaError_t window_tc_launch(void *encode_fn, const AttnProblem &p, int *status, cudaStream_t stream) {
+  if (p.B == 0 || p.H == 0 || p.mask.Lq == 0) return cudaSuccess;
+  auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode_fn);
+  const bool bf16 = p.dtype == LLK_DTYPE_BF16;
+  if (p.D <= 64) return bf16 ? launch_tc<64, true>(enc, p, status, stream) : launch_tc<64, false>(enc, p, status, stream);
+  return bf16 ? launch_tc<128, true>(enc, p, status, stream) : launch_tc<128, false>(enc, p, status, stream);
+}
+
+}  // namespace llk_b200
