@@ -35,37 +35,37 @@ cudaError_t launch_bits(const Params &a, cudaStream_t stream) {
 bool split_supported(const AttnProblem &p, const KvPool *pool) {
   const int64_t g = p.Hkv > 0 ? p.H / p.Hkv : 0, rows = g * p.mask.Lq;
   if (p.dtype != LLK_DTYPE_BF16 && p.dtype != LLK_DTYPE_FP16) return false;
-  if (p.B > 65535 || (rows + 7) / 8 * p.Hkv > 65535) return false;
-  if (pool) return kv_pool_supported(*pool);
+  if (rows * p.Hkv > (int64_t(1) << 30) / (p.B > 0 ? p.B : 1)) return false;  // rows are counted in 32 bits
+  // so are the units of work, and the rows of a pool
+  if ((static_cast<int64_t>(p.mask.Lk) / kSpan + 1) * (p.B > 0 ? p.B : 1) >= (int64_t(1) << 31)) return false;
+  if (pool) return kv_pool_supported(*pool) && pool->num_pages <= 0xffffffffll / pool->Hkv / pool->page;
   const auto on16 = [](const View4 &v) {
     return (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % 8 == 0 && v.sh % 8 == 0 && v.sl % 8 == 0;
   };
   return (p.D == 64 || p.D == 80 || p.D == 96 || p.D == 128 || p.D == 256) && on16(p.k) && on16(p.v);
 }
 
-// As many splits as fill the GPU's resident CTAs once (4 a SM), but at least
-// two blocks of 16 tokens for every warp of a CTA.  The lengths are on the
-// device, so the plan goes by the most keys a sequence can have.
+// As many workers as the GPU holds at once, or as there can be units of work
+// when those are fewer (the lengths are on the device, so this goes by the
+// most keys a sequence can have).
 SplitPlan split_plan(const AttnProblem &p, const KvPool *pool, int sm_count) {
-  (void)pool;
   SplitPlan s;
   const int rows = p.H / p.Hkv * p.mask.Lq, nt = row_tiles(rows, p.D);
   s.row_blocks = (rows + 8 * nt - 1) / (8 * nt);
   int64_t keys = p.mask.Lk;
   if (p.mask.window > 0) {
-    const int64_t seen = static_cast<int64_t>(p.mask.window) + p.mask.Lq + p.mask.sinks;
+    // the window and the sinks, each with a block begun at either end
+    const int64_t seen = static_cast<int64_t>(p.mask.window) + p.mask.Lq + p.mask.sinks + 4 * kTok;
     if (seen < keys) keys = seen;
   }
-  const int64_t base = static_cast<int64_t>(p.B) * p.Hkv * s.row_blocks;
-  const int64_t room = 4 * static_cast<int64_t>(sm_count) / (base > 0 ? base : 1);
-  const int64_t most = (keys + 2 * kWarps * kTok - 1) / (2 * kWarps * kTok);
-  int64_t n = room < most ? room : most;
-  s.splits = static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
+  const int64_t segments = static_cast<int64_t>(p.B) * p.Hkv * s.row_blocks;
+  const int64_t units = segments * (keys > kSpan ? (keys + kSpan - 1) / kSpan : 1);
+  const int64_t room = static_cast<int64_t>(sm_count) *
+                       ctas_per_sm(pool ? pool->bits : 16, p.D, pool ? p.D / pool->group : 1, nt);
+  s.workers = static_cast<int>(units < room ? units : room);
   s.ws_bytes = 0;
-  if (s.splits > 1) {
-    const size_t cols = static_cast<size_t>(base) * s.splits * 8 * nt;
-    s.ws_bytes = cols * (static_cast<size_t>(p.D) * 4 + sizeof(float2));
-  }
+  if (units > segments)  // else no segment has more than one unit: none is cut
+    s.ws_bytes = 2 * static_cast<size_t>(s.workers) * 8 * nt * (static_cast<size_t>(p.D) * 4 + sizeof(float2));
   return s;
 }
 
@@ -77,12 +77,14 @@ cudaError_t split_launch(const AttnProblem &p, const KvPool *pool, const int *bl
   if (pool) a.pool = *pool;
   a.table = block_table;
   a.table_width = table_width;
-  a.splits = plan.splits;
+  a.workers = plan.workers;
   a.row_blocks = plan.row_blocks;
-  const int nt = row_tiles(p.H / p.Hkv * p.mask.Lq, p.D);
-  const size_t cols = static_cast<size_t>(p.B) * p.Hkv * plan.row_blocks * plan.splits * 8 * nt;
-  a.part_ml = static_cast<float2 *>(workspace);
-  a.part_o = reinterpret_cast<float *>(a.part_ml + cols);
+  a.q_vec = (reinterpret_cast<uintptr_t>(p.q.p) & 7) == 0 && p.q.sb % 4 == 0 && p.q.sh % 4 == 0 && p.q.sl % 4 == 0;
+  if (plan.ws_bytes) {
+    const int nt = row_tiles(p.H / p.Hkv * p.mask.Lq, p.D);
+    a.part_ml = static_cast<float2 *>(workspace);
+    a.part_o = reinterpret_cast<float *>(a.part_ml + 2 * static_cast<size_t>(plan.workers) * 8 * nt);
+  }
   if (!pool) return launch_dense(a, stream);
   return pool->bits == 4 ? launch_bits<4>(a, stream) : launch_bits<8>(a, stream);
 }

@@ -2,12 +2,14 @@
 // the keys: over the quantised paged cache (4 or 8 bits) and over dense 16-bit
 // keys and values.  Instantiated by kv_attention.cu and kv_attention_dense.cu.
 //
-// HBM-bound: every key and value byte is read once, from global memory
-// straight into the registers that feed mma.sync (m16n8k16, f32
-// accumulators).  The tensor cores only have to keep up with memory, not to
-// approach their peak, and registers as operands cost no shared-memory round
-// trip and no TMEM round trip for the softmax; so not tcgen05, whose operands
-// come from shared memory.
+// HBM-bound: every key and value byte is read once.  A warp works on blocks
+// of 16 tokens of its own: cp.async copies them into its ring of stages in
+// shared memory, several blocks ahead, and mma.sync (m16n8k16, f32
+// accumulators) takes them from registers.  No barrier but the warp's own
+// until the end.  The tensor cores only have to keep up with memory, not to
+// approach their peak, and operands in registers let the codes be unpacked on
+// the way and the softmax work on the accumulators where they are; tcgen05
+// would want unpacked operands back in shared memory.
 //
 //   S^T [tokens, rows] = K Q^T: A = 16 tokens of codes, B = 8 query rows;
 //   O^T [d, rows]     += V^T P^T: A = 16 elements x 16 tokens of codes.
@@ -35,20 +37,32 @@ namespace split_attn {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTok = 16;  // tokens of a block (one mma tile)
+constexpr int kTok = 16;      // tokens of a block (one mma tile)
+constexpr int kUnit = 8;      // blocks of a unit of work, which a CTA's warps share
+constexpr int kSpan = kUnit * kTok;
+// The reference of the softmax may lag the largest weight by up to this power
+// of two before the sums are rescaled: weights stay below 2^8, far inside f16.
+constexpr float kSlack = 8.f;
+// The reference before any token: below every score, and finite, so that a
+// masked score (-inf) less it is -inf.
+constexpr float kNoRef = -1e38f;
 
 struct Params {
   AttnProblem p;
   KvPool pool;
   const int *table;
   int64_t table_width;
-  int splits, row_blocks;
-  float *part_o;   // [B, Hkv, row_blocks, splits, 8 NT, D]
-  float2 *part_ml; // [B, Hkv, row_blocks, splits, 8 NT] (reference, sum)
+  int row_blocks;
+  int workers;      // CTAs that share the work
+  int q_vec;        // query rows start on 8 bytes
+  float *part_o;    // [2 workers, 8 NT, D]: a CTA's parts of its first and its last segment
+  float2 *part_ml;  // [2 workers, 8 NT] (reference, sum)
 };
 
 constexpr int cmin(int a, int b) { return a < b ? a : b; }
 constexpr int pow2_in(int n) { return n & -n; }
+template <int A, int B>
+constexpr int cmin_v = A < B ? A : B;
 
 // Geometry of one (BITS, D, group): which words of a row a lane holds.
 template <int BITS, int D, int G>
@@ -69,19 +83,57 @@ struct Geo {
   static constexpr int UR = UB < 4 ? 1 : UB / 4;  // registers a unit
   static constexpr int TILES = D / 16;            // 16-element tiles of O^T
   static constexpr int UT = TILES / NU;           // tiles a unit
+  // A warp's turn is HV blocks.  A stage of its ring, for each of them: 16
+  // rows of K, of V, then each token's (scale, min) of K and of V.
+  static constexpr int ROWB = D * BITS / 8, CPR = ROWB / 16;  // bytes, 16-byte chunks a row
+  static constexpr int PG = BITS == 16 ? 0 : 4 * G;           // bytes of a token's parameters, of K or V
+  static constexpr int HV = D * BITS <= 512 ? 2 : 1;
+  static constexpr int BLOCK = kTok * (2 * ROWB + 2 * PG);
+  static constexpr int STAGE = HV * BLOCK;
+  static constexpr int STAGES = STAGE <= 2560 ? 4 : 3;
 };
 
-template <int WORDS>
-__device__ __forceinline__ void ld_stream(const void *p, uint32_t *w) {
-  if constexpr (WORDS == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-        : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-        : "l"(p));
-  } else if constexpr (WORDS == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+// Row t of an mma tile's 16 slots holds token slot_token(t): the four lanes'
+// value tokens (slots 2c, 2c + 1) are of both parities then, which spreads
+// rows of 64 bytes over all banks.
+__host__ __device__ constexpr int slot_token(int t) { return t ^ ((t >> 1) & 1); }
+// Chunks of row (token) t are stored permuted, chunk ^ swizzle(t), so that the
+// key reads (two tokens' neighbouring chunks a quarter warp) and the value
+// reads (four tokens' two chunks) both meet all banks once.
+template <int CPR>
+__device__ __forceinline__ int swizzle(int t) {
+  if constexpr (CPR >= 8 && (CPR & (CPR - 1)) == 0) return ((t & 6) ^ ((t & 1) << 2));
+  if constexpr (CPR == 4) return (t >> 1) & 2;
+  return 0;
+}
+
+// N bytes from global to shared memory; without `in` zeros (nothing is read).
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src) {
+  if constexpr (N == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   } else {
-    asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
   }
+}
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+template <int WORDS>
+__device__ __forceinline__ void lds(uint32_t a, uint32_t *w) {
+  if constexpr (WORDS == 4) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+  } else if constexpr (WORDS == 2) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+  } else {
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a));
+  }
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
+  unsigned short x;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(a));
+  return x;
 }
 
 template <bool kBf16>
@@ -95,6 +147,21 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// The same onto zeros.
+template <bool kBf16>
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
   }
 }
 
@@ -124,12 +191,6 @@ __device__ __forceinline__ float2 unpack2(uint32_t r) {
   }
 }
 
-// One query element (q is bf16 or f16 in every instance).
-__device__ __forceinline__ float load_q(const void *q, int64_t at, int dtype) {
-  return dtype == LLK_DTYPE_FP16 ? __half2float(static_cast<const __half *>(q)[at])
-                                 : __bfloat162float(static_cast<const __nv_bfloat16 *>(q)[at]);
-}
-
 __device__ __forceinline__ void store_o(void *o, int64_t at, int dtype, float v) {
   if (dtype == LLK_DTYPE_FP16) {
     static_cast<__half *>(o)[at] = __float2half_rn(v);
@@ -145,11 +206,13 @@ struct Range {
   int p_first, p_last; // positions of the first and the last query
   int lo, s_end;       // keys seen: [0, s_end) and [lo, n)
   int nsb, wb0, blocks;
+  int full0, full1;    // blocks of which every query sees every token
 };
 
-__device__ __forceinline__ Range seq_range(const AttnMask &mk, int b) {
+__device__ __forceinline__ Range make_range(const AttnMask &mk, int n, int m) {
   Range r;
-  seq_lens(mk, b, r.n, r.m);
+  r.n = n;
+  r.m = m;
   r.p_first = r.n - r.m;
   r.p_last = r.n - 1;
   r.lo = window_lo(mk, r.p_first);
@@ -159,537 +222,725 @@ __device__ __forceinline__ Range seq_range(const AttnMask &mk, int b) {
   if (r.nsb > r.wb0) r.nsb = r.wb0;  // the sinks reach into the window's first block
   const int end = (r.n + kTok - 1) / kTok;
   r.blocks = r.m > 0 && end > r.wb0 ? r.nsb + end - r.wb0 : 0;
+  // (of the window's blocks; the sinks' are looked at token by token)
+  const int last_lo = window_lo(mk, r.p_last);
+  r.full0 = r.nsb + (last_lo + kTok - 1) / kTok - r.wb0;
+  r.full1 = r.nsb + (r.p_first + 1 > 0 ? (r.p_first + 1) / kTok : 0) - r.wb0;
   return r;
 }
+
+// ---- The work and its split.  A segment is a (sequence, key head, block of
+// query rows); its units are kSpan tokens each, at least one (a segment
+// without tokens still writes its zeros).  All units of the call, segment by
+// segment in the order (sequence, key head, row block), are dealt to the
+// workers in equal runs, whatever the lengths are: worker w has the units
+// [total w / workers, total (w + 1) / workers).  A segment that one worker has
+// whole is written by it; of one that is cut, each worker leaves its part in
+// its slot -- the first segment of its run in slot 2 w, else the last in
+// 2 w + 1 -- and combine_kernel joins them in order.
+__device__ __forceinline__ int seq_units(const AttnMask &mk, int b) {
+  int n, m;
+  seq_lens(mk, b, n, m);
+  const int blocks = make_range(mk, n, m).blocks;
+  return blocks > kUnit ? (blocks + kUnit - 1) / kUnit : 1;
+}
+
+// Units of the sequences before b0 (*before) and of all (returned), of one
+// segment each, by one warp.  (split_supported keeps both below 2^31.)
+__device__ __forceinline__ int count_units(const AttnMask &mk, int B, int b0, int *before) {
+  int all = 0, pre = 0;
+  for (int b = threadIdx.x & 31; b < B; b += 32) {
+    const int u = seq_units(mk, b);
+    all += u;
+    pre += b < b0 ? u : 0;
+  }
+  *before = __reduce_add_sync(0xffffffffu, pre);
+  return __reduce_add_sync(0xffffffffu, all);
+}
+
+// The sequence that holds unit `at` of the call (a sequence has per_seq
+// segments): *first = units before that sequence.  By one warp.
+__device__ __forceinline__ int find_seq(const AttnMask &mk, int B, int per_seq, int64_t at, int64_t *first) {
+  const int target = static_cast<int>(at / per_seq);  // in units of one segment a sequence
+  int base = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int b = b0 + (threadIdx.x & 31);
+    const int u = b < B ? seq_units(mk, b) : 0;
+    int inc = u;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, off);
+      if ((threadIdx.x & 31) >= off) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + inc > target);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      *first = static_cast<int64_t>(base + __shfl_sync(0xffffffffu, inc - u, l)) * per_seq;
+      return b0 + l;
+    }
+    base += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  *first = static_cast<int64_t>(base) * per_seq;
+  return B;
+}
+
+__device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) { return total * w / workers; }
+// The worker whose run holds unit u.
+__device__ __forceinline__ int worker_of(int64_t total, int workers, int64_t u) {
+  int w = static_cast<int>(u * workers / total);
+  while (run_begin(total, workers, w + 1) <= u) ++w;
+  while (run_begin(total, workers, w) > u) --w;
+  return w;
+}
+// Workers that take part: every one of them has at least one unit.
+__device__ __forceinline__ int active_workers(int64_t total, int workers) {
+  return total < workers ? static_cast<int>(total) : workers;
+}
+
 
 // Row R of a (sequence, key head): query R / g, head hk g + R % g.
 __device__ __forceinline__ int64_t row_at(const View4 &v, int b, int hk, int g, int R) {
   return b * v.sb + static_cast<int64_t>(hk * g + R % g) * v.sh + static_cast<int64_t>(R / g) * v.sl;
 }
 
-template <int BITS, int D, int G, bool kBf16, int NT, int SUB>
-__global__ void __launch_bounds__(kThreads) split_kernel(const Params A) {
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A block that does not exist, or whose page is not in the pool.
+constexpr uint32_t kNoBlock = 0xffffffffu;
+
+template <int BITS, int D, int G, bool kBf16, int NT, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_constant__ Params A) {
   using X = Geo<BITS, D, G>;
   constexpr int E = X::E, WK = X::WK, VW = X::VW, NU = X::NU, UR = X::UR, UT = X::UT;
   constexpr bool kQuant = BITS < 16;
   constexpr int KS = D / 16;  // k16 steps of a score
   constexpr int kLd = D + 4;
-  __shared__ float buf[8 * NT][kLd];
+  // the warps' rings, and at a segment's end [kWarps][8 NT][kLd] sums in their place
+  extern __shared__ __align__(128) uint8_t smem[];
+  float *buf = reinterpret_cast<float *>(smem);
   __shared__ float2 ml[kWarps][8 * NT];
 
   const AttnProblem &P = A.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int b = blockIdx.z, hk = blockIdx.y / A.row_blocks, rb = blockIdx.y % A.row_blocks, split = blockIdx.x;
-  const int g = P.H / P.Hkv;
+  const int g = P.H / P.Hkv, per_seq = P.Hkv * A.row_blocks;
   pdl_launch_dependents();
   pdl_wait();
-  const Range rg = seq_range(P.mask, b);
-  const int rows = g * rg.m, row0 = rb * 8 * NT;
-  if (row0 >= rows) return;  // no query here: nothing is written, nothing is combined
+  int none;
+  const int64_t total = static_cast<int64_t>(count_units(P.mask, P.B, 0, &none)) * per_seq;
+  const int workers = active_workers(total, A.workers);
+  if (static_cast<int>(blockIdx.x) >= workers) return;
+  int64_t at = run_begin(total, workers, blockIdx.x);
+  const int64_t run0 = at, run1 = run_begin(total, workers, blockIdx.x + 1);
+  int64_t seq0;
+  int b = find_seq(P.mask, P.B, per_seq, at, &seq0);
 
-  // ---- queries: B operands, per-column factors and sums
-  uint32_t qf[NT][KS][2];
-  float fcol[NT][2], mq[NT][kQuant ? G : 1][2];
+  // ---- segment by segment
+  while (at < run1) {
+    int n, m;
+    seq_lens(P.mask, b, n, m);
+    const Range rg = make_range(P.mask, n, m);
+    const int units = rg.blocks > kUnit ? (rg.blocks + kUnit - 1) / kUnit : 1;
+    const int seg = static_cast<int>((at - seq0) / units);
+    const int64_t seg0 = seq0 + static_cast<int64_t>(seg) * units;
+    const int hk = seg / A.row_blocks, rb = seg - hk * A.row_blocks;
+    const int u0 = static_cast<int>(at - seg0);
+    const int u1 = static_cast<int>((run1 - seg0 < units ? run1 - seg0 : units));
+    const int rows = g * rg.m, row0 = rb * 8 * NT;
+    at = seg0 + u1;
+    const int b_now = b;
+    if (seg + 1 == per_seq && u1 == units) {
+      seq0 = at;
+      ++b;
+    }
+    if (row0 >= rows) continue;  // rows behind the sequence's queries: nothing is written
+
+    // ---- queries: B operands, per-column factors and sums
+    uint32_t qf[NT][KS][2];
+    float fcol[NT][2], mq[NT][kQuant ? G : 1][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int R = row0 + 8 * nt + r;
-    const bool in = R < rows;
-    const int64_t at = in ? row_at(P.q, b, hk, g, R) : 0;
-    auto elem = [&](int e) { return in ? load_q(P.q.p, at + e, P.dtype) : 0.f; };
-    float up = 1.f;
-    if constexpr (kQuant) {
-      // q times a power of two into f16: exact down to 2^-24 of the row's
-      // largest element, and 2^-35 of that below
-      float top = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int R = row0 + 8 * nt + r;
+      const bool in = R < rows;
+      const uint16_t *q = static_cast<const uint16_t *>(P.q.p) + (in ? row_at(P.q, b_now, hk, g, R) : 0);
+      uint32_t raw[WK * E / 2];  // this lane's elements, two a word
 #pragma unroll
-      for (int w = 0; w < WK; ++w)
+      for (int i = 0; i < WK * E / 2; ++i) raw[i] = 0;
+      if (in) {
+        if (A.q_vec) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(elem(E * ((w / VW) * 4 * VW + c * VW + w % VW) + e)));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // floor(log2 top)
-      const int k = top > 0.f && ex < 128 ? 9 - ex : 0;
-      up = k > 126 ? 0x1p126f : __uint_as_float(static_cast<uint32_t>(127 + (k < -126 ? -126 : k)) << 23);
-      float sum[G];
-#pragma unroll
-      for (int i = 0; i < G; ++i) sum[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const int word = (w / VW) * 4 * VW + c * VW + w % VW;
-        float x[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          x[e] = elem(E * word + e);
-          sum[(w / VW) * 4 * VW * E / X::GROUP] += x[e];
-          x[e] *= up;
-        }
-        if constexpr (BITS == 4) {
-          qf[nt][2 * w][0] = pack2<false>(x[0], x[4]);
-          qf[nt][2 * w][1] = pack2<false>(x[1] * 0.0625f, x[5] * 0.0625f);
-          qf[nt][2 * w + 1][0] = pack2<false>(x[2], x[6]);
-          qf[nt][2 * w + 1][1] = pack2<false>(x[3] * 0.0625f, x[7] * 0.0625f);
+          for (int i = 0; i < WK * E / 4; ++i) {
+            const int u = 4 * i / (VW * E);
+            const uint2 x = *reinterpret_cast<const uint2 *>(q + E * c * VW + 3 * u * VW * E + 4 * i);
+            raw[2 * i] = x.x;
+            raw[2 * i + 1] = x.y;
+          }
         } else {
-          qf[nt][w][0] = pack2<false>(x[0], x[2]);
-          qf[nt][w][1] = pack2<false>(x[1], x[3]);
+#pragma unroll
+          for (int i = 0; i < WK * E / 2; ++i) {
+            const uint16_t *src = q + E * c * VW + 3 * (2 * i / (VW * E)) * VW * E + 2 * i;
+            raw[i] = src[0] | static_cast<uint32_t>(src[1]) << 16;
+          }
         }
       }
+      float up = 1.f;
+      if constexpr (kQuant) {
+        float x[WK * E];
+        if (P.dtype == LLK_DTYPE_FP16) {
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        sum[i] *= P.scale * kLog2e;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) mq[nt][i][j] = __shfl_sync(0xffffffffu, sum[i], 4 * (2 * c + j));
-      }
-    } else {
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const int word = (w / VW) * 4 * VW + c * VW + w % VW;
-        qf[nt][w / 2][w % 2] = pack2<kBf16>(elem(2 * word), elem(2 * word + 1));
-      }
-      mq[nt][0][0] = mq[nt][0][1] = 0.f;
-    }
-    const float f = P.scale * kLog2e * (kQuant ? 0x1p24f / up : 1.f);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) fcol[nt][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + j));
-  }
-  // the two columns of this lane in a score tile: rows row0 + 8 nt + 2 c + j
-  int pcol[NT][2], wlo[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int R = row0 + 8 * nt + 2 * c + j;
-      pcol[nt][j] = R < rows ? rg.p_first + R / g : -1;
-      wlo[nt][j] = window_lo(P.mask, pcol[nt][j]);
-    }
-
-  // ---- this warp's blocks of the split's [beg, end)
-  const int beg = static_cast<int>(static_cast<int64_t>(rg.blocks) * split / A.splits);
-  const int end = static_cast<int>(static_cast<int64_t>(rg.blocks) * (split + 1) / A.splits);
-  auto token0 = [&](int blk) { return (blk < rg.nsb ? blk : rg.wb0 + blk - rg.nsb) * kTok; };
-  // row of the block's first token (in rows of a head), or -1: no such block, or a page that is not in the pool
-  auto block_row = [&](int blk) -> int64_t {
-    if (blk >= end) return -1;
-    const int t0 = token0(blk);
-    if constexpr (kQuant) {
-      const int page = t0 / A.pool.page;
-      const int entry = A.table[b * A.table_width + page];
-      if (entry < 0 || entry >= A.pool.num_pages) return -1;
-      return (static_cast<int64_t>(entry) * P.Hkv + hk) * A.pool.page + (t0 - page * A.pool.page);
-    } else {
-      return t0;
-    }
-  };
-  const char *kbase, *vbase;
-  int64_t k_sl, v_sl;  // bytes between tokens
-  if constexpr (kQuant) {
-    kbase = static_cast<const char *>(A.pool.k_codes);
-    vbase = static_cast<const char *>(A.pool.v_codes);
-    k_sl = v_sl = D * BITS / 8;
-  } else {
-    kbase = static_cast<const char *>(P.k.p) + 2 * (b * P.k.sb + hk * P.k.sh);
-    vbase = static_cast<const char *>(P.v.p) + 2 * (b * P.v.sb + hk * P.v.sh);
-    k_sl = 2 * P.k.sl;
-    v_sl = 2 * P.v.sl;
-  }
-  // a token that no query of the sequence sees is not read: what lies there may be anything
-  auto seen = [&](int t) { return t < rg.n && (t >= rg.lo || t < rg.s_end); };
-
-  uint32_t kw[SUB][2][WK], vw[SUB][4][NU * UR], kp[SUB][2][kQuant ? G : 1], vp[SUB][2][kQuant ? G : 1];
-  auto load_params = [&](const void *params, int64_t row, bool ok, uint32_t (&w)[kQuant ? G : 1]) {
-    if constexpr (kQuant) {
-#pragma unroll
-      for (int i = 0; i < G; ++i) w[i] = 0;
-      if (ok) {
-        const uint32_t *src = static_cast<const uint32_t *>(params) + row * G;
-        if constexpr (G >= 4) {
-#pragma unroll
-          for (int i = 0; i < G; i += 4) ld_stream<4>(src + i, w + i);
+          for (int i = 0; i < WK * E / 2; ++i) {
+            const float2 y = unpack2<false>(raw[i]);
+            x[2 * i] = y.x;
+            x[2 * i + 1] = y.y;
+          }
         } else {
-          ld_stream<G>(src, w);
+#pragma unroll
+          for (int i = 0; i < WK * E / 2; ++i) {
+            const float2 y = unpack2<true>(raw[i]);
+            x[2 * i] = y.x;
+            x[2 * i + 1] = y.y;
+          }
         }
-      }
-    }
-  };
-  auto load_k = [&](int s, int t0, int64_t row) {
+        // q times a power of two into f16: exact down to 2^-24 of the row's
+        // largest element, and 2^-35 of that below
+        float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = r + 8 * i;
-      const bool ok = row >= 0 && seen(t0 + t);
-      const char *src = kbase + (row + t) * k_sl;
+        for (int i = 0; i < WK * E; ++i) top = fmaxf(top, fabsf(x[i]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // floor(log2 top)
+        const int k = top > 0.f && ex < 128 ? 9 - ex : 0;
+        up = k > 126 ? 0x1p126f : __uint_as_float(static_cast<uint32_t>(127 + (k < -126 ? -126 : k)) << 23);
+        float sum[G];
 #pragma unroll
-      for (int u = 0; u < X::CHUNKS; ++u) {
+        for (int i = 0; i < G; ++i) sum[i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < VW; ++w) kw[s][i][u * VW + w] = 0;
-        if (ok) ld_stream<VW>(src + 4 * (u * 4 * VW + c * VW), &kw[s][i][u * VW]);
-      }
-      load_params(A.pool.k_params, row + t, ok, kp[s][i]);
-    }
-  };
-  auto load_v = [&](int s, int t0, int64_t row) {
+        for (int w = 0; w < WK; ++w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 2 * c + (i & 1) + 8 * (i >> 1);
-      const bool ok = row >= 0 && seen(t0 + t);
-      const char *src = vbase + (row + t) * v_sl;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-#pragma unroll
-        for (int w = 0; w < UR; ++w) vw[s][i][u * UR + w] = 0;
-        if (ok) {
-          if constexpr (X::UB == 2) {
-            unsigned short x;
-            asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(x) : "l"(src + (u * 8 + r) * 2));
-            vw[s][i][u] = x;
+          for (int e = 0; e < E; ++e) {
+            x[w * E + e] *= up;
+            sum[(w / VW) * 4 * VW * E / X::GROUP] += x[w * E + e];
+          }
+          const float *y = x + w * E;
+          if constexpr (BITS == 4) {
+            qf[nt][2 * w][0] = pack2<false>(y[0], y[4]);
+            qf[nt][2 * w][1] = pack2<false>(y[1] * 0.0625f, y[5] * 0.0625f);
+            qf[nt][2 * w + 1][0] = pack2<false>(y[2], y[6]);
+            qf[nt][2 * w + 1][1] = pack2<false>(y[3] * 0.0625f, y[7] * 0.0625f);
           } else {
-            ld_stream<UR>(src + (u * 8 + r) * X::UB, &vw[s][i][u * UR]);
+            qf[nt][w][0] = pack2<false>(y[0], y[2]);
+            qf[nt][w][1] = pack2<false>(y[1], y[3]);
           }
         }
+        // the sums in the units of the tensor core's scores, 2^-24 up
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+          sum[i] *= 0x1p-24f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mq[nt][i][j] = __shfl_sync(0xffffffffu, sum[i], 4 * (2 * c + j));
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < WK; ++w) qf[nt][w / 2][w % 2] = raw[w];
+        mq[nt][0][0] = mq[nt][0][1] = 0.f;
       }
-    }
+      const float f = P.scale * kLog2e * (kQuant ? 0x1p24f / up : 1.f);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      load_params(A.pool.v_params, row + r + 8 * i, row >= 0 && seen(t0 + r + 8 * i), vp[s][i]);
-  };
-
-  float acc[X::TILES][NT][4], mrun[NT][2], l[NT][2], pm[NT][kQuant ? G : 1][2];
-#pragma unroll
-  for (int t = 0; t < X::TILES; ++t)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.f;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      mrun[nt][j] = -INFINITY;
-      l[nt][j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < (kQuant ? G : 1); ++i) pm[nt][i][j] = 0.f;
+      for (int j = 0; j < 2; ++j) fcol[nt][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + j));
     }
 
-  int blk = beg + warp * SUB;
-  int64_t row_now[SUB], row_next[SUB];
+    // ---- this warp's blocks of the segment's units [u0, u1)
+    const int beg = u0 * kUnit, end = u1 * kUnit < rg.blocks ? u1 * kUnit : rg.blocks;
+    auto token0 = [&](int blk) { return (blk < rg.nsb ? blk : rg.wb0 + blk - rg.nsb) * kTok; };
+    // row of a block's first token among the rows of the pool (dense: of the head)
+    auto look = [&](int blk) -> uint32_t {
+      if (blk >= end) return kNoBlock;
+      const int t0 = token0(blk);
+      if constexpr (kQuant) {
+        const int page = t0 / A.pool.page;
+        const int entry = A.table[b_now * A.table_width + page];
+        if (entry < 0 || entry >= A.pool.num_pages) return kNoBlock;
+        return (static_cast<uint32_t>(entry) * P.Hkv + hk) * A.pool.page + (t0 - page * A.pool.page);
+      } else {
+        return t0;
+      }
+    };
+    // lane i looks at the i-th of the warp's next 32 blocks
+    constexpr int HV = X::HV, kTurns = 32 / HV, kStep = kWarps * HV;
+    const int first = beg + warp * HV;
+    auto look_ahead = [&](int turn) { return look(first + (turn + lane / HV) * kStep + lane % HV); };
+    uint32_t rows_now = look_ahead(0), rows_next = look_ahead(kTurns);
+
+    const char *kbase, *vbase;
+    int64_t k_sl, v_sl;  // bytes between tokens
+    if constexpr (kQuant) {
+      kbase = static_cast<const char *>(A.pool.k_codes);
+      vbase = static_cast<const char *>(A.pool.v_codes);
+      k_sl = v_sl = X::ROWB;
+    } else {
+      kbase = static_cast<const char *>(P.k.p) + 2 * (b_now * P.k.sb + hk * P.k.sh);
+      vbase = static_cast<const char *>(P.v.p) + 2 * (b_now * P.v.sb + hk * P.v.sh);
+      k_sl = 2 * P.k.sl;
+      v_sl = 2 * P.v.sl;
+    }
+    // a token that no query of the sequence sees is not read: what lies there may be anything
+    auto seen = [&](int t) { return t < rg.n && (t >= rg.lo || t < rg.s_end); };
+    const uint32_t ring = smem_u32(smem) + warp * X::STAGES * X::STAGE;
+    constexpr int kPer = kTok * X::CPR / 32;  // chunks of K (of V) a lane
+    static_assert(kTok * X::CPR % 32 == 0, "whole chunks a lane");
+    // chunk i of this lane: token (lane + 32 i) / CPR, its place in the stage
+    uint32_t put[kPer];
 #pragma unroll
-  for (int s = 0; s < SUB; ++s) {
-    row_now[s] = block_row(blk + s);
-    load_k(s, token0(blk + s), row_now[s]);
-    load_v(s, token0(blk + s), row_now[s]);
-    row_next[s] = block_row(blk + kWarps * SUB + s);
-  }
-  for (; blk < end; blk += kWarps * SUB) {
-    const int nxt = blk + kWarps * SUB;
-    // ---- scores (times log2 e) of this lane's tokens r, r + 8 and its two columns
-    float s2[SUB][NT][4], sv[SUB][2][kQuant ? G : 1], mv[SUB][2][kQuant ? G : 1];
+    for (int i = 0; i < kPer; ++i) {
+      const int e = lane + 32 * i, t = e / X::CPR;
+      put[i] = t * X::ROWB + (((e % X::CPR) ^ swizzle<X::CPR>(t)) << 4);
+    }
+    const char *psrc = static_cast<const char *>(lane < 16 ? A.pool.k_params : A.pool.v_params) + (lane & 15) * X::PG;
+    const uint32_t pput = 2 * kTok * X::ROWB + (lane & 15) * 2 * X::PG + (lane >> 4) * X::PG;
+    // a block into its place of a stage; tokens that are not read become zeros
+    // (of kNoBlock nothing is used: codes are finite whatever lies in the stage)
+    auto load = [&](uint32_t dst, int blk, uint32_t row) {
+      if (row == kNoBlock) return;
+      if (blk >= rg.full0 && blk < rg.full1) {
+        if constexpr (kQuant) {
+          const int64_t o = static_cast<int64_t>(row) * X::ROWB + lane * 16;
+          const char *ks = kbase + o, *vs = vbase + o;
 #pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      float t[NT][4], um[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[nt][i] = um[nt][i] = 0.f;
-      float cg[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cg[nt][i] = 0.f;
-      constexpr int kWordsAStep = BITS == 16 ? 2 : 1;
-#pragma unroll
-      for (int w = 0; w < WK; w += kWordsAStep) {
-        const uint32_t x = kw[s][0][w], y = kw[s][1][w];
-        if constexpr (BITS == 4) {
-          const uint32_t xs = x >> 8, ys = y >> 8;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<false>(cg[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u,
-                            qf[nt][2 * w][0], qf[nt][2 * w][1]);
-            mma16816<false>(cg[nt], xs & 0x000f000fu, ys & 0x000f000fu, xs & 0x00f000f0u, ys & 0x00f000f0u,
-                            qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+          for (int i = 0; i < kPer; ++i) {
+            cp_async<16>(dst + put[i], ks + 512 * i);
+            cp_async<16>(dst + put[i] + kTok * X::ROWB, vs + 512 * i);
           }
-        } else if constexpr (BITS == 8) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816<false>(cg[nt], x & 0x00ff00ffu, y & 0x00ff00ffu, (x >> 8) & 0x00ff00ffu, (y >> 8) & 0x00ff00ffu,
-                            qf[nt][w][0], qf[nt][w][1]);
         } else {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816<kBf16>(cg[nt], x, y, kw[s][0][w + 1], kw[s][1][w + 1], qf[nt][w / 2][0], qf[nt][w / 2][1]);
-        }
-        if constexpr (kQuant) {
-          // the group's last word: fold its sum in
-          const int gi = (w / VW) * 4 * VW * E / X::GROUP;
-          const bool ends = w + 1 == WK || ((w + 1) / VW) * 4 * VW * E / X::GROUP != gi;
-          if (ends) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t pw = kp[s][i >> 1][gi];
-              const float sc = __uint_as_float(pw << 16), mn = __uint_as_float(pw & 0xffff0000u);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                t[nt][i] = fmaf(sc, cg[nt][i], t[nt][i]);
-                um[nt][i] = fmaf(mn, mq[nt][gi][i & 1], um[nt][i]);
-                cg[nt][i] = 0.f;
-              }
-            }
+          for (int i = 0; i < kPer; ++i) {
+            const int64_t t = row + (lane + 32 * i) / X::CPR;
+            const int ch = (lane + 32 * i) % X::CPR;
+            cp_async<16>(dst + put[i], kbase + t * k_sl + 16 * ch);
+            cp_async<16>(dst + put[i] + kTok * X::ROWB, vbase + t * v_sl + 16 * ch);
           }
         }
+      } else {
+        const int t0 = token0(blk);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int e = lane + 32 * i, t = e / X::CPR, ch = e % X::CPR;
+          const bool in = seen(t0 + t);
+          const int64_t at_row = static_cast<int64_t>(row) + t;
+          cp_async16_if(dst + put[i], in ? kbase + at_row * k_sl + 16 * ch : kbase, in);
+          cp_async16_if(dst + put[i] + kTok * X::ROWB, in ? vbase + at_row * v_sl + 16 * ch : vbase, in);
+        }
       }
+      if constexpr (kQuant) {
+        // (a page is in the pool whole; what is not seen is masked when it is used)
+        const char *src = psrc + static_cast<int64_t>(row) * X::PG;
+#pragma unroll
+        for (int i = 0; i < X::PG; i += 16) cp_async<cmin_v<X::PG, 16>>(dst + pput + i, src + i);
+      }
+    };
+
+    float acc[X::TILES][NT][4], mrun[NT][2], l[NT][2], pm[NT][kQuant ? G : 1][2];
+#pragma unroll
+    for (int t = 0; t < X::TILES; ++t)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s2[s][nt][i] = kQuant ? fmaf(t[nt][i], fcol[nt][i & 1], um[nt][i]) : cg[nt][i] * fcol[nt][i & 1];
-      // masks: only blocks at an edge of some row's range compare token by token
-      const int t0 = token0(blk + s), t1 = t0 + kTok - 1;
-      const bool none = row_now[s] < 0;
-      const bool full = !none && t1 <= rg.p_first && t1 < rg.n &&
-                        (P.mask.window == 0 || t0 >= window_lo(P.mask, rg.p_last) || t1 < P.mask.sinks);
-      if (!full) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (none || !key_visible(t0 + r + 8 * (i >> 1), pcol[nt][i & 1], wlo[nt][i & 1], P.mask.sinks))
-              s2[s][nt][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int gi = 0; gi < (kQuant ? G : 1); ++gi) {
-          sv[s][i][gi] = kQuant ? __uint_as_float(vp[s][i][gi] << 16) : 1.f;
-          mv[s][i][gi] = kQuant ? __uint_as_float(vp[s][i][gi] & 0xffff0000u) : 0.f;
-        }
-    }
-    // the K registers are free: the next blocks' keys load while this one's softmax and values run
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) load_k(s, token0(nxt + s), row_next[s]);
-
-    // ---- softmax: reference = max (score + log2 of the values' scale)
-    float lg[SUB][2];
-#pragma unroll
-    for (int s = 0; s < SUB; ++s)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        lg[s][i] = 0.f;
-        if constexpr (kQuant) {
-          float mx = sv[s][i][0];
-#pragma unroll
-          for (int gi = 1; gi < G; ++gi) mx = fmaxf(mx, sv[s][i][gi]);
-          lg[s][i] = __log2f(mx);
-        }
-      }
-    bool grew = false;
-    float mnew[NT][2];
+        for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float mx = -INFINITY;
+        mrun[nt][j] = kNoRef;
+        l[nt][j] = 0.f;
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) mx = fmaxf(mx, s2[s][nt][2 * i + j] + lg[s][i]);
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        mnew[nt][j] = fmaxf(mrun[nt][j], mx);
-        grew |= mnew[nt][j] > mrun[nt][j];
+        for (int i = 0; i < (kQuant ? G : 1); ++i) pm[nt][i][j] = 0.f;
       }
-    if (__any_sync(0xffffffffu, grew)) {
+
+    const int tr = slot_token(r), tv = slot_token(2 * c);
+    uint32_t none = 0;  // blocks in the ring that do not exist, HV bits a turn, the latest lowest
+    auto load_turn = [&](uint32_t dst, int blk, int turn) {
+#pragma unroll
+      for (int hv = 0; hv < HV; ++hv) {
+        const int at_lane = turn * HV + hv;
+        const uint32_t row = __shfl_sync(0xffffffffu, at_lane < 32 ? rows_now : rows_next, at_lane & 31);
+        load(dst + hv * X::BLOCK, blk + hv, row);
+        none = none << 1 | (row == kNoBlock ? 1u : 0u);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < X::STAGES - 1; ++i) load_turn(ring + i * X::STAGE, first + i * kStep, i);
+    uint32_t at_use = ring, at_load = ring + (X::STAGES - 1) * X::STAGE;
+    const uint32_t ring_end = ring + X::STAGES * X::STAGE;
+    int turn = 0;  // of the 32 rows in rows_now
+    for (int blk = first; blk < end; blk += kStep) {
+      // the turn STAGES - 1 ahead goes where the last one was (all lanes have read it); then this one is waited for
+      __syncwarp();
+      load_turn(at_load, blk + (X::STAGES - 1) * kStep, turn + X::STAGES - 1);
+      at_load = at_load + X::STAGE == ring_end ? ring : at_load + X::STAGE;
+      asm volatile("cp.async.wait_group %0;" ::"n"(X::STAGES - 1) : "memory");
+      __syncwarp();
+      if (++turn == kTurns) {
+        turn = 0;
+        rows_now = rows_next;
+        rows_next = look_ahead((blk - first) / kStep + 1 + kTurns);
+      }
+      const uint32_t absent = none >> ((X::STAGES - 1) * HV);
+      const bool full = blk >= rg.full0 && blk + HV <= rg.full1 && (absent & ((1u << HV) - 1)) == 0;
+      float z[HV][NT][4], sr[HV][2][kQuant ? G : 1], mr[HV][2][kQuant ? G : 1], rs[HV][2];
+#pragma unroll
+      for (int hv = 0; hv < HV; ++hv) {
+        const uint32_t stage = at_use + hv * X::BLOCK;
+        uint32_t kw[2][WK], par[2][kQuant ? 2 * G : 1];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int u = 0; u < X::CHUNKS; ++u)
+            lds<VW>(stage + (tr + 8 * i) * X::ROWB + ((u * 16 * VW + c * 4 * VW) ^ (swizzle<X::CPR>(tr) << 4)),
+                    &kw[i][u * VW]);
+          if constexpr (kQuant) {
+#pragma unroll
+            for (int w = 0; w < 2 * G; w += cmin_v<2 * G, 4>)
+              lds<cmin_v<2 * G, 4>>(stage + 2 * kTok * X::ROWB + (tr + 8 * i) * 2 * X::PG + 4 * w, &par[i][w]);
+          }
+        }
+        if constexpr (kQuant) {
+          if (!full) {
+            // parameters of tokens that no query sees may be anything: here scale 1, min 0
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const bool in = !(absent >> (HV - 1 - hv) & 1) && seen(token0(blk + hv) + tr + 8 * i);
+#pragma unroll
+              for (int w = 0; w < 2 * G; ++w) par[i][w] = in ? par[i][w] : 0x3f80u;
+            }
+          }
+        }
+        // ---- scores of this lane's tokens (slots r, r + 8) and its two columns, in the tensor core's units
+        float s2[NT][4], cg[NT][4];
+        constexpr int kWordsAStep = BITS == 16 ? 2 : 1;
+#pragma unroll
+        for (int w = 0; w < WK; w += kWordsAStep) {
+          const uint32_t x = kw[0][w], y = kw[1][w];
+          const int gi = kQuant ? (w / VW) * 4 * VW * E / X::GROUP : 0;
+          // the first and the last word of a group
+          const bool starts = w == 0 || (kQuant && ((w - 1) / VW) * 4 * VW * E / X::GROUP != gi);
+          const bool ends = kQuant && (w + 1 == WK || ((w + 1) / VW) * 4 * VW * E / X::GROUP != gi);
+          if constexpr (BITS == 4) {
+            const uint32_t xs = x >> 8, ys = y >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (starts) {
+                mma16816_zero<false>(cg[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u,
+                                     qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              } else {
+                mma16816<false>(cg[nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u,
+                                qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              }
+              mma16816<false>(cg[nt], xs & 0x000f000fu, ys & 0x000f000fu, xs & 0x00f000f0u, ys & 0x00f000f0u,
+                              qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+            }
+          } else if constexpr (BITS == 8) {
+            const uint32_t a0 = x & 0x00ff00ffu, a1 = y & 0x00ff00ffu, a2 = (x >> 8) & 0x00ff00ffu,
+                           a3 = (y >> 8) & 0x00ff00ffu;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (starts) {
+                mma16816_zero<false>(cg[nt], a0, a1, a2, a3, qf[nt][w][0], qf[nt][w][1]);
+              } else {
+                mma16816<false>(cg[nt], a0, a1, a2, a3, qf[nt][w][0], qf[nt][w][1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (starts) {
+                mma16816_zero<kBf16>(cg[nt], x, y, kw[0][w + 1], kw[1][w + 1], qf[nt][w / 2][0], qf[nt][w / 2][1]);
+              } else {
+                mma16816<kBf16>(cg[nt], x, y, kw[0][w + 1], kw[1][w + 1], qf[nt][w / 2][0], qf[nt][w / 2][1]);
+              }
+            }
+          }
+          if (ends) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t pw = par[i >> 1][gi];
+              const float sc = __uint_as_float(pw << 16), mn = __uint_as_float(pw & 0xffff0000u);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const float um = gi == 0 ? mn * mq[nt][gi][i & 1] : fmaf(mn, mq[nt][gi][i & 1], s2[nt][i]);
+                s2[nt][i] = fmaf(sc, cg[nt][i], um);
+              }
+            }
+          }
+        }
+        if constexpr (!kQuant) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2[nt][i] = cg[nt][i];
+        }
+        // ---- z = log2 of the weight p s_v; a token's p, its p min_v and its p s_v of a group follow from the weight by
+        // factors of the token
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float lg = 0.f;
+          rs[hv][i] = 1.f;
+          if constexpr (kQuant) {
+            float mx = 0.f;
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+              sr[hv][i][gi] = __uint_as_float(par[i][G + gi] << 16);
+              mx = gi == 0 ? sr[hv][i][gi] : fmaxf(mx, sr[hv][i][gi]);
+            }
+            lg = lg2_approx(mx);
+            rs[hv][i] = rcp_approx(mx);
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+              if constexpr (G > 1) sr[hv][i][gi] *= rs[hv][i];
+              mr[hv][i][gi] = __uint_as_float(par[i][G + gi] & 0xffff0000u) * rs[hv][i];
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) z[hv][nt][2 * i + j] = fmaf(s2[nt][2 * i + j], fcol[nt][j], lg);
+        }
+        // masks: only turns at an edge of some row's range compare token by token
+        if (!full) {
+          const int t0 = token0(blk + hv);
+          const bool gone = absent >> (HV - 1 - hv) & 1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int R = row0 + 8 * nt + 2 * c + (i & 1), p = R < rows ? rg.p_first + R / g : -1;
+              if (gone || !key_visible(t0 + tr + 8 * (i >> 1), p, window_lo(P.mask, p), P.mask.sinks))
+                z[hv][nt][i] = -INFINITY;
+            }
+        }
+      }
+      // ---- the reference, when some weight is far above it
+      bool grew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float corr = mrun[nt][j] == -INFINITY ? 0.f : exp2_approx(mrun[nt][j] - mnew[nt][j]);
-          mrun[nt][j] = mnew[nt][j];
-          l[nt][j] *= corr;
-#pragma unroll
-          for (int gi = 0; gi < (kQuant ? G : 1); ++gi) pm[nt][gi][j] *= corr;
-#pragma unroll
-          for (int t = 0; t < X::TILES; ++t) {
-            acc[t][nt][j] *= corr;
-            acc[t][nt][2 + j] *= corr;
-          }
+          float mx = fmaxf(z[0][nt][j], z[0][nt][2 + j]);
+          if constexpr (HV == 2) mx = fmaxf(mx, fmaxf(z[HV - 1][nt][j], z[HV - 1][nt][2 + j]));
+          grew |= mx > mrun[nt][j] + kSlack;
         }
-    }
-    // ---- weights and values
+      if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      constexpr int kLo = kBf16 ? 2 : 1;  // bf16 weights as a sum of two, so that their rounding does not show
-      uint32_t bw[kQuant ? G : 1][NT][2][kLo];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float p[2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float x = s2[s][nt][2 * i + j];
-            p[j] = x == -INFINITY ? 0.f : exp2_approx(x - mrun[nt][j]);
-            l[nt][j] += p[j];
-          }
+            float mx = mrun[nt][j];
 #pragma unroll
-          for (int gi = 0; gi < (kQuant ? G : 1); ++gi) {
-            if constexpr (kQuant) {
+            for (int hv = 0; hv < HV; ++hv) mx = fmaxf(mx, fmaxf(z[hv][nt][j], z[hv][nt][2 + j]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float corr = exp2_approx(mrun[nt][j] - mx);
+            mrun[nt][j] = mx;
+            l[nt][j] *= corr;
 #pragma unroll
-              for (int j = 0; j < 2; ++j) pm[nt][gi][j] = fmaf(p[j], mv[s][i][gi], pm[nt][gi][j]);
+            for (int gi = 0; gi < (kQuant ? G : 1); ++gi) pm[nt][gi][j] *= corr;
+#pragma unroll
+            for (int t = 0; t < X::TILES; ++t) {
+              acc[t][nt][j] *= corr;
+              acc[t][nt][2 + j] *= corr;
             }
-            const float w0 = p[0] * sv[s][i][gi], w1 = p[1] * sv[s][i][gi];
-            const uint32_t hi = pack2<kBf16>(w0, w1);
-            bw[gi][nt][i][0] = movmatrix_trans(hi);
-            if constexpr (kBf16) {
-              const float2 back = unpack2<true>(hi);
-              bw[gi][nt][i][1] = movmatrix_trans(pack2<true>(w0 - back.x, w1 - back.y));
+          }
+      }
+      // ---- weights and values
+#pragma unroll
+      for (int hv = 0; hv < HV; ++hv) {
+        const uint32_t stage = at_use + hv * X::BLOCK + kTok * X::ROWB;
+        uint32_t vw[4][NU * UR];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = tv ^ (i & 1);
+#pragma unroll
+          for (int u = 0; u < NU; ++u) {
+            const uint32_t a = stage + (t + 8 * (i >> 1)) * X::ROWB +
+                               ((u * 8 * X::UB + r * X::UB) ^ (swizzle<X::CPR>(t) << 4));
+            if constexpr (X::UB == 2) {
+              vw[i][u] = lds_u16(a);
+            } else {
+              lds<UR>(a, &vw[i][u * UR]);
             }
           }
         }
+        constexpr int kLo = kBf16 ? 2 : 1;  // bf16 weights as a sum of two, so that their rounding does not show
+        uint32_t bw[kQuant ? G : 1][NT][2][kLo];
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const int gi = kQuant ? u * 8 * X::UB * 8 / BITS / X::GROUP : 0;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int w = 0; w < UR; ++w) {
-          // halves of the word: lanes' tokens (2c, 2c + 1) and (2c + 8, 2c + 9)
-          const uint32_t x0 = vw[s][0][u * UR + w], x1 = vw[s][1][u * UR + w], x2 = vw[s][2][u * UR + w],
-                         x3 = vw[s][3][u * UR + w];
-          const uint32_t lo01 = __byte_perm(x0, x1, 0x5410), lo23 = __byte_perm(x2, x3, 0x5410);
-          const uint32_t hi01 = X::UB == 2 ? 0u : __byte_perm(x0, x1, 0x7632);
-          const uint32_t hi23 = X::UB == 2 ? 0u : __byte_perm(x2, x3, 0x7632);
-          if constexpr (BITS == 16) {
-            const int tile = u * UT + w;
+          for (int i = 0; i < 2; ++i) {
+            float wt[2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int j = 0; j < 2; ++j) {
+              wt[j] = exp2_approx(z[hv][nt][2 * i + j] - mrun[nt][j]);
+              l[nt][j] = kQuant ? fmaf(wt[j], rs[hv][i], l[nt][j]) : l[nt][j] + wt[j];
+            }
 #pragma unroll
-              for (int q = 0; q < kLo; ++q)
-                mma16816<kBf16>(acc[tile][nt], lo01, hi01, lo23, hi23, bw[0][nt][0][q], bw[0][nt][1][q]);
-          } else {
+            for (int gi = 0; gi < (kQuant ? G : 1); ++gi) {
+              float w0 = wt[0], w1 = wt[1];
+              if constexpr (kQuant) {
 #pragma unroll
-            for (int hf = 0; hf < (X::UB == 2 ? 1 : 2); ++hf) {
-              const uint32_t a = hf ? hi01 : lo01, d = hf ? hi23 : lo23;
-              if constexpr (BITS == 8) {
-                const int tile = u * UT + 2 * w + hf;
+                for (int j = 0; j < 2; ++j) pm[nt][gi][j] = fmaf(wt[j], mr[hv][i][gi], pm[nt][gi][j]);
+                if constexpr (G > 1) {
+                  w0 *= sr[hv][i][gi];
+                  w1 *= sr[hv][i][gi];
+                }
+              }
+              const uint32_t hi = pack2<kBf16>(w0, w1);
+              bw[gi][nt][i][0] = movmatrix_trans(hi);
+              if constexpr (kBf16) {
+                const float2 back = unpack2<true>(hi);
+                bw[gi][nt][i][1] = movmatrix_trans(pack2<true>(w0 - back.x, w1 - back.y));
+              }
+            }
+          }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                  mma16816<false>(acc[tile][nt], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, d & 0x00ff00ffu,
-                                  (d >> 8) & 0x00ff00ffu, bw[gi][nt][0][0], bw[gi][nt][1][0]);
-              } else {
+        for (int u = 0; u < NU; ++u) {
+          const int gi = kQuant ? u * 8 * X::UB * 8 / BITS / X::GROUP : 0;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const uint32_t as = k ? a >> 8 : a, ds = k ? d >> 8 : d;
-                  const int tile = u * UT + 4 * w + 2 * hf + k;
+          for (int w = 0; w < UR; ++w) {
+            // halves of the word: the tokens of slots (2c, 2c + 1) and (2c + 8, 2c + 9)
+            const uint32_t x0 = vw[0][u * UR + w], x1 = vw[1][u * UR + w], x2 = vw[2][u * UR + w],
+                           x3 = vw[3][u * UR + w];
+            const uint32_t lo01 = __byte_perm(x0, x1, 0x5410), lo23 = __byte_perm(x2, x3, 0x5410);
+            const uint32_t hi01 = X::UB == 2 ? 0u : __byte_perm(x0, x1, 0x7632);
+            const uint32_t hi23 = X::UB == 2 ? 0u : __byte_perm(x2, x3, 0x7632);
+            if constexpr (BITS == 16) {
+              const int tile = u * UT + w;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < kLo; ++q)
+                  mma16816<kBf16>(acc[tile][nt], lo01, hi01, lo23, hi23, bw[0][nt][0][q], bw[0][nt][1][q]);
+            } else {
+#pragma unroll
+              for (int hf = 0; hf < (X::UB == 2 ? 1 : 2); ++hf) {
+                const uint32_t a = hf ? hi01 : lo01, d = hf ? hi23 : lo23;
+                if constexpr (BITS == 8) {
+                  const int tile = u * UT + 2 * w + hf;
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt)
-                    mma16816<false>(acc[tile][nt], as & 0x000f000fu, as & 0x00f000f0u, ds & 0x000f000fu,
-                                    ds & 0x00f000f0u, bw[gi][nt][0][0], bw[gi][nt][1][0]);
+                    mma16816<false>(acc[tile][nt], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, d & 0x00ff00ffu,
+                                    (d >> 8) & 0x00ff00ffu, bw[gi][nt][0][0], bw[gi][nt][1][0]);
+                } else {
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) {
+                    const uint32_t as = k ? a >> 8 : a, ds = k ? d >> 8 : d;
+                    const int tile = u * UT + 4 * w + 2 * hf + k;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                      mma16816<false>(acc[tile][nt], as & 0x000f000fu, as & 0x00f000f0u, ds & 0x000f000fu,
+                                      ds & 0x00f000f0u, bw[gi][nt][0][0], bw[gi][nt][1][0]);
+                  }
                 }
               }
             }
           }
         }
       }
+      at_use = at_use + X::STAGE == ring_end ? ring : at_use + X::STAGE;
     }
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      load_v(s, token0(nxt + s), row_next[s]);
-      row_now[s] = row_next[s];
-      row_next[s] = block_row(nxt + kWarps * SUB + s);
-    }
-  }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // every warp has left its ring: the sums go there
 
-  // ---- join the warps: sums over the lanes of a column, then the warps in order
+    // ---- join the warps: each leaves its sums in shared memory, relative to its own reference
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j) {
+        const int col = 8 * nt + 2 * c + j;
 #pragma unroll
-      for (int off = 4; off <= 16; off <<= 1) {
-        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], off);
-        if constexpr (kQuant) {
+        for (int off = 4; off <= 16; off <<= 1) {
+          l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], off);
+          if constexpr (kQuant) {
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) pm[nt][gi][j] += __shfl_xor_sync(0xffffffffu, pm[nt][gi][j], off);
-        }
-      }
-      if (r == 0) ml[warp][8 * nt + 2 * c + j] = make_float2(mrun[nt][j], l[nt][j]);
-    }
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    if (warp == w) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col = 8 * nt + 2 * c + j;
-          float ref = -INFINITY;
-#pragma unroll
-          for (int v = 0; v < kWarps; ++v) ref = fmaxf(ref, ml[v][col].x);
-          const float f = mrun[nt][j] == -INFINITY ? 0.f : exp2_approx(mrun[nt][j] - ref);
-#pragma unroll
-          for (int t = 0; t < X::TILES; ++t) {
-            const int u = t / UT, in_u = t % UT;
-            const int d = BITS == 16 ? (u * 8 + r) * X::UB / 2 + 2 * in_u : (u * 8 + r) * X::UB * 8 / BITS + 2 * in_u;
-            const int gi = kQuant ? u * 8 * X::UB * 8 / BITS / X::GROUP : 0;
-            const float up = kQuant ? 0x1p24f : 1.f, up1 = BITS == 4 ? 0x1p20f : up;
-            const float x = fmaf(acc[t][nt][j], up, pm[nt][gi][j]) * f;
-            const float y = fmaf(acc[t][nt][2 + j], up1, pm[nt][gi][j]) * f;
-            if (w == 0) {
-              buf[col][d] = x;
-              buf[col][d + 1] = y;
-            } else {
-              buf[col][d] += x;
-              buf[col][d + 1] += y;
-            }
+            for (int gi = 0; gi < G; ++gi) pm[nt][gi][j] += __shfl_xor_sync(0xffffffffu, pm[nt][gi][j], off);
           }
         }
-    }
+        if (r == 0) ml[warp][col] = make_float2(mrun[nt][j], l[nt][j]);
+        float *dst = buf + (warp * 8 * NT + col) * kLd;
+#pragma unroll
+        for (int t = 0; t < X::TILES; ++t) {
+          const int u = t / UT, in_u = t % UT;
+          const int d = BITS == 16 ? (u * 8 + r) * X::UB / 2 + 2 * in_u : (u * 8 + r) * X::UB * 8 / BITS + 2 * in_u;
+          const int gi = kQuant ? u * 8 * X::UB * 8 / BITS / X::GROUP : 0;
+          const float up = kQuant ? 0x1p24f : 1.f, up1 = BITS == 4 ? 0x1p20f : up;
+          *reinterpret_cast<float2 *>(dst + d) =
+              make_float2(fmaf(acc[t][nt][j], up, pm[nt][gi][j]), fmaf(acc[t][nt][2 + j], up1, pm[nt][gi][j]));
+        }
+      }
     __syncthreads();
-  }
-  // ---- out: the row's result, or this split's part of it
-  const int64_t part = ((static_cast<int64_t>(b) * P.Hkv + hk) * A.row_blocks + rb) * A.splits + split;
-  for (int col = warp; col < 8 * NT; col += kWarps) {
-    const int R = row0 + col;
-    if (R >= rows) break;
-    float ref = -INFINITY, sum = 0.f;
+    // ---- out: the row's result, or this worker's part of it
+    const bool whole = u0 == 0 && u1 == units;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg0 + u0 == run0 ? 0 : 1);
+    for (int col = warp; col < 8 * NT; col += kWarps) {
+      const int R = row0 + col;
+      if (R >= rows) break;
+      float ref = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) ref = fmaxf(ref, ml[v][col].x);
+      for (int v = 0; v < kWarps; ++v) ref = fmaxf(ref, ml[v][col].x);
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v)
-      sum += ml[v][col].x == -INFINITY ? ml[v][col].y * 0.f : ml[v][col].y * exp2_approx(ml[v][col].x - ref);
-    if (A.splits == 1) {
+      for (int v = 0; v < kWarps; ++v) {
+        f[v] = exp2_approx(ml[v][col].x - ref);
+        sum = fmaf(ml[v][col].y, f[v], sum);
+      }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t at = row_at(P.o, b, hk, g, R);
+      const int64_t o_at = row_at(P.o, b_now, hk, g, R);
       bool bad = false;
       for (int d = lane; d < D; d += 32) {
-        const float x = buf[col][d] * inv;
-        bad |= !isfinite(x);
-        store_o(P.o.p, at + d, P.dtype, x);
+        float x = 0.f;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) x = fmaf(buf[(v * 8 * NT + col) * kLd + d], f[v], x);
+        if (whole) {
+          x *= inv;
+          bad |= !isfinite(x);
+          store_o(P.o.p, o_at + d, P.dtype, x);
+        } else {
+          A.part_o[(slot * 8 * NT + col) * D + d] = x;
+        }
       }
+      if (!whole && lane == 0) A.part_ml[slot * 8 * NT + col] = make_float2(ref, sum);
       if constexpr (!kQuant) {
         // several queries: a value row of another query's range may hold an infinity or NaN
         if (rg.m > 1 && __any_sync(0xffffffffu, bad)) {
           using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
           const int pos = rg.p_first + R / g;
           __syncwarp();
-          attention_row<T>(static_cast<const T *>(P.q.p) + row_at(P.q, b, hk, g, R), reinterpret_cast<const T *>(kbase),
-                           reinterpret_cast<const T *>(vbase), static_cast<T *>(P.o.p) + at, P.k.sl, P.v.sl, D, pos,
-                           window_lo(P.mask, pos), P.mask.sinks, P.scale * kLog2e);
+          attention_row<T>(static_cast<const T *>(P.q.p) + row_at(P.q, b_now, hk, g, R),
+                           reinterpret_cast<const T *>(kbase), reinterpret_cast<const T *>(vbase),
+                           static_cast<T *>(P.o.p) + o_at, P.k.sl, P.v.sl, D, pos, window_lo(P.mask, pos),
+                           P.mask.sinks, P.scale * kLog2e);
         }
       }
-    } else {
-      for (int d = lane; d < D; d += 32) A.part_o[(part * 8 * NT + col) * D + d] = buf[col][d];
-      if (lane == 0) A.part_ml[part * 8 * NT + col] = make_float2(ref, sum);
     }
+    __syncthreads();  // buf and ml are free for the next segment
   }
 }
 
-// Joins the splits of a row: one warp a row, splits in order.
+// Joins the parts of the rows whose segment was cut: one warp a row, the
+// workers in order.
 template <int D, bool kBf16, bool kDense>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const Params A, int nrows) {
   const AttnProblem &P = A.p;
   const int lane = threadIdx.x & 31, g = P.H / P.Hkv;
-  const int rows_all = g * P.mask.Lq;
+  const int rows_all = g * P.mask.Lq, per_seq = P.Hkv * A.row_blocks;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   pdl_launch_dependents();
   pdl_wait();
@@ -701,25 +952,33 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const Params A, int n
   int n, m;
   seq_lens(P.mask, b, n, m);
   if (R >= g * m) return;
-  const int64_t part0 = (bh * A.row_blocks + R / nrows) * A.splits;
+  int before;
+  const int64_t total = static_cast<int64_t>(count_units(P.mask, P.B, b, &before)) * per_seq;
+  const int units = seq_units(P.mask, b), workers = active_workers(total, A.workers);
+  const int64_t seg0 = static_cast<int64_t>(before) * per_seq + static_cast<int64_t>(hk * A.row_blocks + R / nrows) * units;
+  const int w0 = worker_of(total, workers, seg0), w1 = worker_of(total, workers, seg0 + units - 1);
+  if (w0 == w1) return;  // whole: its worker has written it
   const int col = R % nrows;
+  // the segment is the first of every run but w0's, where it is the last (or the first too)
+  auto slot = [&](int w) {
+    return 2 * static_cast<int64_t>(w) + (w == w0 && run_begin(total, workers, w) != seg0 ? 1 : 0);
+  };
   float ref = -INFINITY;
-  for (int s = lane; s < A.splits; s += 32) ref = fmaxf(ref, A.part_ml[(part0 + s) * nrows + col].x);
+  for (int w = w0 + lane; w <= w1; w += 32) ref = fmaxf(ref, A.part_ml[slot(w) * nrows + col].x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, off));
   constexpr int kPer = (D + 31) / 32;
   float acc[kPer], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int s = 0; s < A.splits; ++s) {
-    const float2 t = A.part_ml[(part0 + s) * nrows + col];
-    if (t.x == -INFINITY && t.y == 0.f) continue;  // an empty split
-    const float f = t.x == -INFINITY ? 0.f : exp2_approx(t.x - ref);
+  for (int w = w0; w <= w1; ++w) {
+    const int64_t s = slot(w) * nrows + col;
+    const float2 t = A.part_ml[s];
+    const float f = exp2_approx(t.x - ref);
     sum = fmaf(t.y, f, sum);
-    const float *src = A.part_o + ((part0 + s) * nrows + col) * D;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (lane + 32 * i < D) acc[i] = fmaf(src[lane + 32 * i], f, acc[i]);
+      if (lane + 32 * i < D) acc[i] = fmaf(A.part_o[s * D + lane + 32 * i], f, acc[i]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t at = row_at(P.o, b, hk, g, R);
@@ -744,24 +1003,41 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const Params A, int n
   }
 }
 
+// CTAs of 128 threads an SM holds: what the registers (accumulators, query
+// operand, a block's codes) and the rings leave.
+constexpr int ctas_per_sm(int bits, int D, int G, int NT) {
+  return D == 256   ? (bits == 16 ? 1 : 2)
+         : NT == 2  ? (D == 64 ? 3 : 2)
+         : bits == 16 ? (D == 128 ? 2 : 3)
+                      : (D == 128 && (bits == 8 || G > 1) ? 3 : 4);
+}
+
 template <int BITS, int D, int G, bool kBf16, int NT>
 cudaError_t launch_split(const Params &a, cudaStream_t stream) {
-  // blocks in flight a warp: about 4 KB of codes
-  constexpr int SUB = D * BITS <= 512 ? 2 : 1;
+  using X = Geo<BITS, D, G>;
+  constexpr int CTAS = ctas_per_sm(BITS, D, G, NT);
+  constexpr int sums = kWarps * 8 * NT * (D + 4) * static_cast<int>(sizeof(float));
+  constexpr int rings = kWarps * X::STAGES * X::STAGE;
+  constexpr int smem = sums > rings ? sums : rings;
+  auto kern = split_kernel<BITS, D, G, kBf16, NT, CTAS>;
+  cudaError_t e = cudaSuccess;
+  if (smem + 1024 > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(a.splits), static_cast<unsigned>(a.p.Hkv * a.row_blocks),
-                     static_cast<unsigned>(a.p.B));
+  cfg.gridDim = dim3(static_cast<unsigned>(a.workers));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, split_kernel<BITS, D, G, kBf16, NT, SUB>, a);
-  if (e == cudaSuccess && a.splits > 1) {
+  e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e == cudaSuccess && a.part_ml) {
     const int64_t rows = static_cast<int64_t>(a.p.B) * a.p.H * a.p.mask.Lq;
     cfg.gridDim = dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps));
+    cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, combine_kernel<D, kBf16, BITS == 16>, a, 8 * NT);
   }
   return e != cudaSuccess ? e : cudaGetLastError();

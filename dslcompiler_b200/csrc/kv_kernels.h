@@ -66,9 +66,9 @@ cudaError_t kv_read_launch(const KvPool &p, const View4 &k, const View4 &v, int 
 // Few query rows over many keys, split along the keys.  Over a cache: pool
 // and block_table [B, table_width]; dense: pool == nullptr.
 struct SplitPlan {
-  int splits;       // CTAs a (sequence, key head, row block) is cut into
+  int workers;      // CTAs that share the work
   int row_blocks;   // blocks of query rows of one key head
-  size_t ws_bytes;  // device workspace the launch needs (0 when splits == 1)
+  size_t ws_bytes;  // device workspace the launch needs (0: no work is cut)
 };
 bool split_supported(const AttnProblem &p, const KvPool *pool);
 SplitPlan split_plan(const AttnProblem &p, const KvPool *pool, int sm_count);
