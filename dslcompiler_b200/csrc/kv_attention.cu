@@ -36,8 +36,11 @@ bool split_supported(const AttnProblem &p, const KvPool *pool) {
   const int64_t g = p.Hkv > 0 ? p.H / p.Hkv : 0, rows = g * p.mask.Lq;
   if (p.dtype != LLK_DTYPE_BF16 && p.dtype != LLK_DTYPE_FP16) return false;
   if (rows * p.Hkv > (int64_t(1) << 30) / (p.B > 0 ? p.B : 1)) return false;  // rows are counted in 32 bits
-  // so are the units of work, and the rows of a pool
-  if ((static_cast<int64_t>(p.mask.Lk) / kSpan + 1) * (p.B > 0 ? p.B : 1) >= (int64_t(1) << 31)) return false;
+  // so are the units of work (and a sum of two of them), and the rows of a pool
+  const int64_t units = (static_cast<int64_t>(p.mask.Lk) / kSpan + 2) * p.B;  // kMaxLen's bounds: below 2^53
+  if (units >= (int64_t(1) << 30) || units * p.Hkv >= (int64_t(1) << 30) ||
+      units * p.Hkv * ((rows + 7) / 8) >= (int64_t(1) << 30))
+    return false;
   if (pool) return kv_pool_supported(*pool) && pool->num_pages <= 0xffffffffll / pool->Hkv / pool->page;
   const auto on16 = [](const View4 &v) {
     return (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % 8 == 0 && v.sh % 8 == 0 && v.sl % 8 == 0;
@@ -79,6 +82,9 @@ cudaError_t split_launch(const AttnProblem &p, const KvPool *pool, const int *bl
   a.table_width = table_width;
   a.workers = plan.workers;
   a.row_blocks = plan.row_blocks;
+  a.page_shift = -1;
+  for (int i = 4; pool && i < 17; ++i)
+    if (pool->page == 1 << i) a.page_shift = i;
   a.q_vec = (reinterpret_cast<uintptr_t>(p.q.p) & 7) == 0 && p.q.sb % 4 == 0 && p.q.sh % 4 == 0 && p.q.sl % 4 == 0;
   if (plan.ws_bytes) {
     const int nt = row_tiles(p.H / p.Hkv * p.mask.Lq, p.D);

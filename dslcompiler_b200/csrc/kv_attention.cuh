@@ -54,6 +54,7 @@ struct Params {
   int64_t table_width;
   int row_blocks;
   int workers;      // CTAs that share the work
+  int page_shift;   // log2 of the page, or -1
   int q_vec;        // query rows start on 8 bytes
   float *part_o;    // [2 workers, 8 NT, D]: a CTA's parts of its first and its last segment
   float2 *part_ml;  // [2 workers, 8 NT] (reference, sum)
@@ -121,19 +122,20 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void *src, boo
 }
 
 template <int WORDS>
-__device__ __forceinline__ void lds(uint32_t a, uint32_t *w) {
+__device__ __forceinline__ void lds(const uint8_t *a, uint32_t *w) {
   if constexpr (WORDS == 4) {
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+    const uint4 x = *reinterpret_cast<const uint4 *>(a);
+    w[0] = x.x;
+    w[1] = x.y;
+    w[2] = x.z;
+    w[3] = x.w;
   } else if constexpr (WORDS == 2) {
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+    const uint2 x = *reinterpret_cast<const uint2 *>(a);
+    w[0] = x.x;
+    w[1] = x.y;
   } else {
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a));
+    w[0] = *reinterpret_cast<const uint32_t *>(a);
   }
-}
-__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
-  unsigned short x;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(a));
-  return x;
 }
 
 template <bool kBf16>
@@ -233,11 +235,11 @@ __device__ __forceinline__ Range make_range(const AttnMask &mk, int n, int m) {
 // query rows); its units are kSpan tokens each, at least one (a segment
 // without tokens still writes its zeros).  All units of the call, segment by
 // segment in the order (sequence, key head, row block), are dealt to the
-// workers in equal runs, whatever the lengths are: worker w has the units
-// [total w / workers, total (w + 1) / workers).  A segment that one worker has
-// whole is written by it; of one that is cut, each worker leaves its part in
-// its slot -- the first segment of its run in slot 2 w, else the last in
-// 2 w + 1 -- and combine_kernel joins them in order.
+// workers in runs of equal length (or one more), whatever the lengths are.  A
+// segment that one worker has whole is written by it; of one that is cut, each
+// worker leaves its part in its slot -- the first segment of its run in slot
+// 2 w, else the last in 2 w + 1 -- and combine_kernel joins them in order.
+// (split_supported keeps all counts below 2^31.)
 __device__ __forceinline__ int seq_units(const AttnMask &mk, int b) {
   int n, m;
   seq_lens(mk, b, n, m);
@@ -246,7 +248,7 @@ __device__ __forceinline__ int seq_units(const AttnMask &mk, int b) {
 }
 
 // Units of the sequences before b0 (*before) and of all (returned), of one
-// segment each, by one warp.  (split_supported keeps both below 2^31.)
+// segment each, by one warp.
 __device__ __forceinline__ int count_units(const AttnMask &mk, int B, int b0, int *before) {
   int all = 0, pre = 0;
   for (int b = threadIdx.x & 31; b < B; b += 32) {
@@ -258,10 +260,9 @@ __device__ __forceinline__ int count_units(const AttnMask &mk, int B, int b0, in
   return __reduce_add_sync(0xffffffffu, all);
 }
 
-// The sequence that holds unit `at` of the call (a sequence has per_seq
-// segments): *first = units before that sequence.  By one warp.
-__device__ __forceinline__ int find_seq(const AttnMask &mk, int B, int per_seq, int64_t at, int64_t *first) {
-  const int target = static_cast<int>(at / per_seq);  // in units of one segment a sequence
+// The sequence that holds unit `at`, counting one segment a sequence:
+// *first = units before that sequence.  By one warp.
+__device__ __forceinline__ int find_seq(const AttnMask &mk, int B, int at, int *first) {
   int base = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
@@ -272,31 +273,33 @@ __device__ __forceinline__ int find_seq(const AttnMask &mk, int B, int per_seq, 
       const int v = __shfl_up_sync(0xffffffffu, inc, off);
       if ((threadIdx.x & 31) >= off) inc += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + inc > target);
+    const unsigned hit = __ballot_sync(0xffffffffu, base + inc > at);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      *first = static_cast<int64_t>(base + __shfl_sync(0xffffffffu, inc - u, l)) * per_seq;
+      *first = base + __shfl_sync(0xffffffffu, inc - u, l);
       return b0 + l;
     }
     base += __shfl_sync(0xffffffffu, inc, 31);
   }
-  *first = static_cast<int64_t>(base) * per_seq;
+  *first = base;
   return B;
 }
 
-__device__ __forceinline__ int64_t run_begin(int64_t total, int workers, int w) { return total * w / workers; }
-// The worker whose run holds unit u.
-__device__ __forceinline__ int worker_of(int64_t total, int workers, int64_t u) {
-  int w = static_cast<int>(u * workers / total);
-  while (run_begin(total, workers, w + 1) <= u) ++w;
-  while (run_begin(total, workers, w) > u) --w;
-  return w;
-}
-// Workers that take part: every one of them has at least one unit.
-__device__ __forceinline__ int active_workers(int64_t total, int workers) {
-  return total < workers ? static_cast<int>(total) : workers;
-}
-
+// The runs: of `total` units, worker w has each = total / workers of them,
+// the first `more` workers one more.  At most as many workers as units.
+struct Runs {
+  int each, more, workers;
+  __device__ __forceinline__ Runs(int total, int all) {
+    workers = total < all ? total : all;
+    each = total / workers;
+    more = total - each * workers;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * each + (w < more ? w : more); }
+  __device__ __forceinline__ int worker_of(int u) const {
+    const int edge = more * (each + 1);
+    return u < edge ? u / (each + 1) : more + (u - edge) / each;
+  }
+};
 
 // Row R of a (sequence, key head): query R / g, head hk g + R % g.
 __device__ __forceinline__ int64_t row_at(const View4 &v, int b, int hk, int g, int R) {
@@ -332,16 +335,16 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
   const AttnProblem &P = A.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const int g = P.H / P.Hkv, per_seq = P.Hkv * A.row_blocks;
-  pdl_launch_dependents();
   pdl_wait();
-  int none;
-  const int64_t total = static_cast<int64_t>(count_units(P.mask, P.B, 0, &none)) * per_seq;
-  const int workers = active_workers(total, A.workers);
-  if (static_cast<int>(blockIdx.x) >= workers) return;
-  int64_t at = run_begin(total, workers, blockIdx.x);
-  const int64_t run0 = at, run1 = run_begin(total, workers, blockIdx.x + 1);
-  int64_t seq0;
-  int b = find_seq(P.mask, P.B, per_seq, at, &seq0);
+  pdl_launch_dependents();  // (after the wait: the next kernel may read the lengths before its own)
+  int before;
+  const int total = count_units(P.mask, P.B, 0, &before) * per_seq;
+  const Runs runs(total, A.workers);
+  if (static_cast<int>(blockIdx.x) >= runs.workers) return;
+  const int run0 = runs.begin(blockIdx.x), run1 = runs.begin(blockIdx.x + 1);
+  int at = run0, seq0;
+  int b = find_seq(P.mask, P.B, at / per_seq, &seq0);
+  seq0 *= per_seq;
 
   // ---- segment by segment
   while (at < run1) {
@@ -349,11 +352,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
     seq_lens(P.mask, b, n, m);
     const Range rg = make_range(P.mask, n, m);
     const int units = rg.blocks > kUnit ? (rg.blocks + kUnit - 1) / kUnit : 1;
-    const int seg = static_cast<int>((at - seq0) / units);
-    const int64_t seg0 = seq0 + static_cast<int64_t>(seg) * units;
+    const int seg = (at - seq0) / units, seg0 = seq0 + seg * units;
     const int hk = seg / A.row_blocks, rb = seg - hk * A.row_blocks;
-    const int u0 = static_cast<int>(at - seg0);
-    const int u1 = static_cast<int>((run1 - seg0 < units ? run1 - seg0 : units));
+    const int u0 = at - seg0, u1 = run1 - seg0 < units ? run1 - seg0 : units;
     const int rows = g * rg.m, row0 = rb * 8 * NT;
     at = seg0 + u1;
     const int b_now = b;
@@ -362,6 +363,110 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       ++b;
     }
     if (row0 >= rows) continue;  // rows behind the sequence's queries: nothing is written
+
+    // ---- this warp's blocks of the segment's units [u0, u1)
+    const int beg = u0 * kUnit, end = u1 * kUnit < rg.blocks ? u1 * kUnit : rg.blocks;
+    auto token0 = [&](int blk) { return (blk < rg.nsb ? blk : rg.wb0 + blk - rg.nsb) * kTok; };
+    // row of a block's first token among the rows of the pool (dense: of the head)
+    auto look = [&](int blk) -> uint32_t {
+      if (blk >= end) return kNoBlock;
+      const int t0 = token0(blk);
+      if constexpr (kQuant) {
+        const int page = A.page_shift >= 0 ? t0 >> A.page_shift : t0 / A.pool.page;
+        const int entry = A.table[b_now * A.table_width + page];
+        if (entry < 0 || entry >= A.pool.num_pages) return kNoBlock;
+        return (static_cast<uint32_t>(entry) * P.Hkv + hk) * A.pool.page + (t0 - page * A.pool.page);
+      } else {
+        return t0;
+      }
+    };
+    // lane i looks at the i-th of the warp's next 32 blocks
+    constexpr int HV = X::HV, kTurns = 32 / HV, kStep = kWarps * HV;
+    const int first = beg + warp * HV;
+    auto look_ahead = [&](int turn) { return look(first + (turn + lane / HV) * kStep + lane % HV); };
+    uint32_t rows_now = look_ahead(0), rows_next = end - first > kTurns * kStep ? look_ahead(kTurns) : kNoBlock;
+
+    const char *kbase, *vbase;
+    int64_t k_sl, v_sl;  // bytes between tokens
+    if constexpr (kQuant) {
+      kbase = static_cast<const char *>(A.pool.k_codes);
+      vbase = static_cast<const char *>(A.pool.v_codes);
+      k_sl = v_sl = X::ROWB;
+    } else {
+      kbase = static_cast<const char *>(P.k.p) + 2 * (b_now * P.k.sb + hk * P.k.sh);
+      vbase = static_cast<const char *>(P.v.p) + 2 * (b_now * P.v.sb + hk * P.v.sh);
+      k_sl = 2 * P.k.sl;
+      v_sl = 2 * P.v.sl;
+    }
+    // a token that no query of the sequence sees is not read: what lies there may be anything
+    auto seen = [&](int t) { return t < rg.n && (t >= rg.lo || t < rg.s_end); };
+    const uint8_t *ring = smem + warp * X::STAGES * X::STAGE;
+    constexpr int kPer = kTok * X::CPR / 32;  // chunks of K (of V) a lane
+    static_assert(kTok * X::CPR % 32 == 0, "whole chunks a lane");
+    // chunk i of this lane: token (lane + 32 i) / CPR, its place in the stage
+    uint32_t put[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = lane + 32 * i, t = e / X::CPR;
+      put[i] = t * X::ROWB + (((e % X::CPR) ^ swizzle<X::CPR>(t)) << 4);
+    }
+    const char *psrc = static_cast<const char *>(lane < 16 ? A.pool.k_params : A.pool.v_params) + (lane & 15) * X::PG;
+    const uint32_t pput = 2 * kTok * X::ROWB + (lane & 15) * 2 * X::PG + (lane >> 4) * X::PG;
+    // a block into its place of a stage; tokens that are not read become zeros
+    // (of kNoBlock nothing is used: codes are finite whatever lies in the stage)
+    auto load = [&](uint32_t dst, int blk, uint32_t row) {
+      if (row == kNoBlock) return;
+      if (blk >= rg.full0 && blk < rg.full1) {
+        if constexpr (kQuant) {
+          const int64_t o = static_cast<int64_t>(row) * X::ROWB + lane * 16;
+          const char *ks = kbase + o, *vs = vbase + o;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            cp_async<16>(dst + put[i], ks + 512 * i);
+            cp_async<16>(dst + put[i] + kTok * X::ROWB, vs + 512 * i);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int64_t t = row + (lane + 32 * i) / X::CPR;
+            const int ch = (lane + 32 * i) % X::CPR;
+            cp_async<16>(dst + put[i], kbase + t * k_sl + 16 * ch);
+            cp_async<16>(dst + put[i] + kTok * X::ROWB, vbase + t * v_sl + 16 * ch);
+          }
+        }
+      } else {
+        const int t0 = token0(blk);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int e = lane + 32 * i, t = e / X::CPR, ch = e % X::CPR;
+          const bool in = seen(t0 + t);
+          const int64_t at_row = static_cast<int64_t>(row) + t;
+          cp_async16_if(dst + put[i], in ? kbase + at_row * k_sl + 16 * ch : kbase, in);
+          cp_async16_if(dst + put[i] + kTok * X::ROWB, in ? vbase + at_row * v_sl + 16 * ch : vbase, in);
+        }
+      }
+      if constexpr (kQuant) {
+        // (a page is in the pool whole; what is not seen is masked when it is used)
+        const char *src = psrc + static_cast<int64_t>(row) * X::PG;
+#pragma unroll
+        for (int i = 0; i < X::PG; i += 16) cp_async<cmin_v<X::PG, 16>>(dst + pput + i, src + i);
+      }
+    };
+
+    const int tr = slot_token(r), tv = slot_token(2 * c);
+    uint32_t none = 0;  // blocks in the ring that do not exist, HV bits a turn, the latest lowest
+    auto load_turn = [&](uint32_t dst, int blk, int turn) {
+#pragma unroll
+      for (int hv = 0; hv < HV; ++hv) {
+        const int at_lane = turn * HV + hv;
+        const uint32_t row = __shfl_sync(0xffffffffu, at_lane < 32 ? rows_now : rows_next, at_lane & 31);
+        load(dst + hv * X::BLOCK, blk + hv, row);
+        none = none << 1 | (row == kNoBlock ? 1u : 0u);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < X::STAGES - 1; ++i) load_turn(smem_u32(ring) + i * X::STAGE, first + i * kStep, i);
 
     // ---- queries: B operands, per-column factors and sums
     uint32_t qf[NT][KS][2];
@@ -459,95 +564,6 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       for (int j = 0; j < 2; ++j) fcol[nt][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + j));
     }
 
-    // ---- this warp's blocks of the segment's units [u0, u1)
-    const int beg = u0 * kUnit, end = u1 * kUnit < rg.blocks ? u1 * kUnit : rg.blocks;
-    auto token0 = [&](int blk) { return (blk < rg.nsb ? blk : rg.wb0 + blk - rg.nsb) * kTok; };
-    // row of a block's first token among the rows of the pool (dense: of the head)
-    auto look = [&](int blk) -> uint32_t {
-      if (blk >= end) return kNoBlock;
-      const int t0 = token0(blk);
-      if constexpr (kQuant) {
-        const int page = t0 / A.pool.page;
-        const int entry = A.table[b_now * A.table_width + page];
-        if (entry < 0 || entry >= A.pool.num_pages) return kNoBlock;
-        return (static_cast<uint32_t>(entry) * P.Hkv + hk) * A.pool.page + (t0 - page * A.pool.page);
-      } else {
-        return t0;
-      }
-    };
-    // lane i looks at the i-th of the warp's next 32 blocks
-    constexpr int HV = X::HV, kTurns = 32 / HV, kStep = kWarps * HV;
-    const int first = beg + warp * HV;
-    auto look_ahead = [&](int turn) { return look(first + (turn + lane / HV) * kStep + lane % HV); };
-    uint32_t rows_now = look_ahead(0), rows_next = look_ahead(kTurns);
-
-    const char *kbase, *vbase;
-    int64_t k_sl, v_sl;  // bytes between tokens
-    if constexpr (kQuant) {
-      kbase = static_cast<const char *>(A.pool.k_codes);
-      vbase = static_cast<const char *>(A.pool.v_codes);
-      k_sl = v_sl = X::ROWB;
-    } else {
-      kbase = static_cast<const char *>(P.k.p) + 2 * (b_now * P.k.sb + hk * P.k.sh);
-      vbase = static_cast<const char *>(P.v.p) + 2 * (b_now * P.v.sb + hk * P.v.sh);
-      k_sl = 2 * P.k.sl;
-      v_sl = 2 * P.v.sl;
-    }
-    // a token that no query of the sequence sees is not read: what lies there may be anything
-    auto seen = [&](int t) { return t < rg.n && (t >= rg.lo || t < rg.s_end); };
-    const uint32_t ring = smem_u32(smem) + warp * X::STAGES * X::STAGE;
-    constexpr int kPer = kTok * X::CPR / 32;  // chunks of K (of V) a lane
-    static_assert(kTok * X::CPR % 32 == 0, "whole chunks a lane");
-    // chunk i of this lane: token (lane + 32 i) / CPR, its place in the stage
-    uint32_t put[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = lane + 32 * i, t = e / X::CPR;
-      put[i] = t * X::ROWB + (((e % X::CPR) ^ swizzle<X::CPR>(t)) << 4);
-    }
-    const char *psrc = static_cast<const char *>(lane < 16 ? A.pool.k_params : A.pool.v_params) + (lane & 15) * X::PG;
-    const uint32_t pput = 2 * kTok * X::ROWB + (lane & 15) * 2 * X::PG + (lane >> 4) * X::PG;
-    // a block into its place of a stage; tokens that are not read become zeros
-    // (of kNoBlock nothing is used: codes are finite whatever lies in the stage)
-    auto load = [&](uint32_t dst, int blk, uint32_t row) {
-      if (row == kNoBlock) return;
-      if (blk >= rg.full0 && blk < rg.full1) {
-        if constexpr (kQuant) {
-          const int64_t o = static_cast<int64_t>(row) * X::ROWB + lane * 16;
-          const char *ks = kbase + o, *vs = vbase + o;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            cp_async<16>(dst + put[i], ks + 512 * i);
-            cp_async<16>(dst + put[i] + kTok * X::ROWB, vs + 512 * i);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int64_t t = row + (lane + 32 * i) / X::CPR;
-            const int ch = (lane + 32 * i) % X::CPR;
-            cp_async<16>(dst + put[i], kbase + t * k_sl + 16 * ch);
-            cp_async<16>(dst + put[i] + kTok * X::ROWB, vbase + t * v_sl + 16 * ch);
-          }
-        }
-      } else {
-        const int t0 = token0(blk);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int e = lane + 32 * i, t = e / X::CPR, ch = e % X::CPR;
-          const bool in = seen(t0 + t);
-          const int64_t at_row = static_cast<int64_t>(row) + t;
-          cp_async16_if(dst + put[i], in ? kbase + at_row * k_sl + 16 * ch : kbase, in);
-          cp_async16_if(dst + put[i] + kTok * X::ROWB, in ? vbase + at_row * v_sl + 16 * ch : vbase, in);
-        }
-      }
-      if constexpr (kQuant) {
-        // (a page is in the pool whole; what is not seen is masked when it is used)
-        const char *src = psrc + static_cast<int64_t>(row) * X::PG;
-#pragma unroll
-        for (int i = 0; i < X::PG; i += 16) cp_async<cmin_v<X::PG, 16>>(dst + pput + i, src + i);
-      }
-    };
-
     float acc[X::TILES][NT][4], mrun[NT][2], l[NT][2], pm[NT][kQuant ? G : 1][2];
 #pragma unroll
     for (int t = 0; t < X::TILES; ++t)
@@ -565,27 +581,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
         for (int i = 0; i < (kQuant ? G : 1); ++i) pm[nt][i][j] = 0.f;
       }
 
-    const int tr = slot_token(r), tv = slot_token(2 * c);
-    uint32_t none = 0;  // blocks in the ring that do not exist, HV bits a turn, the latest lowest
-    auto load_turn = [&](uint32_t dst, int blk, int turn) {
-#pragma unroll
-      for (int hv = 0; hv < HV; ++hv) {
-        const int at_lane = turn * HV + hv;
-        const uint32_t row = __shfl_sync(0xffffffffu, at_lane < 32 ? rows_now : rows_next, at_lane & 31);
-        load(dst + hv * X::BLOCK, blk + hv, row);
-        none = none << 1 | (row == kNoBlock ? 1u : 0u);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < X::STAGES - 1; ++i) load_turn(ring + i * X::STAGE, first + i * kStep, i);
-    uint32_t at_use = ring, at_load = ring + (X::STAGES - 1) * X::STAGE;
-    const uint32_t ring_end = ring + X::STAGES * X::STAGE;
+    const uint8_t *at_use = ring, *at_load = ring + (X::STAGES - 1) * X::STAGE;
+    const uint8_t *ring_end = ring + X::STAGES * X::STAGE;
     int turn = 0;  // of the 32 rows in rows_now
     for (int blk = first; blk < end; blk += kStep) {
       // the turn STAGES - 1 ahead goes where the last one was (all lanes have read it); then this one is waited for
       __syncwarp();
-      load_turn(at_load, blk + (X::STAGES - 1) * kStep, turn + X::STAGES - 1);
+      load_turn(smem_u32(at_load), blk + (X::STAGES - 1) * kStep, turn + X::STAGES - 1);
       at_load = at_load + X::STAGE == ring_end ? ring : at_load + X::STAGE;
       asm volatile("cp.async.wait_group %0;" ::"n"(X::STAGES - 1) : "memory");
       __syncwarp();
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       float z[HV][NT][4], sr[HV][2][kQuant ? G : 1], mr[HV][2][kQuant ? G : 1], rs[HV][2];
 #pragma unroll
       for (int hv = 0; hv < HV; ++hv) {
-        const uint32_t stage = at_use + hv * X::BLOCK;
+        const uint8_t *stage = at_use + hv * X::BLOCK;
         uint32_t kw[2][WK], par[2][kQuant ? 2 * G : 1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -764,17 +766,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       // ---- weights and values
 #pragma unroll
       for (int hv = 0; hv < HV; ++hv) {
-        const uint32_t stage = at_use + hv * X::BLOCK + kTok * X::ROWB;
+        const uint8_t *stage = at_use + hv * X::BLOCK + kTok * X::ROWB;
         uint32_t vw[4][NU * UR];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = tv ^ (i & 1);
 #pragma unroll
           for (int u = 0; u < NU; ++u) {
-            const uint32_t a = stage + (t + 8 * (i >> 1)) * X::ROWB +
+            const uint8_t *a = stage + (t + 8 * (i >> 1)) * X::ROWB +
                                ((u * 8 * X::UB + r * X::UB) ^ (swizzle<X::CPR>(t) << 4));
             if constexpr (X::UB == 2) {
-              vw[i][u] = lds_u16(a);
+              vw[i][u] = *reinterpret_cast<const uint16_t *>(a);
             } else {
               lds<UR>(a, &vw[i][u * UR]);
             }
@@ -889,7 +891,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
     __syncthreads();
     // ---- out: the row's result, or this worker's part of it
     const bool whole = u0 == 0 && u1 == units;
-    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg0 + u0 == run0 ? 0 : 1);
+    const int64_t slot = 2 * blockIdx.x + (seg0 + u0 == run0 ? 0 : 1);
     for (int col = warp; col < 8 * NT; col += kWarps) {
       const int R = row0 + col;
       if (R >= rows) break;
@@ -937,48 +939,61 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
 // Joins the parts of the rows whose segment was cut: one warp a row, the
 // workers in order.
 template <int D, bool kBf16, bool kDense>
-__global__ void __launch_bounds__(kThreads) combine_kernel(const Params A, int nrows) {
+__global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant__ Params A, int nrows) {
   const AttnProblem &P = A.p;
   const int lane = threadIdx.x & 31, g = P.H / P.Hkv;
   const int rows_all = g * P.mask.Lq, per_seq = P.Hkv * A.row_blocks;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const unsigned id = blockIdx.x * kWarps + (threadIdx.x >> 5);  // ((b Hkv) + hk) rows_all + R
+  const unsigned bh = id / rows_all;
+  const int R = id - bh * rows_all, b = bh / P.Hkv, hk = bh - b * P.Hkv;
+  if (b >= P.B) return;
+  // Where the parts are, before the wait: the split kernel starts this one
+  // when it has waited for the kernels before it, so the lengths are there.
+  int n, m, before;
+  seq_lens(P.mask, b, n, m);
+  const int total = count_units(P.mask, P.B, b, &before) * per_seq;
+  const Runs runs(total, A.workers);
+  const int units = seq_units(P.mask, b);
+  const int seg0 = before * per_seq + (hk * A.row_blocks + R / nrows) * units;
+  const int w0 = runs.worker_of(seg0), w1 = runs.worker_of(seg0 + units - 1);
+  // whole: its worker writes it; rows behind the queries: nobody
+  const bool cut = w0 != w1 && R < g * m;
+  // the segment is the first of every run but w0's, where it is the last (or the first too)
+  const int col = R % nrows, late = runs.begin(w0) != seg0 ? 1 : 0;
+  auto slot = [&](int w) { return static_cast<int64_t>(2 * w + (w == w0 ? late : 0)) * nrows + col; };
   pdl_launch_dependents();
   pdl_wait();
-  const int R = static_cast<int>(id % rows_all);
-  const int64_t bh = id / rows_all;
-  const int hk = static_cast<int>(bh % P.Hkv);
-  if (bh / P.Hkv >= P.B) return;
-  const int b = static_cast<int>(bh / P.Hkv);
-  int n, m;
-  seq_lens(P.mask, b, n, m);
-  if (R >= g * m) return;
-  int before;
-  const int64_t total = static_cast<int64_t>(count_units(P.mask, P.B, b, &before)) * per_seq;
-  const int units = seq_units(P.mask, b), workers = active_workers(total, A.workers);
-  const int64_t seg0 = static_cast<int64_t>(before) * per_seq + static_cast<int64_t>(hk * A.row_blocks + R / nrows) * units;
-  const int w0 = worker_of(total, workers, seg0), w1 = worker_of(total, workers, seg0 + units - 1);
-  if (w0 == w1) return;  // whole: its worker has written it
-  const int col = R % nrows;
-  // the segment is the first of every run but w0's, where it is the last (or the first too)
-  auto slot = [&](int w) {
-    return 2 * static_cast<int64_t>(w) + (w == w0 && run_begin(total, workers, w) != seg0 ? 1 : 0);
-  };
-  float ref = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32) ref = fmaxf(ref, A.part_ml[slot(w) * nrows + col].x);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, off));
-  constexpr int kPer = (D + 31) / 32;
-  float acc[kPer], sum = 0.f;
+  if (!cut) return;
+  constexpr int kPer = (D + 31) / 32, kAt = 4;  // parts in flight
+  float ref = kNoRef, acc[kPer], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int w = w0; w <= w1; ++w) {
-    const int64_t s = slot(w) * nrows + col;
-    const float2 t = A.part_ml[s];
-    const float f = exp2_approx(t.x - ref);
-    sum = fmaf(t.y, f, sum);
+  for (int w = w0; w <= w1; w += kAt) {
+    float2 t[kAt];
+    float x[kAt][kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane + 32 * i < D) acc[i] = fmaf(A.part_o[s * D + lane + 32 * i], f, acc[i]);
+    for (int k = 0; k < kAt; ++k) {
+      t[k] = make_float2(kNoRef, 0.f);
+      if (w + k <= w1) t[k] = A.part_ml[slot(w + k)];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        x[k][i] = w + k <= w1 && lane + 32 * i < D ? A.part_o[slot(w + k) * D + lane + 32 * i] : 0.f;
+    }
+    float top = ref;
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) top = fmaxf(top, t[k].x);
+    const float corr = exp2_approx(ref - top);
+    sum *= corr;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] *= corr;
+    ref = top;
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) {
+      const float f = exp2_approx(t[k].x - ref);
+      sum = fmaf(t[k].y, f, sum);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] = fmaf(x[k][i], f, acc[i]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t at = row_at(P.o, b, hk, g, R);
