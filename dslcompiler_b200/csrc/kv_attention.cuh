@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
     }
     // a token that no query of the sequence sees is not read: what lies there may be anything
     auto seen = [&](int t) { return t < rg.n && (t >= rg.lo || t < rg.s_end); };
-    const uint8_t *ring = smem + warp * X::STAGES * X::STAGE;
+    const uint32_t ring = warp * X::STAGES * X::STAGE, smem_at = smem_u32(smem);  // (offsets in smem)
     constexpr int kPer = kTok * X::CPR / 32;  // chunks of K (of V) a lane
     static_assert(kTok * X::CPR % 32 == 0, "whole chunks a lane");
     // chunk i of this lane: token (lane + 32 i) / CPR, its place in the stage
@@ -454,6 +454,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
     };
 
     const int tr = slot_token(r), tv = slot_token(2 * c);
+    // where this lane reads in a block: key chunks of row tr, value units of rows tv and tv ^ 1, parameters of row tr
+    uint32_t k_at[X::CHUNKS], v_at[2][NU];
+#pragma unroll
+    for (int u = 0; u < X::CHUNKS; ++u)
+      k_at[u] = tr * X::ROWB + ((u * 16 * VW + c * 4 * VW) ^ (swizzle<X::CPR>(tr) << 4));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        v_at[i][u] = (kTok + (tv ^ i)) * X::ROWB + ((u * 8 * X::UB + r * X::UB) ^ (swizzle<X::CPR>(tv ^ i) << 4));
+    const uint32_t p_at = 2 * kTok * X::ROWB + tr * 2 * X::PG;
     uint32_t none = 0;  // blocks in the ring that do not exist, HV bits a turn, the latest lowest
     auto load_turn = [&](uint32_t dst, int blk, int turn) {
 #pragma unroll
@@ -466,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int i = 0; i < X::STAGES - 1; ++i) load_turn(smem_u32(ring) + i * X::STAGE, first + i * kStep, i);
+    for (int i = 0; i < X::STAGES - 1; ++i) load_turn(smem_at + ring + i * X::STAGE, first + i * kStep, i);
 
     // ---- queries: B operands, per-column factors and sums
     uint32_t qf[NT][KS][2];
@@ -581,13 +592,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
         for (int i = 0; i < (kQuant ? G : 1); ++i) pm[nt][i][j] = 0.f;
       }
 
-    const uint8_t *at_use = ring, *at_load = ring + (X::STAGES - 1) * X::STAGE;
-    const uint8_t *ring_end = ring + X::STAGES * X::STAGE;
+    uint32_t at_use = ring, at_load = ring + (X::STAGES - 1) * X::STAGE;
+    const uint32_t ring_end = ring + X::STAGES * X::STAGE;
     int turn = 0;  // of the 32 rows in rows_now
     for (int blk = first; blk < end; blk += kStep) {
       // the turn STAGES - 1 ahead goes where the last one was (all lanes have read it); then this one is waited for
       __syncwarp();
-      load_turn(smem_u32(at_load), blk + (X::STAGES - 1) * kStep, turn + X::STAGES - 1);
+      load_turn(smem_at + at_load, blk + (X::STAGES - 1) * kStep, turn + X::STAGES - 1);
       at_load = at_load + X::STAGE == ring_end ? ring : at_load + X::STAGE;
       asm volatile("cp.async.wait_group %0;" ::"n"(X::STAGES - 1) : "memory");
       __syncwarp();
@@ -601,18 +612,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       float z[HV][NT][4], sr[HV][2][kQuant ? G : 1], mr[HV][2][kQuant ? G : 1], rs[HV][2];
 #pragma unroll
       for (int hv = 0; hv < HV; ++hv) {
-        const uint8_t *stage = at_use + hv * X::BLOCK;
+        const uint32_t stage = at_use + hv * X::BLOCK;
         uint32_t kw[2][WK], par[2][kQuant ? 2 * G : 1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int u = 0; u < X::CHUNKS; ++u)
-            lds<VW>(stage + (tr + 8 * i) * X::ROWB + ((u * 16 * VW + c * 4 * VW) ^ (swizzle<X::CPR>(tr) << 4)),
-                    &kw[i][u * VW]);
+            lds<VW>(smem + (stage + k_at[u]) + 8 * i * X::ROWB, &kw[i][u * VW]);
           if constexpr (kQuant) {
 #pragma unroll
             for (int w = 0; w < 2 * G; w += cmin_v<2 * G, 4>)
-              lds<cmin_v<2 * G, 4>>(stage + 2 * kTok * X::ROWB + (tr + 8 * i) * 2 * X::PG + 4 * w, &par[i][w]);
+              lds<cmin_v<2 * G, 4>>(smem + (stage + p_at) + 8 * i * 2 * X::PG + 4 * w, &par[i][w]);
           }
         }
         if constexpr (kQuant) {
@@ -637,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
           const bool starts = w == 0 || (kQuant && ((w - 1) / VW) * 4 * VW * E / X::GROUP != gi);
           const bool ends = kQuant && (w + 1 == WK || ((w + 1) / VW) * 4 * VW * E / X::GROUP != gi);
           if constexpr (BITS == 4) {
-            const uint32_t xs = x >> 8, ys = y >> 8;
+            const uint32_t xs = (x >> 8), ys = (y >> 8);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               if (starts) {
@@ -766,15 +776,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       // ---- weights and values
 #pragma unroll
       for (int hv = 0; hv < HV; ++hv) {
-        const uint8_t *stage = at_use + hv * X::BLOCK + kTok * X::ROWB;
+        const uint32_t stage = at_use + hv * X::BLOCK;
         uint32_t vw[4][NU * UR];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int t = tv ^ (i & 1);
 #pragma unroll
           for (int u = 0; u < NU; ++u) {
-            const uint8_t *a = stage + (t + 8 * (i >> 1)) * X::ROWB +
-                               ((u * 8 * X::UB + r * X::UB) ^ (swizzle<X::CPR>(t) << 4));
+            const uint8_t *a = smem + (stage + v_at[i & 1][u]) + 8 * (i >> 1) * X::ROWB;
             if constexpr (X::UB == 2) {
               vw[i][u] = *reinterpret_cast<const uint16_t *>(a);
             } else {
@@ -844,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
                 } else {
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {
-                    const uint32_t as = k ? a >> 8 : a, ds = k ? d >> 8 : d;
+                    const uint32_t as = k ? (a >> 8) : a, ds = k ? (d >> 8) : d;
                     const int tile = u * UT + 4 * w + 2 * hf + k;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
