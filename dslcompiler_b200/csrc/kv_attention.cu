@@ -37,7 +37,7 @@ bool split_supported(const AttnProblem &p, const KvPool *pool) {
   if (p.dtype != LLK_DTYPE_BF16 && p.dtype != LLK_DTYPE_FP16) return false;
   if (rows * p.Hkv > (int64_t(1) << 30) / (p.B > 0 ? p.B : 1)) return false;  // rows are counted in 32 bits
   // so are the units of work (and a sum of two of them), and the rows of a pool
-  const int64_t units = (static_cast<int64_t>(p.mask.Lk) / kSpan + 2) * p.B;  // kMaxLen's bounds: below 2^53
+  const int64_t units = (static_cast<int64_t>(p.mask.Lk) / kSpan + 2 + kStart) * p.B;  // kMaxLen's bounds: below 2^53
   if (units >= (int64_t(1) << 30) || units * p.Hkv >= (int64_t(1) << 30) ||
       units * p.Hkv * ((rows + 7) / 8) >= (int64_t(1) << 30))
     return false;
@@ -62,10 +62,10 @@ SplitPlan split_plan(const AttnProblem &p, const KvPool *pool, int sm_count) {
     if (seen < keys) keys = seen;
   }
   const int64_t segments = static_cast<int64_t>(p.B) * p.Hkv * s.row_blocks;
-  const int64_t units = segments * (keys > kSpan ? (keys + kSpan - 1) / kSpan : 1);
+  const int64_t units = segments * (keys > kSpan ? (keys + kSpan - 1) / kSpan : 1), cost = units + segments * kStart;
   const int64_t room = static_cast<int64_t>(sm_count) *
                        ctas_per_sm(pool ? pool->bits : 16, p.D, pool ? p.D / pool->group : 1, nt);
-  s.workers = static_cast<int>(units < room ? units : room);
+  s.workers = static_cast<int>(cost < room ? cost : room);
   s.ws_bytes = 0;
   if (units > segments)  // else no segment has more than one unit: none is cut
     s.ws_bytes = 2 * static_cast<size_t>(s.workers) * 8 * nt * (static_cast<size_t>(p.D) * 4 + sizeof(float2));
@@ -85,7 +85,7 @@ cudaError_t split_launch(const AttnProblem &p, const KvPool *pool, const int *bl
   a.page_shift = -1;
   for (int i = 4; pool && i < 17; ++i)
     if (pool->page == 1 << i) a.page_shift = i;
-  a.q_vec = (reinterpret_cast<uintptr_t>(p.q.p) & 7) == 0 && p.q.sb % 4 == 0 && p.q.sh % 4 == 0 && p.q.sl % 4 == 0;
+  a.q_vec = (reinterpret_cast<uintptr_t>(p.q.p) & 3) == 0 && p.q.sb % 2 == 0 && p.q.sh % 2 == 0 && p.q.sl % 2 == 0;
   if (plan.ws_bytes) {
     const int nt = row_tiles(p.H / p.Hkv * p.mask.Lq, p.D);
     a.part_ml = static_cast<float2 *>(workspace);

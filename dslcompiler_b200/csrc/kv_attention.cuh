@@ -30,6 +30,8 @@
 // whatever the scales are, and 11 bits of it are kept.
 #pragma once
 
+#include <atomic>
+
 #include "attn_common.cuh"
 
 namespace llk_b200 {
@@ -55,8 +57,8 @@ struct Params {
   int row_blocks;
   int workers;      // CTAs that share the work
   int page_shift;   // log2 of the page, or -1
-  int q_vec;        // query rows start on 8 bytes
-  float *part_o;    // [2 workers, 8 NT, D]: a CTA's parts of its first and its last segment
+  int q_vec;        // query rows start on 4 bytes
+  float *part_o;    // [2 workers, 8 NT, D]: a CTA's parts of cut segments (slots as above combine_kernel)
   float2 *part_ml;  // [2 workers, 8 NT] (reference, sum)
 };
 
@@ -233,13 +235,17 @@ __device__ __forceinline__ Range make_range(const AttnMask &mk, int n, int m) {
 
 // ---- The work and its split.  A segment is a (sequence, key head, block of
 // query rows); its units are kSpan tokens each, at least one (a segment
-// without tokens still writes its zeros).  All units of the call, segment by
-// segment in the order (sequence, key head, row block), are dealt to the
-// workers in runs of equal length (or one more), whatever the lengths are.  A
-// segment that one worker has whole is written by it; of one that is cut, each
-// worker leaves its part in its slot -- the first segment of its run in slot
-// 2 w, else the last in 2 w + 1 -- and combine_kernel joins them in order.
-// (split_supported keeps all counts below 2^31.)
+// without tokens still writes its zeros), and it costs kStart more: the time
+// before a segment's first tokens are there and behind its last, in units
+// (measured: 2.5 us where a unit takes 1.2).  The cost of all segments in the
+// order (sequence, key head, row block), each segment's start in front of its
+// units, is dealt to the workers in runs of equal length (or one more),
+// whatever the sequences' lengths are.  A segment whose units fall to one
+// worker is written by it; of one that is cut, the first of its workers leaves
+// its part in slot 2 w + 1 and each further one (whose run begins with it) in
+// slot 2 w, and combine_kernel joins them in order.  (split_supported keeps
+// all counts below 2^31.)
+constexpr int kStart = 2;
 __device__ __forceinline__ int seq_units(const AttnMask &mk, int b) {
   int n, m;
   seq_lens(mk, b, n, m);
@@ -247,12 +253,12 @@ __device__ __forceinline__ int seq_units(const AttnMask &mk, int b) {
   return blocks > kUnit ? (blocks + kUnit - 1) / kUnit : 1;
 }
 
-// Units of the sequences before b0 (*before) and of all (returned), of one
+// Cost of the sequences before b0 (*before) and of all (returned), of one
 // segment each, by one warp.
-__device__ __forceinline__ int count_units(const AttnMask &mk, int B, int b0, int *before) {
+__device__ __forceinline__ int count_cost(const AttnMask &mk, int B, int b0, int *before) {
   int all = 0, pre = 0;
   for (int b = threadIdx.x & 31; b < B; b += 32) {
-    const int u = seq_units(mk, b);
+    const int u = kStart + seq_units(mk, b);
     all += u;
     pre += b < b0 ? u : 0;
   }
@@ -260,13 +266,13 @@ __device__ __forceinline__ int count_units(const AttnMask &mk, int B, int b0, in
   return __reduce_add_sync(0xffffffffu, all);
 }
 
-// The sequence that holds unit `at`, counting one segment a sequence:
-// *first = units before that sequence.  By one warp.
+// The sequence that holds the place `at`, counting one segment a sequence:
+// *first = cost before that sequence.  By one warp.
 __device__ __forceinline__ int find_seq(const AttnMask &mk, int B, int at, int *first) {
   int base = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
-    const int u = b < B ? seq_units(mk, b) : 0;
+    const int u = b < B ? kStart + seq_units(mk, b) : 0;
     int inc = u;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -285,8 +291,8 @@ __device__ __forceinline__ int find_seq(const AttnMask &mk, int B, int at, int *
   return B;
 }
 
-// The runs: of `total` units, worker w has each = total / workers of them,
-// the first `more` workers one more.  At most as many workers as units.
+// The runs: of a cost of `total`, worker w has each = total / workers, the
+// first `more` workers one more.
 struct Runs {
   int each, more, workers;
   __device__ __forceinline__ Runs(int total, int all) {
@@ -326,11 +332,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
   constexpr int E = X::E, WK = X::WK, VW = X::VW, NU = X::NU, UR = X::UR, UT = X::UT;
   constexpr bool kQuant = BITS < 16;
   constexpr int KS = D / 16;  // k16 steps of a score
-  constexpr int kLd = D + 4;
+  constexpr int kLd = D + 2;
   // the warps' rings, and at a segment's end [kWarps][8 NT][kLd] sums in their place
   extern __shared__ __align__(128) uint8_t smem[];
   float *buf = reinterpret_cast<float *>(smem);
   __shared__ float2 ml[kWarps][8 * NT];
+  __shared__ __align__(16) uint16_t qs[8 * NT][4 * KS * 4];  // the query operand, by row and lane c
+  __shared__ float qfac[8 * NT], qsum[8 * NT][kQuant ? G : 1];
 
   const AttnProblem &P = A.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
@@ -338,13 +346,31 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
   pdl_wait();
   pdl_launch_dependents();  // (after the wait: the next kernel may read the lengths before its own)
   int before;
-  const int total = count_units(P.mask, P.B, 0, &before) * per_seq;
+  const int total = count_cost(P.mask, P.B, 0, &before) * per_seq;
   const Runs runs(total, A.workers);
   if (static_cast<int>(blockIdx.x) >= runs.workers) return;
-  const int run0 = runs.begin(blockIdx.x), run1 = runs.begin(blockIdx.x + 1);
-  int at = run0, seq0;
+  const int run1 = runs.begin(blockIdx.x + 1);
+  int at = runs.begin(blockIdx.x), seq0;
   int b = find_seq(P.mask, P.B, at / per_seq, &seq0);
   seq0 *= per_seq;
+  constexpr int HV = X::HV, kTurns = 32 / HV, kStep = kWarps * HV;
+  auto token0 = [&](const Range &rg, int blk) { return (blk < rg.nsb ? blk : rg.wb0 + blk - rg.nsb) * kTok; };
+  // row of a block's first token among the rows of the pool (dense: of the head)
+  auto look = [&](const Range &rg, int b_at, int hk, int blk, int end) -> uint32_t {
+    if (blk >= end) return kNoBlock;
+    const int t0 = token0(rg, blk);
+    if constexpr (kQuant) {
+      const int page = A.page_shift >= 0 ? t0 >> A.page_shift : t0 / A.pool.page;
+      const int entry = A.table[b_at * A.table_width + page];
+      if (entry < 0 || entry >= A.pool.num_pages) return kNoBlock;
+      return (static_cast<uint32_t>(entry) * P.Hkv + hk) * A.pool.page + (t0 - page * A.pool.page);
+    } else {
+      return t0;
+    }
+  };
+  // the first rows of the next segment, when this one's last are under way
+  uint32_t rows_after = kNoBlock;
+  bool looked = false;
 
   // ---- segment by segment
   while (at < run1) {
@@ -352,39 +378,47 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
     seq_lens(P.mask, b, n, m);
     const Range rg = make_range(P.mask, n, m);
     const int units = rg.blocks > kUnit ? (rg.blocks + kUnit - 1) / kUnit : 1;
-    const int seg = (at - seq0) / units, seg0 = seq0 + seg * units;
+    const int seg = (at - seq0) / (kStart + units), seg0 = seq0 + seg * (kStart + units);
     const int hk = seg / A.row_blocks, rb = seg - hk * A.row_blocks;
-    const int u0 = at - seg0, u1 = run1 - seg0 < units ? run1 - seg0 : units;
+    const int v0 = at - seg0 - kStart, v1 = run1 - seg0 - kStart;
+    const int u0 = v0 > 0 ? v0 : 0, u1 = v1 < units ? v1 : units;
     const int rows = g * rg.m, row0 = rb * 8 * NT;
-    at = seg0 + u1;
+    at = seg0 + kStart + u1;
     const int b_now = b;
     if (seg + 1 == per_seq && u1 == units) {
       seq0 = at;
       ++b;
     }
-    if (row0 >= rows) continue;  // rows behind the sequence's queries: nothing is written
+    const bool had = looked;
+    looked = false;
+    if (u1 <= u0) break;            // the run ends before the segment's first unit
+    if (row0 >= rows) continue;     // rows behind the sequence's queries: nothing is written
 
-    // ---- this warp's blocks of the segment's units [u0, u1)
-    const int beg = u0 * kUnit, end = u1 * kUnit < rg.blocks ? u1 * kUnit : rg.blocks;
-    auto token0 = [&](int blk) { return (blk < rg.nsb ? blk : rg.wb0 + blk - rg.nsb) * kTok; };
-    // row of a block's first token among the rows of the pool (dense: of the head)
-    auto look = [&](int blk) -> uint32_t {
-      if (blk >= end) return kNoBlock;
-      const int t0 = token0(blk);
-      if constexpr (kQuant) {
-        const int page = A.page_shift >= 0 ? t0 >> A.page_shift : t0 / A.pool.page;
-        const int entry = A.table[b_now * A.table_width + page];
-        if (entry < 0 || entry >= A.pool.num_pages) return kNoBlock;
-        return (static_cast<uint32_t>(entry) * P.Hkv + hk) * A.pool.page + (t0 - page * A.pool.page);
-      } else {
-        return t0;
+    // ---- the queries' elements, on their way while the first blocks are sent for: warp w has rows w, w + 4, ..
+    constexpr int kPairs = (D + 63) / 64, kRows = 8 * NT / kWarps;
+    uint32_t qraw[kRows][kPairs];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int R = row0 + warp + kWarps * i;
+      const uint16_t *q = static_cast<const uint16_t *>(P.q.p) + (R < rows ? row_at(P.q, b_now, hk, g, R) : 0);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const int e = 2 * (lane + 32 * k);
+        qraw[i][k] = 0;
+        if (R < rows && e < D)
+          qraw[i][k] = A.q_vec ? *reinterpret_cast<const uint32_t *>(q + e)
+                               : q[e] | static_cast<uint32_t>(q[e + 1]) << 16;
       }
-    };
-    // lane i looks at the i-th of the warp's next 32 blocks
-    constexpr int HV = X::HV, kTurns = 32 / HV, kStep = kWarps * HV;
+    }
+
+    // ---- this warp's blocks of the segment's units [u0, u1); lane i looks at the i-th of the next 32
+    const int beg = u0 * kUnit, end = u1 * kUnit < rg.blocks ? u1 * kUnit : rg.blocks;
     const int first = beg + warp * HV;
-    auto look_ahead = [&](int turn) { return look(first + (turn + lane / HV) * kStep + lane % HV); };
-    uint32_t rows_now = look_ahead(0), rows_next = end - first > kTurns * kStep ? look_ahead(kTurns) : kNoBlock;
+    auto look_ahead = [&](int turn) {
+      return look(rg, b_now, hk, first + (turn + lane / HV) * kStep + lane % HV, end);
+    };
+    uint32_t rows_now = had ? rows_after : look_ahead(0);
+    uint32_t rows_next = end - first > kTurns * kStep ? look_ahead(kTurns) : kNoBlock;
 
     const char *kbase, *vbase;
     int64_t k_sl, v_sl;  // bytes between tokens
@@ -435,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
           }
         }
       } else {
-        const int t0 = token0(blk);
+        const int t0 = token0(rg, blk);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int e = lane + 32 * i, t = e / X::CPR, ch = e % X::CPR;
@@ -479,102 +513,103 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < X::STAGES - 1; ++i) load_turn(smem_at + ring + i * X::STAGE, first + i * kStep, i);
 
-    // ---- queries: B operands, per-column factors and sums
-    uint32_t qf[NT][KS][2];
-    float fcol[NT][2], mq[NT][kQuant ? G : 1][2];
+    // ---- the query operand: each row into shared memory in the order the lanes read it
+#pragma unroll 1
+    for (int i = 0; i < kRows; ++i) {
+      const int row = warp + kWarps * i;
+      float x[kPairs][2], up = 1.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int R = row0 + 8 * nt + r;
-      const bool in = R < rows;
-      const uint16_t *q = static_cast<const uint16_t *>(P.q.p) + (in ? row_at(P.q, b_now, hk, g, R) : 0);
-      uint32_t raw[WK * E / 2];  // this lane's elements, two a word
+      for (int k = 0; k < kPairs; ++k) {
+        uint32_t w = qraw[0][k];
 #pragma unroll
-      for (int i = 0; i < WK * E / 2; ++i) raw[i] = 0;
-      if (in) {
-        if (A.q_vec) {
-#pragma unroll
-          for (int i = 0; i < WK * E / 4; ++i) {
-            const int u = 4 * i / (VW * E);
-            const uint2 x = *reinterpret_cast<const uint2 *>(q + E * c * VW + 3 * u * VW * E + 4 * i);
-            raw[2 * i] = x.x;
-            raw[2 * i + 1] = x.y;
-          }
+        for (int j = 1; j < kRows; ++j) w = i == j ? qraw[j][k] : w;
+        if constexpr (kQuant) {
+          const float2 y = P.dtype == LLK_DTYPE_FP16 ? unpack2<false>(w) : unpack2<true>(w);
+          x[k][0] = y.x;
+          x[k][1] = y.y;
         } else {
-#pragma unroll
-          for (int i = 0; i < WK * E / 2; ++i) {
-            const uint16_t *src = q + E * c * VW + 3 * (2 * i / (VW * E)) * VW * E + 2 * i;
-            raw[i] = src[0] | static_cast<uint32_t>(src[1]) << 16;
-          }
+          x[k][0] = __uint_as_float(w);  // (as it is)
         }
       }
-      float up = 1.f;
       if constexpr (kQuant) {
-        float x[WK * E];
-        if (P.dtype == LLK_DTYPE_FP16) {
-#pragma unroll
-          for (int i = 0; i < WK * E / 2; ++i) {
-            const float2 y = unpack2<false>(raw[i]);
-            x[2 * i] = y.x;
-            x[2 * i + 1] = y.y;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < WK * E / 2; ++i) {
-            const float2 y = unpack2<true>(raw[i]);
-            x[2 * i] = y.x;
-            x[2 * i + 1] = y.y;
-          }
-        }
         // q times a power of two into f16: exact down to 2^-24 of the row's
         // largest element, and 2^-35 of that below
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < WK * E; ++i) top = fmaxf(top, fabsf(x[i]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        for (int k = 0; k < kPairs; ++k) top = fmaxf(top, fmaxf(fabsf(x[k][0]), fabsf(x[k][1])));
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // floor(log2 top)
-        const int k = top > 0.f && ex < 128 ? 9 - ex : 0;
-        up = k > 126 ? 0x1p126f : __uint_as_float(static_cast<uint32_t>(127 + (k < -126 ? -126 : k)) << 23);
-        float sum[G];
+        const int k2 = top > 0.f && ex < 128 ? 9 - ex : 0;
+        up = k2 > 126 ? 0x1p126f : __uint_as_float(static_cast<uint32_t>(127 + (k2 < -126 ? -126 : k2)) << 23);
 #pragma unroll
-        for (int i = 0; i < G; ++i) sum[i] = 0.f;
-#pragma unroll
-        for (int w = 0; w < WK; ++w) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            x[w * E + e] *= up;
-            sum[(w / VW) * 4 * VW * E / X::GROUP] += x[w * E + e];
-          }
-          const float *y = x + w * E;
-          if constexpr (BITS == 4) {
-            qf[nt][2 * w][0] = pack2<false>(y[0], y[4]);
-            qf[nt][2 * w][1] = pack2<false>(y[1] * 0.0625f, y[5] * 0.0625f);
-            qf[nt][2 * w + 1][0] = pack2<false>(y[2], y[6]);
-            qf[nt][2 * w + 1][1] = pack2<false>(y[3] * 0.0625f, y[7] * 0.0625f);
-          } else {
-            qf[nt][w][0] = pack2<false>(y[0], y[2]);
-            qf[nt][w][1] = pack2<false>(y[1], y[3]);
-          }
+        for (int k = 0; k < kPairs; ++k) {
+          x[k][0] *= up;
+          x[k][1] *= up;
         }
-        // the sums in the units of the tensor core's scores, 2^-24 up
+        // each group's sum in the units of the tensor core's scores, 2^-24 up
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-          sum[i] *= 0x1p-24f;
+        for (int gi = 0; gi < G; ++gi) {
+          float sum = 0.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) mq[nt][i][j] = __shfl_sync(0xffffffffu, sum[i], 4 * (2 * c + j));
+          for (int k = 0; k < kPairs; ++k)
+            if (2 * (lane + 32 * k) / X::GROUP == gi) sum += x[k][0] + x[k][1];
+#pragma unroll
+          for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+          if (lane == 0) qsum[row][gi] = sum * 0x1p-24f;
         }
-      } else {
-#pragma unroll
-        for (int w = 0; w < WK; ++w) qf[nt][w / 2][w % 2] = raw[w];
-        mq[nt][0][0] = mq[nt][0][1] = 0.f;
       }
-      const float f = P.scale * kLog2e * (kQuant ? 0x1p24f / up : 1.f);
+      if (lane == 0) qfac[row] = P.scale * kLog2e * (kQuant ? 0x1p24f / up : 1.f);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) fcol[nt][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + j));
+      for (int k = 0; k < kPairs; ++k) {
+        const int e = 2 * (lane + 32 * k);  // even, so e and e + 1 lie in one word
+        if (e < D) {
+          const int word = e / E, in = e % E, lc = word / VW % 4, w = word / (4 * VW) * VW + word % VW;
+          if constexpr (BITS == 4) {
+            // word w's elements (i, i + 4): operand registers 0 (i = 0), 1 (1, held 16 times), 2 (2), 3 (3, 16 times)
+            uint16_t *to = &qs[row][(lc * KS + 2 * w + ((in & 2) >> 1)) * 4 + (in >> 2)];
+            to[0] = __half_as_ushort(__float2half_rn(x[k][0]));
+            to[2] = __half_as_ushort(__float2half_rn(x[k][1] * 0.0625f));
+          } else if constexpr (BITS == 8) {
+            // (0, 2) and (1, 3)
+            uint16_t *to = &qs[row][(lc * KS + w) * 4 + (in >> 1)];
+            to[0] = __half_as_ushort(__float2half_rn(x[k][0]));
+            to[2] = __half_as_ushort(__float2half_rn(x[k][1]));
+          } else {
+            *reinterpret_cast<uint32_t *>(&qs[row][(lc * KS + w / 2) * 4 + 2 * (w % 2)]) = __float_as_uint(x[k][0]);
+          }
+        }
+      }
     }
-
+    __syncthreads();
+    uint32_t qf[NT][KS][2];
+    float fcol[NT][2], mq[NT][kQuant ? G : 1][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(&qs[8 * nt + r][(c * KS + k) * 4]);
+        qf[nt][k][0] = w.x;
+        qf[nt][k][1] = w.y;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        fcol[nt][j] = qfac[8 * nt + 2 * c + j];
+#pragma unroll
+        for (int gi = 0; gi < (kQuant ? G : 1); ++gi) mq[nt][gi][j] = kQuant ? qsum[8 * nt + 2 * c + j][gi] : 0.f;
+      }
+    }
+    if (kQuant && u1 == units && at < run1) {
+      // the run goes on: look at the next segment's first blocks now (kStep at a time, like this one's)
+      int n2, m2;
+      seq_lens(P.mask, b, n2, m2);
+      const Range r2 = make_range(P.mask, n2, m2);
+      const int units2 = r2.blocks > kUnit ? (r2.blocks + kUnit - 1) / kUnit : 1;
+      const int v2 = run1 - at - kStart, e2 = v2 < units2 ? v2 * kUnit : r2.blocks;
+      const int seg2 = b != b_now ? 0 : seg + 1;
+      rows_after = look(r2, b, seg2 / A.row_blocks, (warp + lane / HV * kWarps) * HV + lane % HV,
+                        e2 < r2.blocks ? e2 : r2.blocks);
+      looked = true;
+    }
     float acc[X::TILES][NT][4], mrun[NT][2], l[NT][2], pm[NT][kQuant ? G : 1][2];
 #pragma unroll
     for (int t = 0; t < X::TILES; ++t)
@@ -607,6 +642,18 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
         rows_now = rows_next;
         rows_next = look_ahead((blk - first) / kStep + 1 + kTurns);
       }
+      if (kQuant && looked && blk == first) {
+        // the next segment's first turns into L2
+#pragma unroll
+        for (int i = 0; i < (X::STAGES - 1) * HV; ++i) {
+          const uint32_t row = __shfl_sync(0xffffffffu, rows_after, i);
+          constexpr int kLines = kTok * X::ROWB / 128;
+          if (row != kNoBlock && (lane & 15) < kLines) {
+            const char *at_l2 = (lane < 16 ? kbase : vbase) + static_cast<int64_t>(row) * X::ROWB + (lane & 15) * 128;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(at_l2));
+          }
+        }
+      }
       const uint32_t absent = none >> ((X::STAGES - 1) * HV);
       const bool full = blk >= rg.full0 && blk + HV <= rg.full1 && (absent & ((1u << HV) - 1)) == 0;
       float z[HV][NT][4], sr[HV][2][kQuant ? G : 1], mr[HV][2][kQuant ? G : 1], rs[HV][2];
@@ -630,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
             // parameters of tokens that no query sees may be anything: here scale 1, min 0
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const bool in = !(absent >> (HV - 1 - hv) & 1) && seen(token0(blk + hv) + tr + 8 * i);
+              const bool in = !(absent >> (HV - 1 - hv) & 1) && seen(token0(rg, blk + hv) + tr + 8 * i);
 #pragma unroll
               for (int w = 0; w < 2 * G; ++w) par[i][w] = in ? par[i][w] : 0x3f80u;
             }
@@ -728,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
         }
         // masks: only turns at an edge of some row's range compare token by token
         if (!full) {
-          const int t0 = token0(blk + hv);
+          const int t0 = token0(rg, blk + hv);
           const bool gone = absent >> (HV - 1 - hv) & 1;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -899,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
     __syncthreads();
     // ---- out: the row's result, or this worker's part of it
     const bool whole = u0 == 0 && u1 == units;
-    const int64_t slot = 2 * blockIdx.x + (seg0 + u0 == run0 ? 0 : 1);
+    const int64_t slot = 2 * blockIdx.x + (u0 == 0 ? 1 : 0);
     for (int col = warp; col < 8 * NT; col += kWarps) {
       const int R = row0 + col;
       if (R >= rows) break;
@@ -959,16 +1006,15 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
   // when it has waited for the kernels before it, so the lengths are there.
   int n, m, before;
   seq_lens(P.mask, b, n, m);
-  const int total = count_units(P.mask, P.B, b, &before) * per_seq;
+  const int total = count_cost(P.mask, P.B, b, &before) * per_seq;
   const Runs runs(total, A.workers);
   const int units = seq_units(P.mask, b);
-  const int seg0 = before * per_seq + (hk * A.row_blocks + R / nrows) * units;
-  const int w0 = runs.worker_of(seg0), w1 = runs.worker_of(seg0 + units - 1);
+  const int first = before * per_seq + (hk * A.row_blocks + R / nrows) * (kStart + units) + kStart;
+  const int w0 = runs.worker_of(first), w1 = runs.worker_of(first + units - 1);
   // whole: its worker writes it; rows behind the queries: nobody
   const bool cut = w0 != w1 && R < g * m;
-  // the segment is the first of every run but w0's, where it is the last (or the first too)
-  const int col = R % nrows, late = runs.begin(w0) != seg0 ? 1 : 0;
-  auto slot = [&](int w) { return static_cast<int64_t>(2 * w + (w == w0 ? late : 0)) * nrows + col; };
+  const int col = R % nrows;
+  auto slot = [&](int w) { return static_cast<int64_t>(2 * w + (w == w0 ? 1 : 0)) * nrows + col; };
   pdl_launch_dependents();
   pdl_wait();
   if (!cut) return;
@@ -1039,12 +1085,24 @@ template <int BITS, int D, int G, bool kBf16, int NT>
 cudaError_t launch_split(const Params &a, cudaStream_t stream) {
   using X = Geo<BITS, D, G>;
   constexpr int CTAS = ctas_per_sm(BITS, D, G, NT);
-  constexpr int sums = kWarps * 8 * NT * (D + 4) * static_cast<int>(sizeof(float));
+  constexpr int sums = kWarps * 8 * NT * (D + 2) * static_cast<int>(sizeof(float));
   constexpr int rings = kWarps * X::STAGES * X::STAGE;
   constexpr int smem = sums > rings ? sums : rings;
   auto kern = split_kernel<BITS, D, G, kBf16, NT, CTAS>;
-  cudaError_t e = cudaSuccess;
-  if (smem + 1024 > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  auto join = combine_kernel<D, kBf16, BITS == 16>;
+  // Once a device.  Both kernels ask for the largest shared memory: while one
+  // drains and the next one's CTAs move in, an SM cannot change its split of
+  // shared memory and L1, and would hold fewer of them.
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && !(ready.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(join, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  }
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -1061,7 +1119,7 @@ cudaError_t launch_split(const Params &a, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.p.B) * a.p.H * a.p.mask.Lq;
     cfg.gridDim = dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps));
     cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, combine_kernel<D, kBf16, BITS == 16>, a, 8 * NT);
+    e = cudaLaunchKernelEx(&cfg, join, a, 8 * NT);
   }
   return e != cudaSuccess ? e : cudaGetLastError();
 }
