@@ -7,12 +7,20 @@
 // both quotients as in 64 bits; the group stands for s * code + m.  With 4
 // bits the elements 2j and 2j + 1 share byte j (2j in the low nibble).
 //
-// HBM-bound both ways: a thread owns 8 elements of a row (one 16-byte load
-// for 16-bit types), a row is D / 8 neighbouring lanes, the group's minimum
-// and maximum are shuffles.  Codes next to a border between two (|q - k -
-// 1/2| below the f32 quotient's error, the exact ties of 16-bit inputs among
-// them) are decided by the sign of x - m - (k + 1/2) s in f64, so the codes do
-// not depend on how the quotient was rounded.
+// HBM-bound both ways; what there is to save is instructions.  A thread owns
+// 8 elements of a row (one 16-byte load for 16-bit types), a row is D / 8
+// neighbouring lanes.  A CTA first works out where its tokens lie, once for
+// all heads.  Writing: the group's minimum and maximum are packed 16-bit
+// operations and shuffles of the pair (min, -max); the quotient (x - m) / s is
+// a product with 1 / s and one correction by its remainder, which makes it
+// exact wherever the quotient is a tie between two codes (the remainder is
+// exact, and so is the corrected quotient when it is representable), so
+// rounding to even by adding 1.5 * 2^23 settles the ties of 16-bit inputs;
+// quotients nearer to a tie than the f32 error without surely being one go by the
+// sign of x - m - (k + 1/2) s.  Codes are put together as f32 sums (exact below
+// 2^24), two chains at a time in packed f32 operations.  Reading: a nibble is
+// masked into the mantissa of 2^23 where it lies, so that a subtraction makes
+// it code * 16^i, and one fused multiply-add with scale / 16^i the value.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -28,216 +36,436 @@ constexpr int kBitmapWords = 1024;    // 32768 bits over the low bits of the CTA
 constexpr float kLargest = 65504.f;
 constexpr double kLeastScale = 0x1p-30;
 
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Eight elements of a row as they lie.
 template <typename T>
-__device__ __forceinline__ void load_elems(const T *src, bool vec, float (&x)[8]) {
+struct Eight {
+  uint32_t w[2 * sizeof(T)];
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *src, bool vec, Eight<T> &x) {
   if (vec) {
-    constexpr int kPieces = sizeof(T) * 8 / 16;
-    uint4 w[kPieces];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) w[i] = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
-    const T *e = reinterpret_cast<const T *>(w);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+      const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
+      x.w[4 * i] = v.x;
+      x.w[4 * i + 1] = v.y;
+      x.w[4 * i + 2] = v.z;
+      x.w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+    for (int i = 0; i < 4; ++i) x.w[i] = e[2 * i] | static_cast<uint32_t>(e[2 * i + 1]) << 16;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(src[i]);
+    for (int i = 0; i < 8; ++i) x.w[i] = __float_as_uint(src[i]);
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void store_elems(T *dst, bool vec, const float (&x)[8]) {
-  T e[8];
+__device__ __forceinline__ void widen(const Eight<T> &x, float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
-  if (vec) {
-    constexpr int kPieces = sizeof(T) * 8 / 16;
-    uint4 w[kPieces];
-    memcpy(w, e, sizeof(w));
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4 *>(dst)[i] = w[i];
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x.w[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dst[i] = e[i];
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&x.w[i]));
+        f[2 * i] = y.x;
+        f[2 * i + 1] = y.y;
+      } else {
+        f[2 * i] = __uint_as_float(x.w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(x.w[i] & 0xffff0000u);
+      }
+    }
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *dst, bool vec, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    if (vec) {
+      reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      return;
+    }
+  } else if (vec) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(w[i]) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
+      } else {
+        asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(w[i]) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
+      }
+    }
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dst[i] = from_f32<T>(x[i]);
+}
+
+// Smallest and largest of a group: (min, max) over the gl lanes that share it.
+// NaN if the group holds one.
+template <typename T>
+__device__ __forceinline__ float2 group_range(const Eight<T> &x, int gl) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2 *p = reinterpret_cast<const T2 *>(x.w);
+    T2 mn = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
+    T2 mx = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    // both halves' minima with both halves' negated maxima
+    mx = __hneg2(mx);
+    const uint32_t a = *reinterpret_cast<const uint32_t *>(&mn), b = *reinterpret_cast<const uint32_t *>(&mx);
+    const uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a, b, 0x7632);
+    T2 r = __hmin2_nan(*reinterpret_cast<const T2 *>(&lo), *reinterpret_cast<const T2 *>(&hi));
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&r), off);
+      const T2 both = __hmin2_nan(r, *reinterpret_cast<const T2 *>(&o));
+      if (off < gl) r = both;
+    }
+    return make_float2(to_f32(r.x), -to_f32(r.y));
+  } else {
+    float mn = INFINITY, mx = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = __uint_as_float(x.w[i]);
+      mn = fminf(mn, f);
+      mx = fmaxf(mx, f);
+      nan |= f != f;
+    }
+    if (nan) mn = NAN;
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      const float a = __shfl_xor_sync(0xffffffffu, mn, off), c = __shfl_xor_sync(0xffffffffu, mx, off);
+      if (off < gl) {
+        mn = a != a || mn != mn ? NAN : fminf(mn, a);
+        mx = fmaxf(mx, c);
+      }
+    }
+    return make_float2(mn, mx);
+  }
+}
+
+// scale = bf16(f32(max((mx - m) / top, 2^-30))), the quotient as in 64 bits: in
+// f32 first, in f64 where that lies next to the middle of two bf16.
+template <int BITS>
+__device__ __forceinline__ __nv_bfloat16 scale_of(float mx, float m) {
+  constexpr float kTop = static_cast<float>((1 << BITS) - 1);
+  const float q = (mx - m) * (1.f / kTop);
+  if (q > 0x1p-29f && abs(static_cast<int>(__float_as_uint(q) & 0xffffu) - 0x8000) > 8) return __float2bfloat16_rn(q);
+  const double d = (static_cast<double>(mx) - static_cast<double>(m)) / static_cast<double>(kTop);
+  return __float2bfloat16_rn(static_cast<float>(d < kLeastScale ? kLeastScale : d));
 }
 
 // Codes of one lane's 8 elements (packed, BITS bytes) and its group's
-// (scale, min); gl lanes share a group.
-template <int BITS>
-__device__ __forceinline__ uint64_t quantise8(float (&x)[8], int gl, uint32_t *param) {
+// (scale, min).
+template <typename T, int BITS>
+__device__ __forceinline__ uint64_t quantise8(const Eight<T> &raw, int gl, uint32_t *param) {
   constexpr float kTop = static_cast<float>((1 << BITS) - 1);
-  float mn = INFINITY, mx = -INFINITY;
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+  float x[8];
+  widen(raw, x);
+  float2 range = group_range(raw, gl);
+  if (__any_sync(0xffffffffu, !(range.x >= -kLargest && range.y <= kLargest))) {
+    // some value is not finite or too large
+    float mn = INFINITY, mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kLargest), kLargest);
-    mn = fminf(mn, x[i]);
-    mx = fmaxf(mx, x[i]);
-  }
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) {
-    const float a = __shfl_xor_sync(0xffffffffu, mn, off), c = __shfl_xor_sync(0xffffffffu, mx, off);
-    if (off < gl) {
-      mn = fminf(mn, a);
-      mx = fmaxf(mx, c);
+    for (int i = 0; i < 8; ++i) {
+      x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kLargest), kLargest);
+      mn = fminf(mn, x[i]);
+      mx = fmaxf(mx, x[i]);
     }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      const float a = __shfl_xor_sync(0xffffffffu, mn, off), c = __shfl_xor_sync(0xffffffffu, mx, off);
+      if (off < gl) {
+        mn = fminf(mn, a);
+        mx = fmaxf(mx, c);
+      }
+    }
+    range = make_float2(mn, mx);
   }
-  const __nv_bfloat16 mb = __float2bfloat16_rn(mn);
+  const __nv_bfloat16 mb = __float2bfloat16_rn(range.x);
   const float m = __bfloat162float(mb);
-  const double q = (static_cast<double>(mx) - static_cast<double>(m)) / static_cast<double>((1 << BITS) - 1);
-  const __nv_bfloat16 sb = __float2bfloat16_rn(static_cast<float>(q < kLeastScale ? kLeastScale : q));
+  const __nv_bfloat16 sb = scale_of<BITS>(range.y, m);
   const float s = __bfloat162float(sb), inv = 1.f / s;
   *param = static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | (static_cast<uint32_t>(__bfloat16_as_ushort(mb)) << 16);
-  uint64_t codes = 0;
-  // error of the f32 quotient: three roundings of 2^-24 on at most 2^BITS
-  constexpr float kNear = static_cast<float>(1 << BITS) * 0x1p-21f;
+  const uint64_t m2 = f32x2(-m, -m), inv2 = f32x2(inv, inv), s2 = f32x2(-s, -s), round2 = f32x2(kRound, kRound),
+                 unround2 = f32x2(-kRound, -kRound), one2 = f32x2(-1.f, -1.f);
+  // error of the corrected quotient: an ulp of at most 2^BITS + 1 (and of x - m, 2^-24 of it)
+  constexpr float kNear = static_cast<float>(1 << BITS) * 0x1p-22f, kLo = (0.5f - kNear) * (0.5f - kNear);
+  uint64_t k[4], r2[4];  // of the elements i and i + 4: codes, squared distances to them
+  bool near = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = (x[i] - m) * inv;
-    const float k = floorf(v), f = v - k;
-    float c = f > 0.5f ? k + 1.f : k;
-    if (fabsf(f - 0.5f) < kNear) {
-      const double d = (static_cast<double>(x[i]) - static_cast<double>(m)) -
-                       (static_cast<double>(k) + 0.5) * static_cast<double>(s);
-      c = d > 0.0 || (d == 0.0 && (static_cast<int>(k) & 1)) ? k + 1.f : k;
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t d = add2(f32x2(x[i], x[i + 4]), m2);
+    uint64_t q = mul2(d, inv2);
+    q = fma2(fma2(q, s2, d), inv2, q);
+    // (a lower bound only where m may lie above the smallest element, an upper
+    // one only where the scale's rounding can push the largest past the top)
+    constexpr bool kLow = !std::is_same<T, __nv_bfloat16>::value, kHigh = BITS == 8;
+    if constexpr (kLow || kHigh) {
+      float2 c = split2(q);
+      if constexpr (kLow) c = make_float2(fmaxf(c.x, 0.f), fmaxf(c.y, 0.f));
+      if constexpr (kHigh) c = make_float2(fminf(c.x, kTop), fminf(c.y, kTop));
+      q = f32x2(c.x, c.y);
     }
-    c = fminf(fmaxf(c, 0.f), kTop);
-    codes |= static_cast<uint64_t>(static_cast<uint32_t>(c)) << (BITS * i);
+    k[i] = add2(add2(q, round2), unround2);
+    const uint64_t r = fma2(k[i], one2, q);
+    r2[i] = mul2(r, r);
+    const float2 e = split2(r2[i]);
+    near |= e.x > kLo || e.y > kLo;
   }
-  return codes;
+  if (near && sizeof(T) == 2) {
+    // A tie is settled, if x - m is exact: 8 (f16: 11) and 8 bits no more than
+    // 24 bits apart.
+    constexpr float kApart = std::is_same<T, __half>::value ? 0x1p-11f : 0x1p-14f;
+    near = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 e = split2(r2[i % 4]);
+      const float ri = i < 4 ? e.x : e.y, ax = fabsf(x[i]), am = fabsf(m);
+      const bool exact = (ax >= am * kApart && am >= ax * kApart) || ax == 0.f || am == 0.f;
+      near |= ri > kLo && !(ri == 0.25f && exact);
+    }
+  }
+  if (near) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float c[2];
+      const float2 kk = split2(k[i]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // x - m = d + e exactly; against the border on the quotient's side of k
+        const float xi = x[i + 4 * j], d = xi - m, t = d - xi, e = (xi - (d - t)) - (m + t);
+        const float k0 = j ? kk.y : kk.x, q = d * inv;
+        const float lo = q < k0 ? k0 - 1.f : k0;  // the border between lo and lo + 1
+        const float side = fmaf(-(lo + 0.5f), s, d) + e;
+        c[j] = side > 0.f || (side == 0.f && (static_cast<int>(lo) & 1)) ? lo + 1.f : lo;
+        c[j] = fminf(fmaxf(c[j], 0.f), kTop);
+      }
+      k[i] = f32x2(c[0], c[1]);
+    }
+  }
+  const uint64_t base2 = f32x2(0x1p23f, 0x1p23f);
+  if constexpr (BITS == 4) {
+    const uint64_t by16 = f32x2(16.f, 16.f);
+    const uint64_t c = add2(fma2(fma2(fma2(k[3], by16, k[2]), by16, k[1]), by16, k[0]), base2);
+    return __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(c >> 32), 0x5410);
+  } else {
+    const uint64_t by256 = f32x2(256.f, 256.f);
+    const uint64_t c0 = add2(fma2(k[1], by256, k[0]), base2), c1 = add2(fma2(k[3], by256, k[2]), base2);
+    return __byte_perm(static_cast<uint32_t>(c0), static_cast<uint32_t>(c1), 0x5410) |
+           static_cast<uint64_t>(__byte_perm(static_cast<uint32_t>(c0 >> 32), static_cast<uint32_t>(c1 >> 32), 0x5410))
+               << 32;
+  }
 }
 
-// Writer.  CTA: `tokens` tokens (blockIdx.x) of `pairs` (tensor, head) pairs
-// (blockIdx.y); row = pair * tokens + token.  The same slot twice in a call:
-// the CTA looks through all later tokens' slots (a bitmap over its own slots
-// rules nearly all of them out) and leaves out its tokens that a later one
-// overwrites, so a slot holds its last token whatever order the CTAs run in.
+// The 8 values of a lane.
+template <int BITS>
+__device__ __forceinline__ void values8(uint64_t codes, uint32_t param, float (&x)[8]) {
+  const float s = __uint_as_float(param << 16), m = __uint_as_float(param & 0xffff0000u);
+  const uint64_t m2 = f32x2(m, m), base2 = f32x2(-0x1p23f, -0x1p23f);
+  constexpr int kIn = 16 / BITS;  // codes of a 16-bit piece
+#pragma unroll
+  for (int h = 0; h < 8 / kIn; h += 2) {
+    // pieces h and h + 1, code i of both at once
+    const uint32_t w = static_cast<uint32_t>(codes >> (16 * h)), v = w >> 16;
+#pragma unroll
+    for (int i = 0; i < kIn; ++i) {
+      const uint32_t mask = ((1u << BITS) - 1) << (BITS * i);
+      const uint64_t c = add2(f32x2(__uint_as_float((w & mask) | 0x4b000000u), __uint_as_float((v & mask) | 0x4b000000u)),
+                              base2);
+      const float si = s * (1.f / static_cast<float>(1 << (BITS * i)));
+      const float2 y = split2(fma2(c, f32x2(si, si), m2));
+      x[h * kIn + i] = y.x;
+      x[(h + 1) * kIn + i] = y.y;
+    }
+  }
+}
+
+struct Move {
+  KvPool pool;
+  View4 k, v;
+  const int64_t *slots;
+  uint32_t n_tokens, L;  // B L, L
+  int tokens, shift;     // of a CTA, a power of two
+  int pairs;             // (tensor, head) pairs of a CTA
+  int page_shift;        // log2 of the page, or -1
+  int vec;
+};
+
+// Where a CTA's tokens lie: rows of the dense tensors (element offsets at head
+// 0) and of the pool (at head 0; -1: nowhere).
+struct Place {
+  int64_t k, v, row;
+};
+
+__device__ __forceinline__ int64_t pool_row(const Move &A, int64_t s) {
+  if (s < 0 || s >= A.pool.num_pages * A.pool.page) return -1;
+  const int64_t page = A.page_shift >= 0 ? s >> A.page_shift : s / A.pool.page;
+  return page * A.pool.Hkv * A.pool.page + (s - page * A.pool.page);
+}
+
+__device__ __forceinline__ Place place(const Move &A, uint32_t n) {
+  const uint32_t b = n / A.L, l = n - b * A.L;
+  return {b * A.k.sb + l * A.k.sl, b * A.v.sb + l * A.v.sl, pool_row(A, A.slots[n])};
+}
+
+// Writer.  CTA: `tokens` tokens (blockIdx.x) of `pairs` pairs (blockIdx.y);
+// row = pair * tokens + token.  The same slot twice in a call: the CTA looks
+// through all later tokens' slots (a bitmap over its own slots rules nearly
+// all of them out) and leaves out its tokens that a later one overwrites, so a
+// slot holds its last token whatever order the CTAs run in.
 template <typename T, int BITS>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvPool P, const View4 K, const View4 V,
-                                                            const int64_t *__restrict__ slots, uint32_t n_tokens,
-                                                            uint32_t L, int tokens, int pairs, int vec) {
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ Move A) {
+  __shared__ Place at[kMaxTokens];
   __shared__ int64_t slot[kMaxTokens];
   __shared__ uint32_t bitmap[kBitmapWords];
-  const uint32_t n0 = blockIdx.x * tokens;
-  const int cnt = n_tokens - n0 < static_cast<uint32_t>(tokens) ? static_cast<int>(n_tokens - n0) : tokens;
-  const int64_t n_slots = P.num_pages * P.page;
+  const KvPool &P = A.pool;
+  const uint32_t n0 = blockIdx.x * A.tokens, n_tokens = A.n_tokens;
+  const int cnt = n_tokens - n0 < static_cast<uint32_t>(A.tokens) ? static_cast<int>(n_tokens - n0) : A.tokens;
   if (n_tokens > 1)
     for (int i = threadIdx.x; i < kBitmapWords; i += kThreads) bitmap[i] = 0;
   __syncthreads();
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   if (threadIdx.x < cnt) {
-    const int64_t s = slots[n0 + threadIdx.x];
-    const bool ok = s >= 0 && s < n_slots;
-    slot[threadIdx.x] = ok ? s : -1;
-    if (ok && n_tokens > 1) atomicOr(&bitmap[(s >> 5) & (kBitmapWords - 1)], 1u << (s & 31));
+    const Place p = place(A, n0 + threadIdx.x);
+    const int64_t s = p.row >= 0 ? A.slots[n0 + threadIdx.x] : -1;
+    at[threadIdx.x] = p;
+    slot[threadIdx.x] = s;
+    if (s >= 0 && n_tokens > 1) atomicOr(&bitmap[(s >> 5) & (kBitmapWords - 1)], 1u << (s & 31));
   }
   __syncthreads();
-  for (uint32_t n = n0 + 1 + threadIdx.x; n < n_tokens; n += kThreads) {
-    const int64_t s = slots[n];
-    if (s < 0 || s >= n_slots || !(bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1)) continue;
-    const int before = n - n0 < static_cast<uint32_t>(cnt) ? static_cast<int>(n - n0) : cnt;
-    for (int t = 0; t < before; ++t)
-      if (slot[t] == s) slot[t] = -1;  // only ever set to -1 here: threads agree, and a later equal token remains
+  if (n_tokens > 1) {
+    const int64_t n_slots = P.num_pages * P.page;
+    for (uint32_t n = n0 + 1 + threadIdx.x; n < n_tokens; n += kThreads) {
+      const int64_t s = A.slots[n];
+      if (s < 0 || s >= n_slots || !(bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1)) continue;
+      const int before = n - n0 < static_cast<uint32_t>(cnt) ? static_cast<int>(n - n0) : cnt;
+      for (int t = 0; t < before; ++t)
+        if (slot[t] == s) at[t].row = -1;  // (whoever finds it writes the same)
+    }
+    __syncthreads();
   }
-  __syncthreads();
 
-  const int lpr = P.D / 8;  // lanes a row
-  const int rows = cnt * pairs, l = threadIdx.x % lpr;
+  const int lpr = P.D / 8, l = threadIdx.x & (lpr - 1);  // lanes a row
+  const int rows = A.tokens * A.pairs;
   const int gl = P.group / 8, groups = P.D / P.group;
-  const int64_t row_bytes = P.D * BITS / 8;
-  constexpr int kU = 4;  // rows in flight a thread
-  const int step = kThreads / lpr;
+  constexpr int kU = sizeof(T) == 4 ? 2 : 4;  // rows in flight a thread
+  const int step = kThreads / lpr, mine = threadIdx.x / lpr;
   // every lane runs every round (the group's shuffles take the whole warp)
   for (int r0 = 0; r0 < rows; r0 += kU * step) {
-    float x[kU][8];
-    int64_t at[kU];
-    int which[kU];
+    Eight<T> x[kU];
+    int64_t row[kU];
+    bool is_v[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int r = r0 + u * step + threadIdx.x / lpr;
-      at[u] = -1;
-      which[u] = 0;
+      const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
+      is_v[u] = pair >= P.Hkv;
+      const int h = is_v[u] ? pair - P.Hkv : pair;
+      row[u] = r < rows && t < cnt ? at[t].row : -1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
-      if (r < rows) {
-        const int pair = blockIdx.y * pairs + r / cnt, t = r % cnt;
-        const int64_t s = slot[t];
-        which[u] = pair >= P.Hkv;
-        const int h = which[u] ? pair - P.Hkv : pair;
-        if (s >= 0) {
-          const View4 &src = which[u] ? V : K;
-          const uint32_t n = n0 + t, b = n / L;
-          load_elems(static_cast<const T *>(src.p) + b * src.sb + h * src.sh + (n - b * L) * src.sl + 8 * l, vec,
-                     x[u]);
-          at[u] = (s / P.page * P.Hkv + h) * P.page + s % P.page;
-        }
+      for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) x[u].w[i] = 0;
+      if (row[u] >= 0) {
+        const View4 &src = is_v[u] ? A.v : A.k;
+        load8(static_cast<const T *>(src.p) + (is_v[u] ? at[t].v : at[t].k) + h * src.sh + 8 * l, A.vec, x[u]);
+        row[u] += static_cast<int64_t>(h) * P.page;
       }
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       uint32_t param;
-      const uint64_t codes = quantise8<BITS>(x[u], gl, &param);
-      if (at[u] < 0) continue;
-      uint8_t *dst = static_cast<uint8_t *>(which[u] ? P.v_codes : P.k_codes) + at[u] * row_bytes + BITS * l;
+      const uint64_t codes = quantise8<T, BITS>(x[u], gl, &param);
+      if (row[u] < 0) continue;
+      uint8_t *dst = static_cast<uint8_t *>(is_v[u] ? P.v_codes : P.k_codes) + row[u] * (P.D * BITS / 8) + BITS * l;
       if constexpr (BITS == 4) {
         *reinterpret_cast<uint32_t *>(dst) = static_cast<uint32_t>(codes);
       } else {
         *reinterpret_cast<uint64_t *>(dst) = codes;
       }
-      if (l % gl == 0) static_cast<uint32_t *>(which[u] ? P.v_params : P.k_params)[at[u] * groups + l / gl] = param;
+      if ((l & (gl - 1)) == 0)
+        static_cast<uint32_t *>(is_v[u] ? P.v_params : P.k_params)[row[u] * groups + l / gl] = param;
     }
   }
 }
 
-// Reader.  A thread turns the codes of 8 elements into values, one fused
-// multiply-add each (s * code is exact in f32); rows in the order of the
-// output, kU of them in flight a thread.
+// Reader.  CTAs as the writer's.
 template <typename T, int BITS>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvPool P, const View4 K, const View4 V,
-                                                           const int64_t *__restrict__ slots, uint32_t n_rows,
-                                                           uint32_t B, uint32_t L, int vec) {
-  const int64_t n_slots = P.num_pages * P.page;
-  const int lpr = P.D / 8, l = threadIdx.x % lpr, gl = P.group / 8, groups = P.D / P.group;
-  const int64_t row_bytes = P.D * BITS / 8;
-  constexpr int kU = 4;
-  const uint32_t step = kThreads / lpr;
-  pdl_launch_dependents();
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ Move A) {
+  __shared__ Place at[kMaxTokens];
+  const KvPool &P = A.pool;
+  const uint32_t n0 = blockIdx.x * A.tokens;
+  const int cnt = A.n_tokens - n0 < static_cast<uint32_t>(A.tokens) ? static_cast<int>(A.n_tokens - n0) : A.tokens;
   pdl_wait();
-  const uint32_t r0 = blockIdx.x * (kU * step) + threadIdx.x / lpr;
-  uint64_t codes[kU];
-  uint32_t param[kU];
-  int64_t dst[kU];
+  pdl_launch_dependents();
+  if (threadIdx.x < cnt) at[threadIdx.x] = place(A, n0 + threadIdx.x);
+  __syncthreads();
+  const int lpr = P.D / 8, l = threadIdx.x & (lpr - 1);
+  const int rows = A.tokens * A.pairs;
+  const int gl = P.group / 8, groups = P.D / P.group;
+  constexpr int kU = 8;
+  const int step = kThreads / lpr, mine = threadIdx.x / lpr;
+  for (int r0 = 0; r0 < rows; r0 += kU * step) {
+    uint64_t codes[kU];
+    uint32_t param[kU];
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const uint32_t r = r0 + u * step;
-    codes[u] = 0;
-    param[u] = 0;
-    dst[u] = -1;
-    if (r >= n_rows) continue;
-    // r = ((which * B + b) * Hkv + h) * L + t
-    const uint32_t t = r % L, wbh = r / L, h = wbh % P.Hkv, wb = wbh / P.Hkv;
-    const bool isv = wb >= B;
-    const uint32_t b = isv ? wb - B : wb;
-    const View4 &out = isv ? V : K;
-    dst[u] = b * out.sb + h * out.sh + t * out.sl + 8 * l;
-    const int64_t s = slots[static_cast<int64_t>(b) * L + t];
-    if (s < 0 || s >= n_slots) continue;  // reads as zeros
-    const int64_t at = (s / P.page * P.Hkv + h) * P.page + s % P.page;
-    const uint8_t *src = static_cast<const uint8_t *>(isv ? P.v_codes : P.k_codes) + at * row_bytes + BITS * l;
-    codes[u] = BITS == 4 ? *reinterpret_cast<const uint32_t *>(src) : *reinterpret_cast<const uint64_t *>(src);
-    param[u] = static_cast<const uint32_t *>(isv ? P.v_params : P.k_params)[at * groups + l / gl];
-  }
+    for (int u = 0; u < kU; ++u) {
+      const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
+      const bool is_v = pair >= P.Hkv;
+      codes[u] = 0;
+      param[u] = 0;  // a slot outside the cache reads as zeros
+      if (r < rows && t < cnt && at[t].row >= 0) {
+        const int64_t row = at[t].row + static_cast<int64_t>(is_v ? pair - P.Hkv : pair) * P.page;
+        const uint8_t *src = static_cast<const uint8_t *>(is_v ? P.v_codes : P.k_codes) + row * (P.D * BITS / 8) + BITS * l;
+        codes[u] = BITS == 4 ? *reinterpret_cast<const uint32_t *>(src) : *reinterpret_cast<const uint64_t *>(src);
+        param[u] = static_cast<const uint32_t *>(is_v ? P.v_params : P.k_params)[row * groups + l / gl];
+      }
+    }
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const uint32_t r = r0 + u * step;
-    if (r >= n_rows) continue;
-    const bool isv = r / L / P.Hkv >= B;
-    const float s = __uint_as_float(param[u] << 16), m = __uint_as_float(param[u] & 0xffff0000u);
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = fmaf(s, static_cast<float>(static_cast<uint32_t>(codes[u] >> (BITS * i)) & ((1u << BITS) - 1)), m);
-    store_elems(static_cast<T *>(isv ? V.p : K.p) + dst[u], vec, x);
+    for (int u = 0; u < kU; ++u) {
+      const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
+      if (r >= rows || t >= cnt) continue;
+      const bool is_v = pair >= P.Hkv;
+      const View4 &out = is_v ? A.v : A.k;
+      float x[8];
+      values8<BITS>(codes[u], param[u], x);
+      store8(static_cast<T *>(out.p) + (is_v ? at[t].v : at[t].k) + (is_v ? pair - P.Hkv : pair) * out.sh + 8 * l, A.vec,
+             x);
+    }
   }
 }
 
@@ -246,46 +474,53 @@ bool rows_on_16_bytes(const View4 &v, int64_t el) {
          v.sl * el % 16 == 0;
 }
 
-template <typename... Args>
-cudaError_t launch(void (*kern)(Args...), dim3 grid, cudaStream_t stream, Args... args) {
+template <typename T>
+cudaError_t move_t(bool write, const KvPool &p, const View4 &k, const View4 &v, int64_t B, int64_t L,
+                   const int64_t *slots, int sm_count, cudaStream_t stream) {
+  Move a = {};
+  a.pool = p;
+  a.k = k;
+  a.v = v;
+  a.slots = slots;
+  a.n_tokens = static_cast<uint32_t>(B * L);
+  a.L = static_cast<uint32_t>(L);
+  a.vec = rows_on_16_bytes(k, sizeof(T)) && rows_on_16_bytes(v, sizeof(T));
+  a.page_shift = -1;
+  for (int i = 4; i < 17; ++i)
+    if (p.page == 1 << i) a.page_shift = i;
+  // A writer's CTA looks through all later slots, so few of them should: a
+  // CTA takes many tokens and all heads, as long as the GPU is filled a few
+  // times over; then it takes fewer tokens, then fewer heads.
+  const int64_t n = B * L;
+  int ysplit = 1;
+  a.shift = 6;
+  auto ctas = [&] { return ((n + (1 << a.shift) - 1) >> a.shift) * ysplit; };
+  while (ctas() < 4 * sm_count && a.shift > 4) --a.shift;
+  while (ctas() < 4 * sm_count && 2 * p.Hkv % (2 * ysplit) == 0) ysplit *= 2;
+  while (ctas() < 4 * sm_count && a.shift > 0) --a.shift;
+  a.tokens = 1 << a.shift;
+  a.pairs = 2 * p.Hkv / ysplit;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3(static_cast<unsigned>((n + a.tokens - 1) >> a.shift), static_cast<unsigned>(ysplit));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  const cudaError_t e =
+      write ? cudaLaunchKernelEx(&cfg, p.bits == 4 ? kv_write_kernel<T, 4> : kv_write_kernel<T, 8>, a)
+            : cudaLaunchKernelEx(&cfg, p.bits == 4 ? kv_read_kernel<T, 4> : kv_read_kernel<T, 8>, a);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t write_t(const KvPool &p, const View4 &k, const View4 &v, int64_t B, int64_t L, const int64_t *slots,
-                    int sm_count, cudaStream_t stream) {
-  const int vec = rows_on_16_bytes(k, sizeof(T)) && rows_on_16_bytes(v, sizeof(T));
-  const int64_t n = B * L;
-  // Few CTAs look through the slots (each reads all later ones) and fill the
-  // GPU twice: shrink a CTA's tokens, then its heads, until they do.
-  int tokens = kMaxTokens, ysplit = 1;
-  const int total = 2 * p.Hkv;
-  auto ctas = [&] { return (n + tokens - 1) / tokens * ysplit; };
-  while (ctas() < 2 * sm_count && tokens > 16) tokens /= 2;
-  while (ctas() < 2 * sm_count && total % (2 * ysplit) == 0) ysplit *= 2;
-  while (ctas() < 2 * sm_count && tokens > 1) tokens /= 2;
-  const dim3 grid(static_cast<unsigned>((n + tokens - 1) / tokens), static_cast<unsigned>(ysplit));
-  return launch(p.bits == 4 ? kv_write_kernel<T, 4> : kv_write_kernel<T, 8>, grid, stream, p, k, v, slots,
-                static_cast<uint32_t>(n), static_cast<uint32_t>(L), tokens, total / ysplit, vec);
-}
-
-template <typename T>
-cudaError_t read_t(const KvPool &p, const View4 &k, const View4 &v, int64_t B, int64_t L, const int64_t *slots,
-                   cudaStream_t stream) {
-  const int vec = rows_on_16_bytes(k, sizeof(T)) && rows_on_16_bytes(v, sizeof(T));
-  const uint32_t rows = static_cast<uint32_t>(2 * B * p.Hkv * L), per = 4 * (kThreads / (p.D / 8));
-  return launch(p.bits == 4 ? kv_read_kernel<T, 4> : kv_read_kernel<T, 8>, dim3((rows + per - 1) / per), stream, p, k,
-                v, slots, rows, static_cast<uint32_t>(B), static_cast<uint32_t>(L), vec);
+cudaError_t move(bool write, const KvPool &p, const View4 &k, const View4 &v, int dtype, int64_t B, int64_t L,
+                 const int64_t *slots, int sm_count, cudaStream_t stream) {
+  if (B * L == 0) return cudaSuccess;
+  if (dtype == LLK_DTYPE_FP32) return move_t<float>(write, p, k, v, B, L, slots, sm_count, stream);
+  if (dtype == LLK_DTYPE_FP16) return move_t<__half>(write, p, k, v, B, L, slots, sm_count, stream);
+  return move_t<__nv_bfloat16>(write, p, k, v, B, L, slots, sm_count, stream);
 }
 
 }  // namespace
@@ -299,18 +534,12 @@ bool kv_pool_supported(const KvPool &p) {
 
 cudaError_t kv_write_launch(const KvPool &p, const View4 &k, const View4 &v, int dtype, int64_t B, int64_t L,
                             const int64_t *slots, int sm_count, cudaStream_t stream) {
-  if (B * L == 0) return cudaSuccess;
-  if (dtype == LLK_DTYPE_FP32) return write_t<float>(p, k, v, B, L, slots, sm_count, stream);
-  if (dtype == LLK_DTYPE_FP16) return write_t<__half>(p, k, v, B, L, slots, sm_count, stream);
-  return write_t<__nv_bfloat16>(p, k, v, B, L, slots, sm_count, stream);
+  return move(true, p, k, v, dtype, B, L, slots, sm_count, stream);
 }
 
 cudaError_t kv_read_launch(const KvPool &p, const View4 &k, const View4 &v, int dtype, int64_t B, int64_t L,
                            const int64_t *slots, int sm_count, cudaStream_t stream) {
-  if (B * L == 0) return cudaSuccess;
-  if (dtype == LLK_DTYPE_FP32) return read_t<float>(p, k, v, B, L, slots, stream);
-  if (dtype == LLK_DTYPE_FP16) return read_t<__half>(p, k, v, B, L, slots, stream);
-  return read_t<__nv_bfloat16>(p, k, v, B, L, slots, stream);
+  return move(false, p, k, v, dtype, B, L, slots, sm_count, stream);
 }
 
 }  // namespace llk_b200

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import threading
 
 from . import capi
 from .capi import KernelContext, KvCache, Tensor4D, check, lib
@@ -26,12 +27,30 @@ except Exception:  # pragma: no cover
     _DTYPES = {}
 
 
-def _tensor4d(t) -> Tensor4D:
-    return Tensor4D(t.data_ptr(), tuple(t.shape), t.stride())
+class _Views(threading.local):
+    """This thread's descriptors by argument, sizes and strides (building one costs more than a launch)."""
+
+    def __init__(self):
+        self.known = {}
+
+
+_views = _Views()
+
+
+def _tensor4d(t, arg=0) -> Tensor4D:
+    """t's descriptor for the next call of this thread; `arg` tells a call's tensors apart."""
+    key = (arg, t.shape, t.stride())
+    d = _views.known.get(key)
+    if d is None:
+        if len(_views.known) >= 1024:
+            _views.known.clear()
+        d = _views.known[key] = Tensor4D(0, tuple(t.shape), t.stride())
+    d.data = t.data_ptr()
+    return d
 
 
 def _check_data(what, t, dtypes=None, dtype=None):
-    if not _is_torch(t) or not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{what} must be a torch CUDA tensor")
     if t.dim() != 4:
         raise ValueError(f"{what} must be [B, H, L, D]")
@@ -58,8 +77,7 @@ def _ranges(window, sinks):
 
 def _new_out(q, q_lens):
     # rows behind a sequence's queries are not written: they read as zeros
-    return torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_lens is None else torch.zeros(
-        q.shape, dtype=q.dtype, device=q.device)
+    return torch.empty_like(q) if q_lens is None else torch.zeros_like(q)
 
 
 def _scratch(nbytes, like, stream):
@@ -67,7 +85,7 @@ def _scratch(nbytes, like, stream):
     share it."""
     if not nbytes:
         return None, None
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    buf = like.new_empty((nbytes + 1) // 2)
     if stream is not None:
         _used_on(buf, stream)
     return buf, KernelContext(buf.data_ptr(), nbytes)
@@ -122,8 +140,8 @@ def window_attention(q, k, v, *, window=0, sinks: int = 0, scale: float | None =
     if made and stream is not None:
         _used_on(out, stream)
     g = gpu_context(q.device.index, _stream_of(q, stream))
-    rc = lib().llk_window_attention(_tensor4d(q), _tensor4d(k), _tensor4d(v), _tensor4d(out), dtype, pq, pk, window,
-                                    sinks, 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale), ctx, g)
+    rc = lib().llk_window_attention(_tensor4d(q), _tensor4d(k, 1), _tensor4d(v, 2), _tensor4d(out, 3), dtype, pq, pk,
+                                    window, sinks, 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale), ctx, g)
     if rc:
         check(rc, "llk_window_attention")
     return out
@@ -191,7 +209,7 @@ class QuantizedKVCache:
         _check_data("v", v, dtype=k.dtype)
         ps = _check_ints("slots", slots, torch.int64, (k.shape[0], k.shape[2]))
         g = gpu_context(self.device.index, _stream_of(k, stream))
-        rc = lib().llk_kv_cache_write(self._c, _tensor4d(k), _tensor4d(v), _DTYPES[k.dtype], ps, g)
+        rc = lib().llk_kv_cache_write(self._c, _tensor4d(k), _tensor4d(v, 1), _DTYPES[k.dtype], ps, g)
         if rc:
             check(rc, "llk_kv_cache_write")
 
@@ -203,7 +221,7 @@ class QuantizedKVCache:
         ps = _check_ints("slots", slots, torch.int64, tuple(slots.shape))
         if out is None:
             shape = (slots.shape[0], self.kv_heads, slots.shape[1], self.head_dim)
-            k, v = (torch.empty(shape, dtype=dtype or torch.bfloat16, device=self.device) for _ in range(2))
+            k, v = torch.empty((2,) + shape, dtype=dtype or torch.bfloat16, device=self.device).unbind(0)
             if stream is not None:
                 _used_on(k, stream)
                 _used_on(v, stream)
@@ -216,7 +234,7 @@ class QuantizedKVCache:
         if (k.shape[0], k.shape[2]) != tuple(slots.shape):
             raise ValueError("out must be [B, kv_heads, L, head_dim] with the slots' B and L")
         g = gpu_context(self.device.index, _stream_of(slots, stream))
-        rc = lib().llk_kv_cache_read(self._c, _tensor4d(k), _tensor4d(v), _DTYPES[k.dtype], ps, g)
+        rc = lib().llk_kv_cache_read(self._c, _tensor4d(k), _tensor4d(v, 1), _DTYPES[k.dtype], ps, g)
         if rc:
             check(rc, "llk_kv_cache_read")
         return k, v
@@ -248,7 +266,7 @@ class QuantizedKVCache:
             _used_on(out, stream)
         g = gpu_context(self.device.index, _stream_of(q, stream))
         rc = lib().llk_kv_cache_attention(_tensor4d(q), self._c, block_table.data_ptr(), W,
-                                          block_table.stride(0) if B > 1 else W, pq, pk, _tensor4d(out),
+                                          block_table.stride(0) if B > 1 else W, pq, pk, _tensor4d(out, 1),
                                           _DTYPES[q.dtype], window, sinks,
                                           1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale), ctx, g)
         if rc:

@@ -495,7 +495,36 @@ def test_serving_refusals_on_device():
         from dslcompiler_b200.serving import _tensor4d
         from dslcompiler_b200.swiglu import _stream_of, gpu_context
 
-        rc = capi.lib().llk_window_attention(_tensor4d(q), _tensor4d(big), _tensor4d(big.clone()), _tensor4d(o),
+        rc = capi.lib().llk_window_attention(_tensor4d(q), _tensor4d(big, 1), _tensor4d(big.clone(), 2), _tensor4d(o, 3),
                                              capi.LLK_DTYPE_BF16, None, None, 0, 0, 0.125, None,
                                              ctypes.byref(gpu_context(0, _stream_of(q, None))))
     assert rc == capi.LLK_ERR_NOMEM
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_cache_codes_next_to_borders(bits, dtype):
+    """Groups whose elements lie on the borders between two codes, a step of the type above and below them, and
+    next to a minimum that their difference to does not fit 24 bits: the codes are those of 64 bits."""
+    D, L, page = 128, 512, 64
+    g = torch.Generator().manual_seed(bits)
+    top = 2**bits - 1
+    scale = torch.exp2(torch.randint(-6, 7, (1, 1, L, 1), generator=g).double()) * (
+        1 + torch.randint(0, 128, (1, 1, L, 1), generator=g) / 128.0)
+    low = torch.randn((1, 1, L, 1), generator=g).double() * scale * 4
+    low = low.to(BF16).double()
+    border = low + scale * (torch.randint(0, top, (1, 1, L, D), generator=g).double() + 0.5)
+    x = border.to(dtype)
+    step = torch.randint(-1, 2, x.shape, generator=g)
+    bump = {BF16: torch.int16, F16: torch.int16, F32: torch.int32}[dtype]
+    x = (x.view(bump) + torch.where(x != 0, step, 0).to(bump)).view(dtype)
+    x[..., 0], x[..., 1] = low[..., 0].to(dtype), (low + top * scale)[..., 0].to(dtype)
+    x[0, 0, ::3, 2::5] = (torch.randn((len(range(0, L, 3)), len(range(2, D, 5))), generator=g) * 2.0**-30).to(dtype)
+    x[0, 0, ::7] = x[0, 0, ::7].abs()
+    x[0, 0, ::7, 3] = 2.0**-24
+    cache = llk.QuantizedKVCache.empty(L // page, page, 1, D, bits=bits, group_size=128)
+    cache.write(x.cuda(), x.cuda(), torch.arange(L)[None].cuda())
+    c, s, m = ref.quantise(x, bits, 128)
+    got = ref.unpack(cache.k_codes, bits).reshape(L, D)
+    assert torch.equal(cache.k_params.cpu().double().reshape(L, 2), torch.cat([s, m], -1)[0, 0])
+    assert torch.equal(got, c.long()[0, 0])
