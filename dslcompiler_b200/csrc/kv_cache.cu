@@ -8,8 +8,7 @@
 // bits the elements 2j and 2j + 1 share byte j (2j in the low nibble).
 //
 // HBM-bound both ways; what there is to save is instructions.  A thread owns
-// 8 elements of a row (one 16-byte load for 16-bit types), a row is D / 8
-// neighbouring lanes.  A CTA first works out where its tokens lie, once for
+// 16 elements of a row, a row is D / 16 neighbouring lanes.  A CTA first works out where its tokens lie, once for
 // all heads.  Writing: the group's minimum and maximum are packed 16-bit
 // operations and shuffles of the pair (min, -max); the quotient (x - m) / s is
 // a product with 1 / s and one correction by its remainder, which makes it
@@ -31,6 +30,7 @@ namespace llk_b200 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kCtas = 4;              // resident on an SM: 64 registers
 constexpr int kMaxTokens = 64;        // tokens of a writer's CTA
 constexpr int kBitmapWords = 1024;    // 32768 bits over the low bits of the CTA's slots
 constexpr float kLargest = 65504.f;
@@ -62,17 +62,18 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// Eight elements of a row as they lie.
+// A thread's elements of a row, as they lie.
+constexpr int kN = 16;
 template <typename T>
-struct Eight {
-  uint32_t w[2 * sizeof(T)];
+struct Piece {
+  uint32_t w[kN * sizeof(T) / 4];
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T *src, bool vec, Eight<T> &x) {
+__device__ __forceinline__ void load_piece(const T *src, bool vec, Piece<T> &x) {
   if (vec) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    for (int i = 0; i < kN * static_cast<int>(sizeof(T)) / 16; ++i) {
       const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
       x.w[4 * i] = v.x;
       x.w[4 * i + 1] = v.y;
@@ -82,33 +83,26 @@ __device__ __forceinline__ void load8(const T *src, bool vec, Eight<T> &x) {
   } else if constexpr (sizeof(T) == 2) {
     const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x.w[i] = e[2 * i] | static_cast<uint32_t>(e[2 * i + 1]) << 16;
+    for (int i = 0; i < kN / 2; ++i) x.w[i] = e[2 * i] | static_cast<uint32_t>(e[2 * i + 1]) << 16;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x.w[i] = __float_as_uint(src[i]);
+    for (int i = 0; i < kN; ++i) x.w[i] = __float_as_uint(src[i]);
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void widen(const Eight<T> &x, float (&f)[8]) {
+__device__ __forceinline__ float element(const Piece<T> &x, int i) {
   if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x.w[i]);
+    return __uint_as_float(x.w[i]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = *reinterpret_cast<const __half2 *>(&x.w[i / 2]);
+    return i % 2 ? __high2float(h) : __low2float(h);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&x.w[i]));
-        f[2 * i] = y.x;
-        f[2 * i + 1] = y.y;
-      } else {
-        f[2 * i] = __uint_as_float(x.w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(x.w[i] & 0xffff0000u);
-      }
-    }
+    return __uint_as_float(i % 2 ? x.w[i / 2] & 0xffff0000u : x.w[i / 2] << 16);
   }
 }
 
+// 8 values to 8 elements.
 template <typename T>
 __device__ __forceinline__ void store8(T *dst, bool vec, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
@@ -134,22 +128,28 @@ __device__ __forceinline__ void store8(T *dst, bool vec, const float (&x)[8]) {
   for (int i = 0; i < 8; ++i) dst[i] = from_f32<T>(x[i]);
 }
 
-// Smallest and largest of a group: (min, max) over the gl lanes that share it.
-// NaN if the group holds one.
+__device__ __forceinline__ float saturate(float v) { return v != v ? 0.f : fminf(fmaxf(v, -kLargest), kLargest); }
+
+// Smallest and largest of a group over the gl lanes that share it; NaN if it
+// holds one.
 template <typename T>
-__device__ __forceinline__ float2 group_range(const Eight<T> &x, int gl) {
+__device__ __forceinline__ float2 group_range(const Piece<T> &x, int gl) {
   if constexpr (sizeof(T) == 2) {
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     const T2 *p = reinterpret_cast<const T2 *>(x.w);
-    T2 mn = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
-    T2 mx = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    T2 mn = p[0], mx = p[0];
+#pragma unroll
+    for (int i = 1; i < kN / 2; ++i) {
+      mn = __hmin2_nan(mn, p[i]);
+      mx = __hmax2_nan(mx, p[i]);
+    }
     // both halves' minima with both halves' negated maxima
     mx = __hneg2(mx);
     const uint32_t a = *reinterpret_cast<const uint32_t *>(&mn), b = *reinterpret_cast<const uint32_t *>(&mx);
     const uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a, b, 0x7632);
     T2 r = __hmin2_nan(*reinterpret_cast<const T2 *>(&lo), *reinterpret_cast<const T2 *>(&hi));
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
+    for (int off = 1; off < 8; off <<= 1) {
       const uint32_t o = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&r), off);
       const T2 both = __hmin2_nan(r, *reinterpret_cast<const T2 *>(&o));
       if (off < gl) r = both;
@@ -159,7 +159,7 @@ __device__ __forceinline__ float2 group_range(const Eight<T> &x, int gl) {
     float mn = INFINITY, mx = -INFINITY;
     bool nan = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kN; ++i) {
       const float f = __uint_as_float(x.w[i]);
       mn = fminf(mn, f);
       mx = fmaxf(mx, f);
@@ -167,7 +167,7 @@ __device__ __forceinline__ float2 group_range(const Eight<T> &x, int gl) {
     }
     if (nan) mn = NAN;
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
+    for (int off = 1; off < 8; off <<= 1) {
       const float a = __shfl_xor_sync(0xffffffffu, mn, off), c = __shfl_xor_sync(0xffffffffu, mx, off);
       if (off < gl) {
         mn = a != a || mn != mn ? NAN : fminf(mn, a);
@@ -176,6 +176,24 @@ __device__ __forceinline__ float2 group_range(const Eight<T> &x, int gl) {
     }
     return make_float2(mn, mx);
   }
+}
+
+// Whether x - m is exact for every x of the piece, 16-bit: 8 bits (f16: 11)
+// and m's 8 no more than 24 bits apart, or one of them 0.  Magnitudes compare
+// as their bits do; less one, a 0 becomes the largest.
+template <typename T>
+__device__ __forceinline__ bool exact_differences(const Piece<T> &x, float m, float largest) {
+  constexpr float kApart = std::is_same<T, __half>::value ? 0x1p-11f : 0x1p-14f;
+  uint32_t least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) least = __viaddmin_u16x2(x.w[i] & 0x7fff7fffu, 0xffffffffu, least);
+  // of both halves, and one back (all zero: 0xffff + 1 has no 16 bits, and is larger than any)
+  const uint32_t bits = min(least & 0xffffu, least >> 16) + 1;
+  const float am = fabsf(m);
+  if (bits > 0xffffu || am == 0.f) return true;
+  const unsigned short us = static_cast<unsigned short>(bits);
+  const float small = to_f32(*reinterpret_cast<const T *>(&us));
+  return small >= am * kApart && am >= largest * kApart;
 }
 
 // scale = bf16(f32(max((mx - m) / top, 2^-30))), the quotient as in 64 bits: in
@@ -189,48 +207,38 @@ __device__ __forceinline__ __nv_bfloat16 scale_of(float mx, float m) {
   return __float2bfloat16_rn(static_cast<float>(d < kLeastScale ? kLeastScale : d));
 }
 
-// Codes of one lane's 8 elements (packed, BITS bytes) and its group's
-// (scale, min).
-template <typename T, int BITS>
-__device__ __forceinline__ uint64_t quantise8(const Eight<T> &raw, int gl, uint32_t *param) {
+// Codes of a thread's elements (packed: words of the row) and its group's
+// (scale, min), from the group's (smallest, largest).  kWild: some element of
+// the warp is not finite or too large, and each saturates.
+template <typename T, int BITS, bool kWild>
+__device__ __forceinline__ void quantise_in(const Piece<T> &raw, float2 range, uint32_t (&words)[kN * BITS / 32],
+                                            uint32_t *param) {
   constexpr float kTop = static_cast<float>((1 << BITS) - 1);
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23
-  float x[8];
-  widen(raw, x);
-  float2 range = group_range(raw, gl);
-  if (__any_sync(0xffffffffu, !(range.x >= -kLargest && range.y <= kLargest))) {
-    // some value is not finite or too large
-    float mn = INFINITY, mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kLargest), kLargest);
-      mn = fminf(mn, x[i]);
-      mx = fmaxf(mx, x[i]);
-    }
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
-      const float a = __shfl_xor_sync(0xffffffffu, mn, off), c = __shfl_xor_sync(0xffffffffu, mx, off);
-      if (off < gl) {
-        mn = fminf(mn, a);
-        mx = fmaxf(mx, c);
-      }
-    }
-    range = make_float2(mn, mx);
-  }
+  auto x = [&](int i) {
+    const float v = element(raw, i);
+    return kWild ? saturate(v) : v;
+  };
   const __nv_bfloat16 mb = __float2bfloat16_rn(range.x);
   const float m = __bfloat162float(mb);
   const __nv_bfloat16 sb = scale_of<BITS>(range.y, m);
-  const float s = __bfloat162float(sb), inv = 1.f / s;
+  const float s = __bfloat162float(sb);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   *param = static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | (static_cast<uint32_t>(__bfloat16_as_ushort(mb)) << 16);
   const uint64_t m2 = f32x2(-m, -m), inv2 = f32x2(inv, inv), s2 = f32x2(-s, -s), round2 = f32x2(kRound, kRound),
                  unround2 = f32x2(-kRound, -kRound), one2 = f32x2(-1.f, -1.f);
-  // error of the corrected quotient: an ulp of at most 2^BITS + 1 (and of x - m, 2^-24 of it)
+  // error of the corrected quotient: an ulp or two of at most 2^BITS + 1 (and of x - m, 2^-24 of it)
   constexpr float kNear = static_cast<float>(1 << BITS) * 0x1p-22f, kLo = (0.5f - kNear) * (0.5f - kNear);
-  uint64_t k[4], r2[4];  // of the elements i and i + 4: codes, squared distances to them
+  // the squared distance to the code: (kLo, 1/4) iff within kHalf of kMid (with a margin, so that 1/4 itself is not)
+  constexpr float kMid = (kLo + 0.25f) / 2, kHalf = (0.25f - kLo) * 0.49f;
+  const uint64_t mid2 = f32x2(-kMid, -kMid);
+  uint64_t k[kN / 2];  // codes of the elements 8 h + i and 8 h + i + 4 in k[4 h + i]
   bool near = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint64_t d = add2(f32x2(x[i], x[i + 4]), m2);
+  for (int p = 0; p < kN / 2; ++p) {
+    const int e = p / 4 * 8 + p % 4;
+    const uint64_t d = add2(f32x2(x(e), x(e + 4)), m2);
     uint64_t q = mul2(d, inv2);
     q = fma2(fma2(q, s2, d), inv2, q);
     // (a lower bound only where m may lie above the smallest element, an upper
@@ -242,76 +250,95 @@ __device__ __forceinline__ uint64_t quantise8(const Eight<T> &raw, int gl, uint3
       if constexpr (kHigh) c = make_float2(fminf(c.x, kTop), fminf(c.y, kTop));
       q = f32x2(c.x, c.y);
     }
-    k[i] = add2(add2(q, round2), unround2);
-    const uint64_t r = fma2(k[i], one2, q);
-    r2[i] = mul2(r, r);
-    const float2 e = split2(r2[i]);
-    near |= e.x > kLo || e.y > kLo;
-  }
-  if (near && sizeof(T) == 2) {
-    // A tie is settled, if x - m is exact: 8 (f16: 11) and 8 bits no more than
-    // 24 bits apart.
-    constexpr float kApart = std::is_same<T, __half>::value ? 0x1p-11f : 0x1p-14f;
-    near = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 e = split2(r2[i % 4]);
-      const float ri = i < 4 ? e.x : e.y, ax = fabsf(x[i]), am = fabsf(m);
-      const bool exact = (ax >= am * kApart && am >= ax * kApart) || ax == 0.f || am == 0.f;
-      near |= ri > kLo && !(ri == 0.25f && exact);
+    k[p] = add2(add2(q, round2), unround2);
+    const uint64_t r = fma2(k[p], one2, q);
+    if constexpr (sizeof(T) == 2) {
+      // a tie (1/4) is settled where x - m is exact, see below
+      const float2 v = split2(fma2(r, r, mid2));
+      near |= fabsf(v.x) < kHalf || fabsf(v.y) < kHalf;
+    } else {
+      const float2 v = split2(mul2(r, r));
+      near |= v.x > kLo || v.y > kLo;
     }
   }
+  if constexpr (sizeof(T) == 2) near |= !exact_differences(raw, m, fmaxf(fabsf(range.y), fabsf(m)));
   if (near) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int p = 0; p < kN / 2; ++p) {
       float c[2];
-      const float2 kk = split2(k[i]);
+      const float2 kk = split2(k[p]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // x - m = d + e exactly; against the border on the quotient's side of k
-        const float xi = x[i + 4 * j], d = xi - m, t = d - xi, e = (xi - (d - t)) - (m + t);
+        const float xi = x(p / 4 * 8 + p % 4 + 4 * j), d = xi - m, t = d - xi, e = (xi - (d - t)) - (m + t);
         const float k0 = j ? kk.y : kk.x, q = d * inv;
         const float lo = q < k0 ? k0 - 1.f : k0;  // the border between lo and lo + 1
         const float side = fmaf(-(lo + 0.5f), s, d) + e;
         c[j] = side > 0.f || (side == 0.f && (static_cast<int>(lo) & 1)) ? lo + 1.f : lo;
         c[j] = fminf(fmaxf(c[j], 0.f), kTop);
       }
-      k[i] = f32x2(c[0], c[1]);
+      k[p] = f32x2(c[0], c[1]);
     }
   }
   const uint64_t base2 = f32x2(0x1p23f, 0x1p23f);
-  if constexpr (BITS == 4) {
-    const uint64_t by16 = f32x2(16.f, 16.f);
-    const uint64_t c = add2(fma2(fma2(fma2(k[3], by16, k[2]), by16, k[1]), by16, k[0]), base2);
-    return __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(c >> 32), 0x5410);
-  } else {
-    const uint64_t by256 = f32x2(256.f, 256.f);
-    const uint64_t c0 = add2(fma2(k[1], by256, k[0]), base2), c1 = add2(fma2(k[3], by256, k[2]), base2);
-    return __byte_perm(static_cast<uint32_t>(c0), static_cast<uint32_t>(c1), 0x5410) |
-           static_cast<uint64_t>(__byte_perm(static_cast<uint32_t>(c0 >> 32), static_cast<uint32_t>(c1 >> 32), 0x5410))
-               << 32;
+#pragma unroll
+  for (int h = 0; h < kN / 8; ++h) {
+    const uint64_t *kh = k + 4 * h;
+    if constexpr (BITS == 4) {
+      const uint64_t by16 = f32x2(16.f, 16.f);
+      const uint64_t c = add2(fma2(fma2(fma2(kh[3], by16, kh[2]), by16, kh[1]), by16, kh[0]), base2);
+      words[h] = __byte_perm(static_cast<uint32_t>(c), static_cast<uint32_t>(c >> 32), 0x5410);
+    } else {
+      const uint64_t by256 = f32x2(256.f, 256.f);
+      const uint64_t c0 = add2(fma2(kh[1], by256, kh[0]), base2), c1 = add2(fma2(kh[3], by256, kh[2]), base2);
+      words[2 * h] = __byte_perm(static_cast<uint32_t>(c0), static_cast<uint32_t>(c1), 0x5410);
+      words[2 * h + 1] = __byte_perm(static_cast<uint32_t>(c0 >> 32), static_cast<uint32_t>(c1 >> 32), 0x5410);
+    }
   }
 }
 
-// The 8 values of a lane.
-template <int BITS>
-__device__ __forceinline__ void values8(uint64_t codes, uint32_t param, float (&x)[8]) {
-  const float s = __uint_as_float(param << 16), m = __uint_as_float(param & 0xffff0000u);
-  const uint64_t m2 = f32x2(m, m), base2 = f32x2(-0x1p23f, -0x1p23f);
-  constexpr int kIn = 16 / BITS;  // codes of a 16-bit piece
+template <typename T, int BITS>
+__device__ __forceinline__ void quantise(const Piece<T> &raw, int gl, uint32_t (&words)[kN * BITS / 32],
+                                         uint32_t *param) {
+  float2 range = group_range(raw, gl);
+  if (!__any_sync(0xffffffffu, !(range.x >= -kLargest && range.y <= kLargest))) {
+    quantise_in<T, BITS, false>(raw, range, words, param);
+    return;
+  }
+  float mn = INFINITY, mx = -INFINITY;
 #pragma unroll
-  for (int h = 0; h < 8 / kIn; h += 2) {
-    // pieces h and h + 1, code i of both at once
-    const uint32_t w = static_cast<uint32_t>(codes >> (16 * h)), v = w >> 16;
+  for (int i = 0; i < kN; ++i) {
+    const float v = saturate(element(raw, i));
+    mn = fminf(mn, v);
+    mx = fmaxf(mx, v);
+  }
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) {
+    const float a = __shfl_xor_sync(0xffffffffu, mn, off), c = __shfl_xor_sync(0xffffffffu, mx, off);
+    if (off < gl) {
+      mn = fminf(mn, a);
+      mx = fmaxf(mx, c);
+    }
+  }
+  quantise_in<T, BITS, true>(raw, make_float2(mn, mx), words, param);
+}
+
+// 8 values from their codes; si[i] = (scale / 2^(BITS i)) twice, m2 = min twice.
+template <int BITS>
+__device__ __forceinline__ void values8(const uint32_t *words, const uint64_t *si, uint64_t m2, float (&x)[8]) {
+  const uint64_t base2 = f32x2(-0x1p23f, -0x1p23f);
+  constexpr int kIn = 16 / BITS;  // codes of a 16-bit half word
+#pragma unroll
+  for (int h = 0; h < BITS / 4; ++h) {
+    const uint32_t w = words[h], v = w >> 16;
 #pragma unroll
     for (int i = 0; i < kIn; ++i) {
       const uint32_t mask = ((1u << BITS) - 1) << (BITS * i);
       const uint64_t c = add2(f32x2(__uint_as_float((w & mask) | 0x4b000000u), __uint_as_float((v & mask) | 0x4b000000u)),
                               base2);
-      const float si = s * (1.f / static_cast<float>(1 << (BITS * i)));
-      const float2 y = split2(fma2(c, f32x2(si, si), m2));
-      x[h * kIn + i] = y.x;
-      x[(h + 1) * kIn + i] = y.y;
+      const float2 y = split2(fma2(c, si[i], m2));
+      x[2 * h * kIn + i] = y.x;
+      x[(2 * h + 1) * kIn + i] = y.y;
     }
   }
 }
@@ -350,7 +377,7 @@ __device__ __forceinline__ Place place(const Move &A, uint32_t n) {
 // all of them out) and leaves out its tokens that a later one overwrites, so a
 // slot holds its last token whatever order the CTAs run in.
 template <typename T, int BITS>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ Move A) {
+__global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_constant__ Move A) {
   __shared__ Place at[kMaxTokens];
   __shared__ int64_t slot[kMaxTokens];
   __shared__ uint32_t bitmap[kBitmapWords];
@@ -371,51 +398,68 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
   }
   __syncthreads();
   if (n_tokens > 1) {
-    const int64_t n_slots = P.num_pages * P.page;
+    // (a slot's low word decides for nearly all)
+    const uint32_t *low = reinterpret_cast<const uint32_t *>(A.slots);
+#pragma unroll 4
     for (uint32_t n = n0 + 1 + threadIdx.x; n < n_tokens; n += kThreads) {
-      const int64_t s = A.slots[n];
-      if (s < 0 || s >= n_slots || !(bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1)) continue;
-      const int before = n - n0 < static_cast<uint32_t>(cnt) ? static_cast<int>(n - n0) : cnt;
-      for (int t = 0; t < before; ++t)
-        if (slot[t] == s) at[t].row = -1;  // (whoever finds it writes the same)
+      const uint32_t s = low[2 * static_cast<size_t>(n)];
+      if (bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1) {
+        const int64_t full = A.slots[n];
+        const int before = n - n0 < static_cast<uint32_t>(cnt) ? static_cast<int>(n - n0) : cnt;
+        for (int t = 0; t < before; ++t)
+          if (slot[t] == full) at[t].row = -1;  // (whoever finds it writes the same)
+      }
     }
     __syncthreads();
   }
 
-  const int lpr = P.D / 8, l = threadIdx.x & (lpr - 1);  // lanes a row
+  const int lpr = P.D / kN, l = threadIdx.x & (lpr - 1);  // lanes a row
   const int rows = A.tokens * A.pairs;
-  const int gl = P.group / 8, groups = P.D / P.group;
-  constexpr int kU = sizeof(T) == 4 ? 2 : 4;  // rows in flight a thread
+  const int gl = P.group / kN, groups = P.D / P.group;
+  constexpr int kU = 1;  // rows in flight a thread, and as many ahead
   const int step = kThreads / lpr, mine = threadIdx.x / lpr;
-  // every lane runs every round (the group's shuffles take the whole warp)
-  for (int r0 = 0; r0 < rows; r0 += kU * step) {
-    Eight<T> x[kU];
-    int64_t row[kU];
-    bool is_v[kU];
+  // every lane runs every round (the group's shuffles take the whole warp);
+  // the next round's rows load while this one's are worked on
+  Piece<T> x[kU], ahead[kU];
+  int64_t row[kU], row_ahead[kU];
+  bool is_v[kU], is_v_ahead[kU];
+  auto load = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
-      is_v[u] = pair >= P.Hkv;
-      const int h = is_v[u] ? pair - P.Hkv : pair;
-      row[u] = r < rows && t < cnt ? at[t].row : -1;
+      is_v_ahead[u] = pair >= P.Hkv;
+      const int h = is_v_ahead[u] ? pair - P.Hkv : pair;
+      row_ahead[u] = r < rows && t < cnt ? at[t].row : -1;
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) x[u].w[i] = 0;
-      if (row[u] >= 0) {
-        const View4 &src = is_v[u] ? A.v : A.k;
-        load8(static_cast<const T *>(src.p) + (is_v[u] ? at[t].v : at[t].k) + h * src.sh + 8 * l, A.vec, x[u]);
-        row[u] += static_cast<int64_t>(h) * P.page;
+      for (int i = 0; i < static_cast<int>(kN * sizeof(T) / 4); ++i) ahead[u].w[i] = 0;
+      if (row_ahead[u] >= 0) {
+        const View4 &src = is_v_ahead[u] ? A.v : A.k;
+        load_piece(static_cast<const T *>(src.p) + (is_v_ahead[u] ? at[t].v : at[t].k) + h * src.sh + kN * l, A.vec,
+                   ahead[u]);
+        row_ahead[u] += static_cast<int64_t>(h) * P.page;
       }
     }
+  };
+  load(0);
+  for (int r0 = 0; r0 < rows; r0 += kU * step) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      uint32_t param;
-      const uint64_t codes = quantise8<T, BITS>(x[u], gl, &param);
+      x[u] = ahead[u];
+      row[u] = row_ahead[u];
+      is_v[u] = is_v_ahead[u];
+    }
+    if (r0 + kU * step < rows) load(r0 + kU * step);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      uint32_t param, words[kN * BITS / 32];
+      quantise<T, BITS>(x[u], gl, words, &param);
       if (row[u] < 0) continue;
-      uint8_t *dst = static_cast<uint8_t *>(is_v[u] ? P.v_codes : P.k_codes) + row[u] * (P.D * BITS / 8) + BITS * l;
+      uint8_t *dst =
+          static_cast<uint8_t *>(is_v[u] ? P.v_codes : P.k_codes) + row[u] * (P.D * BITS / 8) + kN * BITS / 8 * l;
       if constexpr (BITS == 4) {
-        *reinterpret_cast<uint32_t *>(dst) = static_cast<uint32_t>(codes);
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(words[0], words[1]);
       } else {
-        *reinterpret_cast<uint64_t *>(dst) = codes;
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(words[0], words[1], words[2], words[3]);
       }
       if ((l & (gl - 1)) == 0)
         static_cast<uint32_t *>(is_v[u] ? P.v_params : P.k_params)[row[u] * groups + l / gl] = param;
@@ -425,7 +469,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
 
 // Reader.  CTAs as the writer's.
 template <typename T, int BITS>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ Move A) {
+__global__ void __launch_bounds__(kThreads, kCtas) kv_read_kernel(const __grid_constant__ Move A) {
   __shared__ Place at[kMaxTokens];
   const KvPool &P = A.pool;
   const uint32_t n0 = blockIdx.x * A.tokens;
@@ -434,37 +478,70 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
   pdl_launch_dependents();
   if (threadIdx.x < cnt) at[threadIdx.x] = place(A, n0 + threadIdx.x);
   __syncthreads();
-  const int lpr = P.D / 8, l = threadIdx.x & (lpr - 1);
+  const int lpr = P.D / kN, l = threadIdx.x & (lpr - 1);
   const int rows = A.tokens * A.pairs;
-  const int gl = P.group / 8, groups = P.D / P.group;
-  constexpr int kU = 8;
+  const int gl = P.group / kN, groups = P.D / P.group;
+  constexpr int kU = 2, kW = kN * BITS / 32;
   const int step = kThreads / lpr, mine = threadIdx.x / lpr;
-  for (int r0 = 0; r0 < rows; r0 += kU * step) {
-    uint64_t codes[kU];
-    uint32_t param[kU];
+  uint32_t words[kU][kW], param[kU], words_ahead[kU][kW], param_ahead[kU];
+  T *dst[kU], *dst_ahead[kU];
+  auto load = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
       const bool is_v = pair >= P.Hkv;
-      codes[u] = 0;
-      param[u] = 0;  // a slot outside the cache reads as zeros
-      if (r < rows && t < cnt && at[t].row >= 0) {
-        const int64_t row = at[t].row + static_cast<int64_t>(is_v ? pair - P.Hkv : pair) * P.page;
-        const uint8_t *src = static_cast<const uint8_t *>(is_v ? P.v_codes : P.k_codes) + row * (P.D * BITS / 8) + BITS * l;
-        codes[u] = BITS == 4 ? *reinterpret_cast<const uint32_t *>(src) : *reinterpret_cast<const uint64_t *>(src);
-        param[u] = static_cast<const uint32_t *>(is_v ? P.v_params : P.k_params)[row * groups + l / gl];
-      }
-    }
+      const int h = is_v ? pair - P.Hkv : pair;
+      dst_ahead[u] = nullptr;
+      param_ahead[u] = 0;  // a slot outside the cache reads as zeros
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
+      for (int i = 0; i < kW; ++i) words_ahead[u][i] = 0;
       if (r >= rows || t >= cnt) continue;
-      const bool is_v = pair >= P.Hkv;
       const View4 &out = is_v ? A.v : A.k;
-      float x[8];
-      values8<BITS>(codes[u], param[u], x);
-      store8(static_cast<T *>(out.p) + (is_v ? at[t].v : at[t].k) + (is_v ? pair - P.Hkv : pair) * out.sh + 8 * l, A.vec,
-             x);
+      dst_ahead[u] = static_cast<T *>(out.p) + (is_v ? at[t].v : at[t].k) + h * out.sh + kN * l;
+      if (at[t].row < 0) continue;
+      const int64_t row = at[t].row + static_cast<int64_t>(h) * P.page;
+      const uint8_t *src = static_cast<const uint8_t *>(is_v ? P.v_codes : P.k_codes) + row * (P.D * BITS / 8) +
+                           kN * BITS / 8 * l;
+      if constexpr (BITS == 4) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(src);
+        words_ahead[u][0] = w.x;
+        words_ahead[u][1] = w.y;
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4 *>(src);
+        words_ahead[u][0] = w.x;
+        words_ahead[u][1] = w.y;
+        words_ahead[u][2] = w.z;
+        words_ahead[u][3] = w.w;
+      }
+      param_ahead[u] = static_cast<const uint32_t *>(is_v ? P.v_params : P.k_params)[row * groups + l / gl];
+    }
+  };
+  load(0);
+  for (int r0 = 0; r0 < rows; r0 += kU * step) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      dst[u] = dst_ahead[u];
+      param[u] = param_ahead[u];
+#pragma unroll
+      for (int i = 0; i < kW; ++i) words[u][i] = words_ahead[u][i];
+    }
+    if (r0 + kU * step < rows) load(r0 + kU * step);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (!dst[u]) continue;
+      const float s = __uint_as_float(param[u] << 16), m = __uint_as_float(param[u] & 0xffff0000u);
+      uint64_t si[16 / BITS];
+#pragma unroll
+      for (int i = 0; i < 16 / BITS; ++i) {
+        const float f = s * (1.f / static_cast<float>(1 << (BITS * i)));
+        si[i] = f32x2(f, f);
+      }
+#pragma unroll
+      for (int g = 0; g < kN / 8; ++g) {
+        float x[8];
+        values8<BITS>(&words[u][g * BITS / 4], si, f32x2(m, m), x);
+        store8(dst[u] + 8 * g, A.vec, x);
+      }
     }
   }
 }
@@ -488,16 +565,27 @@ cudaError_t move_t(bool write, const KvPool &p, const View4 &k, const View4 &v, 
   a.page_shift = -1;
   for (int i = 4; i < 17; ++i)
     if (p.page == 1 << i) a.page_shift = i;
-  // A writer's CTA looks through all later slots, so few of them should: a
-  // CTA takes many tokens and all heads, as long as the GPU is filled a few
-  // times over; then it takes fewer tokens, then fewer heads.
+  // CTAs: tokens x a share of the heads.  A writer's CTA looks through all
+  // later slots, so it should have many rows; but the SM with the most CTAs is
+  // the last to finish.  The least CTAs of an SM x instructions of their warps,
+  // as counted: ~400 for 16 elements of each lane, 12 for 32 slots looked
+  // through, 600 to begin with.
   const int64_t n = B * L;
   int ysplit = 1;
-  a.shift = 6;
-  auto ctas = [&] { return ((n + (1 << a.shift) - 1) >> a.shift) * ysplit; };
-  while (ctas() < 4 * sm_count && a.shift > 4) --a.shift;
-  while (ctas() < 4 * sm_count && 2 * p.Hkv % (2 * ysplit) == 0) ysplit *= 2;
-  while (ctas() < 4 * sm_count && a.shift > 0) --a.shift;
+  double least = 0;
+  for (int shift = 6; shift >= 0; --shift)
+    for (int y = 1; 2 * p.Hkv % y == 0; y *= 2) {
+      const int64_t ctas = ((n + (1 << shift) - 1) >> shift) * y;
+      const double rounds = static_cast<double>((static_cast<int64_t>(2 * p.Hkv / y) << shift) * (p.D / kN) + kThreads - 1);
+      const double cost = static_cast<double>((ctas + sm_count - 1) / sm_count) *
+                          (600 + 400 * static_cast<double>(static_cast<int64_t>(rounds / kThreads)) +
+                           (write ? 12.0 / kThreads * static_cast<double>(n) / 2 : 0));
+      if (least == 0 || cost < least) {
+        least = cost;
+        a.shift = shift;
+        ysplit = y;
+      }
+    }
   a.tokens = 1 << a.shift;
   a.pairs = 2 * p.Hkv / ysplit;
   cudaLaunchConfig_t cfg = {};
