@@ -111,6 +111,16 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
+// One lane of the warp, the same one every time (the compiler knows that it
+// is one, and keeps the issuing code in uniform registers).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void tmem_st_x8(uint32_t t, const uint32_t *r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -256,9 +266,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 9) {
     // ----------------------------------------------------------------- MMA
-    // (the whole warp follows; lane 0 issues)
+    // (the whole warp follows; one lane issues)
     if (n > 0) {
-      const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem_kv);
+      // Descriptors are made once; an operand's place is added to the address
+      // field (in 16-byte units), whose 14 bits hold any address of the CTA.
+      // (Made anew, they cost 100 clocks an instruction: more than it runs.)
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem_kv), 16, 1024);
+      const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem_kv), KT * 128, 1024);
       constexpr uint32_t idesc_s = idesc_16(kBf16, kBM, KT, false), idesc_o = idesc_16(kBf16, kBM, D, true);
       int cnt_s[2] = {0, 0}, cnt_o[2] = {0, 0};
       bool ok = true;
@@ -270,33 +285,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto scores = [&](int j) {
         const int i = idx_k(j), k0 = w.key0(j, KT);
-        const uint32_t k_addr = kv_addr + (i % ST) * C::kStageBytes;
+        const uint64_t k_at = k_desc + (i % ST) * (C::kStageBytes >> 4);
         if (!wait(&st->kv_full[i % ST], i / ST)) return;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (!w.active(t, k0, KT)) continue;
           if (cnt_s[t] == 0 && !wait(&st->q_full[t], 0)) return;
           if (cnt_s[t] > 0 && !wait(&st->s_empty[t], cnt_s[t] - 1)) return;
-          if (lane == 0) {
+          if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk & 3) * 32;
+            for (int kk = 0; kk < D / 16; ++kk)
               tc_mma_bf16(tmem + C::kColS + t * KT,
-                          make_smem_desc_sw128(q_addr + t * C::kQBytes + (kk >> 2) * kBM * 128 + off, 16, 1024),
-                          make_smem_desc_sw128(k_addr + (kk >> 2) * KT * 128 + off, 16, 1024), idesc_s, kk > 0);
-            }
+                          q_desc + ((t * C::kQBytes + (kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
+                          k_at + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
             tc_commit(&st->s_full[t]);
           }
           ++cnt_s[t];
         }
-        if (lane == 0) tc_commit(&st->kv_empty[i % ST]);
+        if (elect_one()) tc_commit(&st->kv_empty[i % ST]);
       };
       scores(0);
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) scores(j + 1);
         if (!ok) break;
         const int i = idx_v(j), k0 = w.key0(j, KT);
-        const uint32_t v_addr = kv_addr + (i % ST) * C::kStageBytes;
+        const uint64_t v_at = v_desc + (i % ST) * (C::kStageBytes >> 4);
         if (!wait(&st->kv_full[i % ST], i / ST)) break;
         // rows of V that no row of the CTA sees may hold anything: they become
         // zero before the product (a weight of 0 does not undo a NaN)
@@ -314,19 +327,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < 2; ++t) {
           if (!ok || !w.active(t, k0, KT)) continue;
           if (!wait(&st->p_ready[t], cnt_o[t])) continue;
-          if (lane == 0) {
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < KT / 16; ++kk)
-              mma_ts(tmem + C::kColO + t * D, tmem + C::kColP + t * (KT / 2) + kk * 8,
-                     make_smem_desc_sw128(v_addr + kk * 2048, KT * 128, 1024), idesc_o, cnt_o[t] > 0 || kk > 0);
+              mma_ts(tmem + C::kColO + t * D, tmem + C::kColP + t * (KT / 2) + kk * 8, v_at + (kk * 2048 >> 4), idesc_o,
+                     cnt_o[t] > 0 || kk > 0);
             tc_commit(&st->pv_done[t]);
           }
           ++cnt_o[t];
         }
-        if (ok && lane == 0) tc_commit(&st->kv_empty[i % ST]);
+        if (ok && elect_one()) tc_commit(&st->kv_empty[i % ST]);
       }
       // every MMA of this CTA has finished before TMEM is released
-      if (lane == 0) {
+      if (elect_one()) {
         tc_commit(&st->mma_done);
         int dummy = 0;
         mbar_wait_bounded(&st->mma_done, 0, &dummy, 1, 100000000ull);
