@@ -69,7 +69,7 @@ struct Cfg {
 };
 
 struct Tail {
-  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], mma_done;
+  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], landed, mma_done;
   uint32_t tmem;
   int abort;
 };
@@ -147,15 +147,28 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 // The key tiles of a CTA: s_tiles of sinks, then from the window's first.
 struct Sweep {
   int n, m, p0, hi, lo, s_keys, s_tiles, w_first, tiles, sinks, window;
+  // of each query tile: the window's tiles that some row sees, [from, to) (no
+  // row: to = -1); and the tiles that hold a sink, [0, sink_to)
+  int from0, from1, to0, to1, sink_to;
   __device__ __forceinline__ int key0(int j, int kt) const { return (j < s_tiles ? j : w_first + j - s_tiles) * kt; }
-  // does any row of query tile t (rows p0 + 128 t ..) see a key of the tile at k0?
-  __device__ __forceinline__ bool active(int t, int k0, int kt) const {
-    const int first = p0 + kBM * t;
-    int last = first + kBM - 1;
-    last = last < hi - 1 ? last : hi - 1;
-    if (last < first || last < k0) return false;
-    const int flo = window > 0 && first >= window ? first - window + 1 : 0;
-    return k0 + kt > flo || k0 < sinks;
+  __device__ __forceinline__ bool active(int t, int j) const {
+    return j < (t ? to1 : to0) && (j >= (t ? from1 : from0) || j < sink_to);
+  }
+  // values of the tile at k0 that no row sees
+  __device__ __forceinline__ bool dead(int k0, int kt) const { return k0 + kt > hi || (k0 < lo && k0 + kt > s_keys); }
+  __device__ __forceinline__ bool dead_key(int key) const { return key >= hi || (key < lo && key >= s_keys); }
+};
+
+// A place in the ring of stages.
+template <int ST>
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == ST) {
+      stage = 0;
+      phase ^= 1;
+    }
   }
 };
 
@@ -188,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&st->kv_full[i], 1);
       mbar_init(&st->kv_empty[i], 1);
     }
+    mbar_init(&st->landed, 1);
     mbar_init(&st->mma_done, 1);
     st->abort = 0;
     fence_mbar_init();
@@ -217,48 +231,85 @@ __global__ void __launch_bounds__(kThreads, 1)
   w.lo = window_lo(P.mask, w.p0);
   w.s_keys = w.sinks < w.lo ? w.sinks : w.lo;
   w.w_first = w.lo / KT;
-  const int s_all = (w.s_keys + KT - 1) / KT;
+  const int s_all = (w.s_keys + KT - 1) / KT, s_sinks = (w.sinks + KT - 1) / KT;
   w.s_tiles = s_all < w.w_first ? s_all : w.w_first;
   const int end_tile = w.hi > 0 ? (w.hi + KT - 1) / KT : 0;
   w.tiles = rows > 0 && end_tile > w.w_first ? w.s_tiles + end_tile - w.w_first : 0;
+  const int shift = w.s_tiles - w.w_first;
+  auto last_tile = [&](int first) {
+    const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
+    return last >= first && last >= 0 ? shift + last / KT + 1 : -1;
+  };
+  w.from0 = shift + w.lo / KT;
+  w.from1 = shift + window_lo(P.mask, w.p0 + kBM) / KT;
+  w.to0 = last_tile(w.p0);
+  w.to1 = last_tile(w.p0 + kBM);
+  w.sink_to = w.s_tiles + (s_sinks > w.w_first ? s_sinks - w.w_first : 0);
   const int n = w.tiles;
-  // K and V tiles share the ring in the order K0, K1, V0, K2, V1, ..
-  auto idx_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
-  auto idx_v = [&](int j) { return j < n - 1 ? 2 * j + 2 : 2 * n - 1; };
 
   if (warp == 8) {
     // ------------------------------------------------------------ producer
-    if (lane == 0 && n > 0) {
+    // K and V tiles share the ring in the order K0, K1, V0, K2, V1, ..  The
+    // whole warp follows, one lane issues.  Rows of V that no row of the CTA
+    // sees may hold anything (a weight of 0 does not undo a NaN): such a tile
+    // lands on a barrier of the warp's own, the warp makes the rows zero and
+    // only then says that the stage is full.
+    if (n > 0) {
       bool ok = true;
       const int q_tiles = rows > kBM ? 2 : 1;
-      for (int t = 0; t < q_tiles; ++t) {
-        mbar_arrive_expect_tx(&st->q_full[t], C::kQBytes);
-        for (int s = 0; s < C::kSlabs; ++s)
-          tma_load_4d(smem + t * C::kQBytes + s * kBM * 128, &maps.q, &st->q_full[t], 64 * s, q0 + kBM * t, h * A.qh,
-                      b * A.qb);
-      }
+      if (elect_one())
+        for (int t = 0; t < q_tiles; ++t) {
+          mbar_arrive_expect_tx(&st->q_full[t], C::kQBytes);
+          for (int s = 0; s < C::kSlabs; ++s)
+            tma_load_4d(smem + t * C::kQBytes + s * kBM * 128, &maps.q, &st->q_full[t], 64 * s, q0 + kBM * t, h * A.qh,
+                        b * A.qb);
+        }
+      __syncwarp();
+      Ring<ST> ring;
       int issued = 0;
-      auto load = [&](const CUtensorMap *map, int j, int ch, int cb) {
-        const int stage = issued % ST;
-        if (issued >= ST && !mbar_wait_bounded(&st->kv_empty[stage], ((issued / ST) - 1) & 1, abort, LLK_ERR_TIMEOUT,
-                                               kWaitLimitNs))
-          return false;
-        uint8_t *dst = smem_kv + stage * C::kStageBytes;
-        mbar_arrive_expect_tx(&st->kv_full[stage], C::kStageBytes);
-        for (int s = 0; s < C::kSlabs; ++s)
-          tma_load_4d(dst + s * KT * 128, map, &st->kv_full[stage], 64 * s, w.key0(j, KT), ch, cb);
+      auto wait = [&](uint64_t *bar, uint32_t phase) {
+        const bool r = mbar_wait_bounded(bar, phase, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+        return static_cast<bool>(__all_sync(0xffffffffu, r));
+      };
+      auto load = [&](const CUtensorMap *map, int j, int ch, int cb, uint64_t *full) {
+        if (issued >= ST && !wait(&st->kv_empty[ring.stage], ring.phase ^ 1)) return false;
+        if (elect_one()) {
+          uint8_t *dst = smem_kv + ring.stage * C::kStageBytes;
+          mbar_arrive_expect_tx(full, C::kStageBytes);
+          for (int s = 0; s < C::kSlabs; ++s) tma_load_4d(dst + s * KT * 128, map, full, 64 * s, w.key0(j, KT), ch, cb);
+        }
+        __syncwarp();
         ++issued;
         return true;
       };
-      ok = load(&maps.k, 0, hk * A.kh, b * A.kb);
+      uint32_t landings = 0;
+      ok = load(&maps.k, 0, hk * A.kh, b * A.kb, &st->kv_full[0]);
+      ring.next();
       for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) ok = load(&maps.k, j + 1, hk * A.kh, b * A.kb);
-        if (ok) ok = load(&maps.v, j, hk * A.vh, b * A.vb);
+        if (j + 1 < n) {
+          ok = load(&maps.k, j + 1, hk * A.kh, b * A.kb, &st->kv_full[ring.stage]);
+          ring.next();
+        }
+        const int k0 = w.key0(j, KT);
+        const bool dead = w.dead(k0, KT);
+        if (!ok || !(ok = load(&maps.v, j, hk * A.vh, b * A.vb, dead ? &st->landed : &st->kv_full[ring.stage]))) break;
+        if (dead) {
+          if (!(ok = wait(&st->landed, landings & 1))) break;
+          ++landings;
+          uint8_t *v = smem_kv + ring.stage * C::kStageBytes;
+          for (int e = lane; e < KT * C::kSlabs * 8; e += 32)
+            if (w.dead_key(k0 + (e >> 3) % KT)) *reinterpret_cast<uint4 *>(v + e * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (elect_one()) mbar_arrive(&st->kv_full[ring.stage]);
+        }
+        ring.next();
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         // the copies in flight land before the CTA's shared memory goes
         int dummy = 0;
         for (int t = 0; t < q_tiles; ++t) mbar_wait_bounded(&st->q_full[t], 0, &dummy, 1, 100000000ull);
+        mbar_wait_bounded(&st->landed, landings & 1, &dummy, 1, 100000000ull);  // (or nothing is on its way there)
         for (int i = issued > ST ? issued - ST : 0; i < issued; ++i)
           mbar_wait_bounded(&st->kv_full[i % ST], (i / ST) & 1, &dummy, 1, 100000000ull);
       }
@@ -266,84 +317,64 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 9) {
     // ----------------------------------------------------------------- MMA
-    // (the whole warp follows; one lane issues)
-    if (n > 0) {
-      // Descriptors are made once; an operand's place is added to the address
-      // field (in 16-byte units), whose 14 bits hold any address of the CTA.
-      // (Made anew, they cost 100 clocks an instruction: more than it runs.)
+    // One lane.  What lies between two products costs more than it looks (the
+    // softmax warps take most issue slots, and only about 7 products queue
+    // up): descriptors are made once, an operand's place is added to the
+    // address field (in 16-byte units, its 14 bits hold any address of the
+    // CTA), and the ring's places are counted along.
+    if (n > 0 && elect_one()) {
       const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem_kv), 16, 1024);
       const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem_kv), KT * 128, 1024);
       constexpr uint32_t idesc_s = idesc_16(kBf16, kBM, KT, false), idesc_o = idesc_16(kBf16, kBM, D, true);
       int cnt_s[2] = {0, 0}, cnt_o[2] = {0, 0};
       bool ok = true;
-      auto wait = [&](uint64_t *bar, int phase) {
-        const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
-        ok = __all_sync(0xffffffffu, r);
+      Ring<ST> ring;
+      auto wait = [&](uint64_t *bar, uint32_t phase) {
+        if (!mbar_try_wait(bar, phase & 1)) ok = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
         tc_fence_after();
         return ok;
       };
       auto scores = [&](int j) {
-        const int i = idx_k(j), k0 = w.key0(j, KT);
-        const uint64_t k_at = k_desc + (i % ST) * (C::kStageBytes >> 4);
-        if (!wait(&st->kv_full[i % ST], i / ST)) return;
+        if (!wait(&st->kv_full[ring.stage], ring.phase)) return;
+        const uint64_t k_at = k_desc + ring.stage * (C::kStageBytes >> 4);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (!w.active(t, k0, KT)) continue;
-          if (cnt_s[t] == 0 && !wait(&st->q_full[t], 0)) return;
-          if (cnt_s[t] > 0 && !wait(&st->s_empty[t], cnt_s[t] - 1)) return;
-          if (elect_one()) {
+          if (!w.active(t, j)) continue;
+          if (cnt_s[t] == 0 ? !wait(&st->q_full[t], 0) : !wait(&st->s_empty[t], cnt_s[t] - 1)) return;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              tc_mma_bf16(tmem + C::kColS + t * KT,
-                          q_desc + ((t * C::kQBytes + (kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
-                          k_at + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
-            tc_commit(&st->s_full[t]);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            tc_mma_bf16(tmem + C::kColS + t * KT,
+                        q_desc + ((t * C::kQBytes + (kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
+                        k_at + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+          tc_commit(&st->s_full[t]);
           ++cnt_s[t];
         }
-        if (elect_one()) tc_commit(&st->kv_empty[i % ST]);
+        tc_commit(&st->kv_empty[ring.stage]);
+        ring.next();
       };
       scores(0);
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) scores(j + 1);
-        if (!ok) break;
-        const int i = idx_v(j), k0 = w.key0(j, KT);
-        const uint64_t v_at = v_desc + (i % ST) * (C::kStageBytes >> 4);
-        if (!wait(&st->kv_full[i % ST], i / ST)) break;
-        // rows of V that no row of the CTA sees may hold anything: they become
-        // zero before the product (a weight of 0 does not undo a NaN)
-        if (k0 + KT > w.hi || (k0 < w.lo && k0 + KT > w.s_keys)) {
-          uint8_t *v = smem_kv + (i % ST) * C::kStageBytes;
-          for (int e = lane; e < KT * C::kSlabs * 8; e += 32) {
-            const int key = k0 + (e >> 3) % KT;
-            if (key >= w.hi || (key < w.lo && key >= w.s_keys))
-              *reinterpret_cast<uint4 *>(v + e * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
+        if (!ok || !wait(&st->kv_full[ring.stage], ring.phase)) break;
+        const uint64_t v_at = v_desc + ring.stage * (C::kStageBytes >> 4);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (!ok || !w.active(t, k0, KT)) continue;
-          if (!wait(&st->p_ready[t], cnt_o[t])) continue;
-          if (elect_one()) {
+          if (!ok || !w.active(t, j) || !wait(&st->p_ready[t], cnt_o[t])) continue;
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk)
-              mma_ts(tmem + C::kColO + t * D, tmem + C::kColP + t * (KT / 2) + kk * 8, v_at + (kk * 2048 >> 4), idesc_o,
-                     cnt_o[t] > 0 || kk > 0);
-            tc_commit(&st->pv_done[t]);
-          }
+          for (int kk = 0; kk < KT / 16; ++kk)
+            mma_ts(tmem + C::kColO + t * D, tmem + C::kColP + t * (KT / 2) + kk * 8, v_at + (kk * 2048 >> 4), idesc_o,
+                   cnt_o[t] > 0 || kk > 0);
+          tc_commit(&st->pv_done[t]);
           ++cnt_o[t];
         }
-        if (ok && elect_one()) tc_commit(&st->kv_empty[i % ST]);
+        if (ok) tc_commit(&st->kv_empty[ring.stage]);
+        ring.next();
       }
       // every MMA of this CTA has finished before TMEM is released
-      if (elect_one()) {
-        tc_commit(&st->mma_done);
-        int dummy = 0;
-        mbar_wait_bounded(&st->mma_done, 0, &dummy, 1, 100000000ull);
-      }
+      tc_commit(&st->mma_done);
+      int dummy = 0;
+      mbar_wait_bounded(&st->mma_done, 0, &dummy, 1, 100000000ull);
     }
     __syncwarp();
   } else {
@@ -370,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
     const int last_lo = window_lo(P.mask, last);
     for (int j = 0; j < n; ++j) {
+      if (!w.active(t, j)) continue;
       const int k0 = w.key0(j, KT);
-      if (!w.active(t, k0, KT)) continue;
       if (!wait(&st->s_full[t], cnt)) break;
       uint32_t sb[KT];
 #pragma unroll
