@@ -11,9 +11,9 @@
 //   warps 0-3, 4-7  softmax of query tile 0 / 1, one thread a row: S from
 //                   TMEM to registers, P back to TMEM in 16 bits, O's rescale
 //                   when the reference moves, the output
-//   warp 8          TMA: Q once, K and V tiles through one ring of stages
-//   warp 9          tcgen05.mma: S = Q K^T (both operands in shared memory),
-//                   O += P V (P from TMEM)
+//   warps 8, 9      tcgen05.mma of query tile 0 / 1: S = Q K^T (both operands
+//                   in shared memory), O += P V (P from TMEM)
+//   warp 10         TMA: Q once, K and V tiles through one ring of stages
 // TMEM columns: O0, O1, S0, S1, P0, P1.  S and P do not share columns, so
 // the next S of a query tile is computed while its softmax runs on the
 // registers, and the softmax warps never wait for the tensor core; that, and
@@ -37,7 +37,7 @@ namespace llk_b200 {
 namespace {
 
 constexpr int kBM = 128;                // rows of a query tile
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 // The reference m may lag a row's maximum by up to this power of two before O
 // is rescaled: P stays below 2^8, far inside f16, its relative rounding is
@@ -199,10 +199,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < ST; ++i) {
       mbar_init(&st->kv_full[i], 1);
-      mbar_init(&st->kv_empty[i], 1);
+      mbar_init(&st->kv_empty[i], 2);
     }
     mbar_init(&st->landed, 1);
-    mbar_init(&st->mma_done, 1);
+    mbar_init(&st->mma_done, 2);
     st->abort = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.q);
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   w.sink_to = w.s_tiles + (s_sinks > w.w_first ? s_sinks - w.w_first : 0);
   const int n = w.tiles;
 
-  if (warp == 8) {
+  if (warp == 10) {
     // ------------------------------------------------------------ producer
     // K and V tiles share the ring in the order K0, K1, V0, K2, V1, ..  The
     // whole warp follows, one lane issues.  Rows of V that no row of the CTA
@@ -315,19 +315,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp >= 8) {
     // ----------------------------------------------------------------- MMA
-    // One lane.  What lies between two products costs more than it looks (the
-    // softmax warps take most issue slots, and only about 7 products queue
-    // up): descriptors are made once, an operand's place is added to the
-    // address field (in 16-byte units, its 14 bits hold any address of the
-    // CTA), and the ring's places are counted along.
+    // One lane, for one query tile.  What lies between two products costs more
+    // than it looks (the softmax warps take most issue slots, and only about 7
+    // products queue up): descriptors are made once, an operand's place is
+    // added to the address field (in 16-byte units, its 14 bits hold any
+    // address of the CTA), and the ring's places are counted along.  A warp a
+    // query tile: products that wait for the tensor core also hold up the
+    // exponentials of the softmax warps on their scheduler, and two schedulers
+    // share that (with one warp for both tiles its scheduler's softmax warps
+    // ran 1000 clocks a key tile behind the others).
     if (n > 0 && elect_one()) {
-      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
+      const int t = warp - 8;
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem) + t * C::kQBytes, 16, 1024);
       const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem_kv), 16, 1024);
       const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem_kv), KT * 128, 1024);
       constexpr uint32_t idesc_s = idesc_16(kBf16, kBM, KT, false), idesc_o = idesc_16(kBf16, kBM, D, true);
-      int cnt_s[2] = {0, 0}, cnt_o[2] = {0, 0};
+      const uint32_t ts = tmem + C::kColS + t * KT, tp = tmem + C::kColP + t * (KT / 2), to = tmem + C::kColO + t * D;
+      uint32_t cnt_s = 0, cnt_o = 0;
       bool ok = true;
       Ring<ST> ring;
       auto wait = [&](uint64_t *bar, uint32_t phase) {
@@ -337,38 +343,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto scores = [&](int j) {
         if (!wait(&st->kv_full[ring.stage], ring.phase)) return;
-        const uint64_t k_at = k_desc + ring.stage * (C::kStageBytes >> 4);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!w.active(t, j)) continue;
-          if (cnt_s[t] == 0 ? !wait(&st->q_full[t], 0) : !wait(&st->s_empty[t], cnt_s[t] - 1)) return;
+        if (!w.active(t, j)) {
+          mbar_arrive(&st->kv_empty[ring.stage]);  // (of a full stage: not a lap ahead of the copies)
+        } else {
+          if (cnt_s == 0 ? !wait(&st->q_full[t], 0) : !wait(&st->s_empty[t], cnt_s - 1)) return;
+          const uint64_t k_at = k_desc + ring.stage * (C::kStageBytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            tc_mma_bf16(tmem + C::kColS + t * KT,
-                        q_desc + ((t * C::kQBytes + (kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
+            tc_mma_bf16(ts, q_desc + (((kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
                         k_at + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
           tc_commit(&st->s_full[t]);
-          ++cnt_s[t];
+          tc_commit(&st->kv_empty[ring.stage]);
+          ++cnt_s;
         }
-        tc_commit(&st->kv_empty[ring.stage]);
         ring.next();
       };
       scores(0);
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) scores(j + 1);
         if (!ok || !wait(&st->kv_full[ring.stage], ring.phase)) break;
-        const uint64_t v_at = v_desc + ring.stage * (C::kStageBytes >> 4);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!ok || !w.active(t, j) || !wait(&st->p_ready[t], cnt_o[t])) continue;
+        if (!w.active(t, j)) {
+          mbar_arrive(&st->kv_empty[ring.stage]);
+        } else {
+          if (!wait(&st->p_ready[t], cnt_o)) break;
+          const uint64_t v_at = v_desc + ring.stage * (C::kStageBytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < KT / 16; ++kk)
-            mma_ts(tmem + C::kColO + t * D, tmem + C::kColP + t * (KT / 2) + kk * 8, v_at + (kk * 2048 >> 4), idesc_o,
-                   cnt_o[t] > 0 || kk > 0);
+            mma_ts(to, tp + kk * 8, v_at + (kk * 2048 >> 4), idesc_o, cnt_o > 0 || kk > 0);
           tc_commit(&st->pv_done[t]);
-          ++cnt_o[t];
+          tc_commit(&st->kv_empty[ring.stage]);
+          ++cnt_o;
         }
-        if (ok) tc_commit(&st->kv_empty[ring.stage]);
         ring.next();
       }
       // every MMA of this CTA has finished before TMEM is released
