@@ -54,7 +54,7 @@ cudaError_t window_simt_launch(const AttnProblem &p, cudaStream_t stream);
 // encode_fn: cuTensorMapEncodeTiled; status: the device's error word (a
 // bounded wait that gave up).
 bool window_tc_supported(const AttnProblem &p);
-cudaError_t window_tc_launch(void *encode_fn, const AttnProblem &p, int *status, cudaStream_t stream);
+cudaError_t window_tc_launch(void *encode_fn, const AttnProblem &p, int *status, int sm_count, cudaStream_t stream);
 
 bool kv_pool_supported(const KvPool &p);
 // k, v: [B, Hkv, L, D] views of type dtype; slots [B, L].

@@ -1223,7 +1223,7 @@ int llk_window_attention(const llk_tensor4d *q, const llk_tensor4d *k, const llk
     return launched(split_launch(P, nullptr, nullptr, 0, plan, ws, stream));
   }
   if (window_tc_supported(P))
-    return launched(window_tc_launch(reinterpret_cast<void *>(g_encode), P, ds->status, stream));
+    return launched(window_tc_launch(reinterpret_cast<void *>(g_encode), P, ds->status, ds->sm_count, stream));
   if (!window_simt_supported(P)) return LLK_ERR_UNSUPPORTED;
   return launched(window_simt_launch(P, stream));
 }

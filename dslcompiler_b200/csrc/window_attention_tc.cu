@@ -5,9 +5,11 @@
 // per key tile, with the running reference m of the softmax (a row's maximum,
 // or up to 2^8 below it: see kSlack) and O / l at the end.
 //
-// A CTA owns 256 query rows of one head as two tiles of 128, and sweeps the
-// key tiles that any of its rows sees: the sinks' tiles, then the window's.
-// A query tile skips the key tiles that none of its own rows sees.
+// One CTA an SM takes 256 query rows of one head after another, as two tiles
+// of 128, and sweeps the key tiles that any of the rows sees: the sinks' tiles,
+// then the window's.  A query tile skips the key tiles that none of its own
+// rows sees.  The next rows' queries and keys are on their way while these are
+// finished (started anew, a CTA waits 4000 clocks for its first scores).
 //   warps 0-3, 4-7  softmax of query tile 0 / 1, one thread a row: S from
 //                   TMEM to registers, P back to TMEM in 16 bits, O's rescale
 //                   when the reference moves, the output
@@ -69,7 +71,7 @@ struct Cfg {
 };
 
 struct Tail {
-  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], landed, mma_done;
+  uint64_t q_full[2], q_empty[2], o_free[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], landed, mma_done;
   uint32_t tmem;
   int abort;
 };
@@ -146,11 +148,14 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 
 // The key tiles of a CTA: s_tiles of sinks, then from the window's first.
 struct Sweep {
-  int n, m, p0, hi, lo, s_keys, s_tiles, w_first, tiles, sinks, window;
+  int b, h, q0;  // the rows: sequence, head, first query
+  int m, rows;   // queries of the sequence, of these rows (may be <= 0 or > 256)
+  int p0, hi, lo, s_keys, s_tiles, w_first, tiles, sinks;
   // of each query tile: the window's tiles that some row sees, [from, to) (no
   // row: to = -1); and the tiles that hold a sink, [0, sink_to)
   int from0, from1, to0, to1, sink_to;
   __device__ __forceinline__ int key0(int j, int kt) const { return (j < s_tiles ? j : w_first + j - s_tiles) * kt; }
+  __device__ __forceinline__ bool any(int t) const { return (t ? to1 : to0) > 0; }
   __device__ __forceinline__ bool active(int t, int j) const {
     return j < (t ? to1 : to0) && (j >= (t ? from1 : from0) || j < sink_to);
   }
@@ -183,15 +188,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   Tail *st = reinterpret_cast<Tail *>(smem_kv + ST * C::kStageBytes);
   const AttnProblem &P = A.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int BH = P.B * P.H;
-  // the last query blocks first: under the causal mask they have the most keys
-  const int b = static_cast<int>(blockIdx.x % BH) / P.H, h = static_cast<int>(blockIdx.x % BH) % P.H;
-  const int q0 = (A.q_blocks - 1 - static_cast<int>(blockIdx.x / BH)) * 2 * kBM;
-  const int hk = h / (P.H / P.Hkv);
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&st->q_full[i], 1);
+      mbar_init(&st->q_empty[i], 1);
+      mbar_init(&st->o_free[i], kBM);
       mbar_init(&st->s_full[i], 1);
       mbar_init(&st->s_empty[i], kBM);
       mbar_init(&st->p_ready[i], kBM);
@@ -221,31 +222,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = st->tmem;
   volatile int *abort = &st->abort;
 
-  Sweep w;
-  seq_lens(P.mask, b, w.n, w.m);
-  w.sinks = P.mask.sinks;
-  w.window = P.mask.window;
-  const int rows = w.m - q0;  // of this CTA (may be <= 0 or > 256)
-  w.p0 = w.n - w.m + q0;
-  w.hi = w.p0 + (rows < 2 * kBM ? rows : 2 * kBM);
-  w.lo = window_lo(P.mask, w.p0);
-  w.s_keys = w.sinks < w.lo ? w.sinks : w.lo;
-  w.w_first = w.lo / KT;
-  const int s_all = (w.s_keys + KT - 1) / KT, s_sinks = (w.sinks + KT - 1) / KT;
-  w.s_tiles = s_all < w.w_first ? s_all : w.w_first;
-  const int end_tile = w.hi > 0 ? (w.hi + KT - 1) / KT : 0;
-  w.tiles = rows > 0 && end_tile > w.w_first ? w.s_tiles + end_tile - w.w_first : 0;
-  const int shift = w.s_tiles - w.w_first;
-  auto last_tile = [&](int first) {
-    const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
-    return last >= first && last >= 0 ? shift + last / KT + 1 : -1;
+  // This CTA's blocks of rows: the last ones of the sequences, which have the
+  // most keys, first, and every other round of them in reverse.
+  const int BH = P.B * P.H, items = A.q_blocks * BH;
+  auto item_of = [&](int round) {
+    return round * static_cast<int>(gridDim.x) +
+           static_cast<int>(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   };
-  w.from0 = shift + w.lo / KT;
-  w.from1 = shift + window_lo(P.mask, w.p0 + kBM) / KT;
-  w.to0 = last_tile(w.p0);
-  w.to1 = last_tile(w.p0 + kBM);
-  w.sink_to = w.s_tiles + (s_sinks > w.w_first ? s_sinks - w.w_first : 0);
-  const int n = w.tiles;
+  auto plan = [&](int item) {
+    Sweep w;
+    const int bh = item % BH;
+    w.b = bh / P.H;
+    w.h = bh - w.b * P.H;
+    w.q0 = (A.q_blocks - 1 - item / BH) * 2 * kBM;
+    int n;
+    seq_lens(P.mask, w.b, n, w.m);
+    w.sinks = P.mask.sinks;
+    w.rows = w.m - w.q0;
+    w.p0 = n - w.m + w.q0;
+    w.hi = w.p0 + (w.rows < 2 * kBM ? w.rows : 2 * kBM);
+    w.lo = window_lo(P.mask, w.p0);
+    w.s_keys = w.sinks < w.lo ? w.sinks : w.lo;
+    w.w_first = w.lo / KT;
+    const int s_all = (w.s_keys + KT - 1) / KT, s_sinks = (w.sinks + KT - 1) / KT;
+    w.s_tiles = s_all < w.w_first ? s_all : w.w_first;
+    const int end_tile = w.hi > 0 ? (w.hi + KT - 1) / KT : 0;
+    w.tiles = w.rows > 0 && end_tile > w.w_first ? w.s_tiles + end_tile - w.w_first : 0;
+    const int shift = w.s_tiles - w.w_first;
+    auto last_tile = [&](int first) {
+      const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
+      return w.tiles > 0 && last >= first && last >= 0 ? shift + last / KT + 1 : -1;
+    };
+    w.from0 = shift + w.lo / KT;
+    w.from1 = shift + window_lo(P.mask, w.p0 + kBM) / KT;
+    w.to0 = last_tile(w.p0);
+    w.to1 = last_tile(w.p0 + kBM);
+    w.sink_to = w.s_tiles + (s_sinks > w.w_first ? s_sinks - w.w_first : 0);
+    return w;
+  };
+  const int g = P.H / P.Hkv;
 
   if (warp == 10) {
     // ------------------------------------------------------------ producer
@@ -254,23 +269,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     // sees may hold anything (a weight of 0 does not undo a NaN): such a tile
     // lands on a barrier of the warp's own, the warp makes the rows zero and
     // only then says that the stage is full.
-    if (n > 0) {
-      bool ok = true;
-      const int q_tiles = rows > kBM ? 2 : 1;
-      if (elect_one())
-        for (int t = 0; t < q_tiles; ++t) {
+    bool ok = true;
+    Ring<ST> ring;
+    int issued = 0;
+    uint32_t landings = 0, queries[2] = {0, 0};
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+      const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+      return static_cast<bool>(__all_sync(0xffffffffu, r));
+    };
+    for (int round = 0; ok && item_of(round) < items; ++round) {
+      const Sweep w = plan(item_of(round));
+      const int n = w.tiles, hk = w.h / g;
+      if (n == 0) continue;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || !w.any(t)) continue;
+        if (queries[t] > 0 && !(ok = wait(&st->q_empty[t], queries[t] - 1))) continue;
+        if (elect_one()) {
           mbar_arrive_expect_tx(&st->q_full[t], C::kQBytes);
           for (int s = 0; s < C::kSlabs; ++s)
-            tma_load_4d(smem + t * C::kQBytes + s * kBM * 128, &maps.q, &st->q_full[t], 64 * s, q0 + kBM * t, h * A.qh,
-                        b * A.qb);
+            tma_load_4d(smem + t * C::kQBytes + s * kBM * 128, &maps.q, &st->q_full[t], 64 * s, w.q0 + kBM * t,
+                        w.h * A.qh, w.b * A.qb);
         }
-      __syncwarp();
-      Ring<ST> ring;
-      int issued = 0;
-      auto wait = [&](uint64_t *bar, uint32_t phase) {
-        const bool r = mbar_wait_bounded(bar, phase, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
-        return static_cast<bool>(__all_sync(0xffffffffu, r));
-      };
+        __syncwarp();
+        ++queries[t];
+      }
       auto load = [&](const CUtensorMap *map, int j, int ch, int cb, uint64_t *full) {
         if (issued >= ST && !wait(&st->kv_empty[ring.stage], ring.phase ^ 1)) return false;
         if (elect_one()) {
@@ -282,19 +305,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++issued;
         return true;
       };
-      uint32_t landings = 0;
-      ok = load(&maps.k, 0, hk * A.kh, b * A.kb, &st->kv_full[0]);
+      ok = ok && load(&maps.k, 0, hk * A.kh, w.b * A.kb, &st->kv_full[ring.stage]);
       ring.next();
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) {
-          ok = load(&maps.k, j + 1, hk * A.kh, b * A.kb, &st->kv_full[ring.stage]);
+          ok = load(&maps.k, j + 1, hk * A.kh, w.b * A.kb, &st->kv_full[ring.stage]);
           ring.next();
         }
         const int k0 = w.key0(j, KT);
         const bool dead = w.dead(k0, KT);
-        if (!ok || !(ok = load(&maps.v, j, hk * A.vh, b * A.vb, dead ? &st->landed : &st->kv_full[ring.stage]))) break;
+        if (!ok || !(ok = load(&maps.v, j, hk * A.vh, w.b * A.vb, dead ? &st->landed : &st->kv_full[ring.stage]))) break;
         if (dead) {
-          if (!(ok = wait(&st->landed, landings & 1))) break;
+          if (!(ok = wait(&st->landed, landings))) break;
           ++landings;
           uint8_t *v = smem_kv + ring.stage * C::kStageBytes;
           for (int e = lane; e < KT * C::kSlabs * 8; e += 32)
@@ -305,13 +327,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ring.next();
       }
-      if (!ok && lane == 0) {
-        // the copies in flight land before the CTA's shared memory goes
-        int dummy = 0;
-        for (int t = 0; t < q_tiles; ++t) mbar_wait_bounded(&st->q_full[t], 0, &dummy, 1, 100000000ull);
-        mbar_wait_bounded(&st->landed, landings & 1, &dummy, 1, 100000000ull);  // (or nothing is on its way there)
-        for (int i = issued > ST ? issued - ST : 0; i < issued; ++i)
-          mbar_wait_bounded(&st->kv_full[i % ST], (i / ST) & 1, &dummy, 1, 100000000ull);
+    }
+    if (!ok && lane == 0) {
+      // the copies in flight land before the CTA's shared memory goes (where
+      // nothing is on its way, the wait runs out)
+      int dummy = 0;
+      for (int t = 0; t < 2; ++t)
+        if (queries[t] > 0) mbar_wait_bounded(&st->q_full[t], (queries[t] - 1) & 1, &dummy, 1, 100000000ull);
+      dummy = 0;
+      mbar_wait_bounded(&st->landed, landings & 1, &dummy, 1, 100000000ull);
+      for (int i = issued > ST ? issued - ST : 0; i < issued; ++i) {
+        dummy = 0;
+        mbar_wait_bounded(&st->kv_full[i % ST], (i / ST) & 1, &dummy, 1, 100000000ull);
       }
     }
     __syncwarp();
@@ -326,14 +353,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // exponentials of the softmax warps on their scheduler, and two schedulers
     // share that (with one warp for both tiles its scheduler's softmax warps
     // ran 1000 clocks a key tile behind the others).
-    if (n > 0 && elect_one()) {
+    if (elect_one()) {
       const int t = warp - 8;
       const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem) + t * C::kQBytes, 16, 1024);
       const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem_kv), 16, 1024);
       const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem_kv), KT * 128, 1024);
       constexpr uint32_t idesc_s = idesc_16(kBf16, kBM, KT, false), idesc_o = idesc_16(kBf16, kBM, D, true);
       const uint32_t ts = tmem + C::kColS + t * KT, tp = tmem + C::kColP + t * (KT / 2), to = tmem + C::kColO + t * D;
-      uint32_t cnt_s = 0, cnt_o = 0;
+      uint32_t cnt_s = 0, cnt_o = 0, queries = 0;  // score tiles, value tiles, blocks of rows so far
       bool ok = true;
       Ring<ST> ring;
       auto wait = [&](uint64_t *bar, uint32_t phase) {
@@ -341,40 +368,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         return ok;
       };
-      auto scores = [&](int j) {
-        if (!wait(&st->kv_full[ring.stage], ring.phase)) return;
-        if (!w.active(t, j)) {
-          mbar_arrive(&st->kv_empty[ring.stage]);  // (of a full stage: not a lap ahead of the copies)
-        } else {
-          if (cnt_s == 0 ? !wait(&st->q_full[t], 0) : !wait(&st->s_empty[t], cnt_s - 1)) return;
-          const uint64_t k_at = k_desc + ring.stage * (C::kStageBytes >> 4);
+      for (int round = 0; ok && item_of(round) < items; ++round) {
+        const Sweep w = plan(item_of(round));
+        const int n = w.tiles, last = (t ? w.to1 : w.to0) - 1;
+        if (n == 0) continue;
+        bool first_s = true, first_o = true;
+        auto scores = [&](int j) {
+          if (!wait(&st->kv_full[ring.stage], ring.phase)) return;
+          if (!w.active(t, j)) {
+            mbar_arrive(&st->kv_empty[ring.stage]);  // (of a full stage: not a lap ahead of the copies)
+          } else {
+            if (first_s && !wait(&st->q_full[t], queries)) return;
+            if (cnt_s > 0 && !wait(&st->s_empty[t], cnt_s - 1)) return;
+            const uint64_t k_at = k_desc + ring.stage * (C::kStageBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            tc_mma_bf16(ts, q_desc + (((kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
-                        k_at + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
-          tc_commit(&st->s_full[t]);
-          tc_commit(&st->kv_empty[ring.stage]);
-          ++cnt_s;
-        }
-        ring.next();
-      };
-      scores(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) scores(j + 1);
-        if (!ok || !wait(&st->kv_full[ring.stage], ring.phase)) break;
-        if (!w.active(t, j)) {
-          mbar_arrive(&st->kv_empty[ring.stage]);
-        } else {
-          if (!wait(&st->p_ready[t], cnt_o)) break;
-          const uint64_t v_at = v_desc + ring.stage * (C::kStageBytes >> 4);
+            for (int kk = 0; kk < D / 16; ++kk)
+              tc_mma_bf16(ts, q_desc + (((kk >> 2) * kBM * 128 + (kk & 3) * 32) >> 4),
+                          k_at + (((kk >> 2) * KT * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+            tc_commit(&st->s_full[t]);
+            tc_commit(&st->kv_empty[ring.stage]);
+            if (j == last) tc_commit(&st->q_empty[t]);
+            ++cnt_s;
+            first_s = false;
+          }
+          ring.next();
+        };
+        scores(0);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + 1 < n) scores(j + 1);
+          if (!ok || !wait(&st->kv_full[ring.stage], ring.phase)) break;
+          if (!w.active(t, j)) {
+            mbar_arrive(&st->kv_empty[ring.stage]);
+          } else {
+            if (!wait(&st->p_ready[t], cnt_o)) break;
+            if (first_o && queries > 0 && !wait(&st->o_free[t], queries - 1)) break;
+            const uint64_t v_at = v_desc + ring.stage * (C::kStageBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < KT / 16; ++kk)
-            mma_ts(to, tp + kk * 8, v_at + (kk * 2048 >> 4), idesc_o, cnt_o > 0 || kk > 0);
-          tc_commit(&st->pv_done[t]);
-          tc_commit(&st->kv_empty[ring.stage]);
-          ++cnt_o;
+            for (int kk = 0; kk < KT / 16; ++kk)
+              mma_ts(to, tp + kk * 8, v_at + (kk * 2048 >> 4), idesc_o, !first_o || kk > 0);
+            tc_commit(&st->pv_done[t]);
+            tc_commit(&st->kv_empty[ring.stage]);
+            ++cnt_o;
+            first_o = false;
+          }
+          ring.next();
         }
-        ring.next();
+        if (last >= 0) ++queries;
       }
       // every MMA of this CTA has finished before TMEM is released
       tc_commit(&st->mma_done);
@@ -384,128 +423,142 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------- softmax
+    using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
     const int t = warp >> 2, quarter = warp & 3;
     const int row_in = quarter * 32 + lane;
-    const int row = q0 + kBM * t + row_in, pos = w.p0 + kBM * t + row_in;
-    const int row_lo = window_lo(P.mask, pos);
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t ts = t_lane + C::kColS + t * KT, tp = t_lane + C::kColP + t * (KT / 2),
                    to = t_lane + C::kColO + t * D;
     const float sc = P.scale * kLog2e;
-    float m = -INFINITY;
-    uint64_t l2 = 0;  // two partial sums
-    int cnt = 0;
+    const uint64_t sc2 = pack_f32x2(sc, sc);
+    uint32_t cnt = 0;  // score tiles so far
     bool ok = true;
-    auto wait = [&](uint64_t *bar, int phase) {
-      const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+      const bool r = mbar_try_wait(bar, phase & 1) ||
+                     mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
       ok = __all_sync(0xffffffffu, r);
       tc_fence_after();
       return ok;
     };
-    const int first = w.p0 + kBM * t;  // of the tile's rows that exist, the first and the last position
-    const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
-    const int last_lo = window_lo(P.mask, last);
-    for (int j = 0; j < n; ++j) {
-      if (!w.active(t, j)) continue;
-      const int k0 = w.key0(j, KT);
-      if (!wait(&st->s_full[t], cnt)) break;
-      uint32_t sb[KT];
+    for (int round = 0; ok && item_of(round) < items; ++round) {
+      const Sweep w = plan(item_of(round));
+      if (w.rows <= kBM * t) continue;  // no query of this tile: nothing is written
+      const int n = w.tiles, hk = w.h / g;
+      const int row = w.q0 + kBM * t + row_in, pos = w.p0 + kBM * t + row_in;
+      const int row_lo = window_lo(P.mask, pos);
+      const int first = w.p0 + kBM * t;  // of the tile's rows that exist, the first and the last position
+      const int last = first + kBM - 1 < w.hi - 1 ? first + kBM - 1 : w.hi - 1;
+      const int last_lo = window_lo(P.mask, last);
+      float m = -INFINITY;
+      uint64_t l2 = 0;  // two partial sums
+      bool begun = false;
+      for (int j = 0; j < n; ++j) {
+        if (!w.active(t, j)) continue;
+        const int k0 = w.key0(j, KT);
+        if (!wait(&st->s_full[t], cnt)) break;
+        uint32_t sb[KT];
 #pragma unroll
-      for (int c = 0; c < KT; c += 16)
-        tmem_ld_32x32b_x16(ts + c, *reinterpret_cast<uint32_t(*)[16]>(&sb[c]));
-      tmem_ld_wait();
-      tc_fence_before();
-      mbar_arrive(&st->s_empty[t]);
-      float s[KT];
+        for (int c = 0; c < KT; c += 16) tmem_ld_32x32b_x16(ts + c, *reinterpret_cast<uint32_t(*)[16]>(&sb[c]));
+        tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(&st->s_empty[t]);
+        float s[KT];
 #pragma unroll
-      for (int i = 0; i < KT; ++i) s[i] = __uint_as_float(sb[i]);
-      // every row of the tile sees every key of it, or the rows look key by key
-      const bool full = k0 + KT - 1 <= first && (k0 >= last_lo || k0 + KT <= w.sinks);
-      if (!full) {
-        const int hi_c = pos - k0, lo_c = row_lo - k0, s_c = w.sinks - k0;
+        for (int i = 0; i < KT; ++i) s[i] = __uint_as_float(sb[i]);
+        // every row of the tile sees every key of it, or the rows look key by key
+        if (!(k0 + KT - 1 <= first && (k0 >= last_lo || k0 + KT <= w.sinks))) {
+          auto below = [](int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; };
 #pragma unroll
-        for (int i = 0; i < KT; ++i)
-          if (i > hi_c || (i < lo_c && i >= s_c)) s[i] = -INFINITY;
-      }
-      float mx0 = s[0], mx1 = s[1];
+          for (int c = 0; c < KT; c += 32) {
+            const uint32_t see = below(pos + 1 - k0 - c) & (~below(row_lo - k0 - c) | below(w.sinks - k0 - c));
 #pragma unroll
-      for (int i = 2; i < KT; i += 2) {
-        mx0 = fmaxf(mx0, s[i]);
-        mx1 = fmaxf(mx1, s[i + 1]);
-      }
-      const float top = fmaxf(mx0, mx1) * sc;  // scale > 0
-      float corr = 1.f;
-      bool move = false;
-      if (cnt == 0) {
-        m = top;
-      } else {
-        move = __any_sync(0xffffffffu, top > m + kSlack);
-        if (move) {
-          const float m_new = fmaxf(m, top);
-          corr = m_new == -INFINITY ? 1.f : exp2_approx(m - m_new);
-          m = m_new;
-          float a, c;
-          unpack_f32x2(l2, a, c);
-          l2 = pack_f32x2(a * corr, c * corr);
-        }
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      const uint64_t sc2 = pack_f32x2(sc, sc), ref2 = pack_f32x2(-ref, -ref);
-      uint32_t pk[KT / 2];
-#pragma unroll
-      for (int i = 0; i < KT; i += 2) {
-        float a, c;
-        unpack_f32x2(fma_f32x2(pack_f32x2(s[i], s[i + 1]), sc2, ref2), a, c);
-        a = exp2_approx(a);
-        c = exp2_approx(c);
-        l2 = add_f32x2(l2, pack_f32x2(a, c));
-        pk[i / 2] = pack16<kBf16>(a, c);
-      }
-      if (cnt > 0) {
-        // P's columns are free and O is whole
-        if (!wait(&st->pv_done[t], cnt - 1)) break;
-        if (move) {
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t x[16];
-            tmem_ld_32x32b_x16(to + c, x);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
-            tmem_st_x8(to + c, x);
-            tmem_st_x8(to + c + 8, x + 8);
+            for (int i = 0; i < 32 && c + i < KT; ++i)
+              if (!(see >> i & 1)) s[c + i] = -INFINITY;
           }
         }
-      }
+        float mx0 = s[0], mx1 = s[1];
 #pragma unroll
-      for (int c = 0; c < KT / 2; c += 8) tmem_st_x8(tp + c, pk + c);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&st->p_ready[t]);
-      ++cnt;
-    }
-    // ------------------------------------------------------------- output
-    if (ok && cnt > 0) wait(&st->pv_done[t], cnt - 1);
-    if (ok && rows > kBM * t) {
-      using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+        for (int i = 2; i < KT; i += 2) {
+          mx0 = fmaxf(mx0, s[i]);
+          mx1 = fmaxf(mx1, s[i + 1]);
+        }
+        const float top = fmaxf(mx0, mx1) * sc;  // scale > 0
+        float corr = 1.f;
+        bool move = false;
+        if (!begun) {
+          m = top;
+        } else {
+          move = __any_sync(0xffffffffu, top > m + kSlack);
+          if (move) {
+            const float m_new = fmaxf(m, top);
+            corr = m_new == -INFINITY ? 1.f : exp2_approx(m - m_new);
+            m = m_new;
+            float a, c;
+            unpack_f32x2(l2, a, c);
+            l2 = pack_f32x2(a * corr, c * corr);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const uint64_t ref2 = pack_f32x2(-ref, -ref);
+        uint32_t pk[KT / 2];
+#pragma unroll
+        for (int i = 0; i < KT; i += 2) {
+          float a, c;
+          unpack_f32x2(fma_f32x2(pack_f32x2(s[i], s[i + 1]), sc2, ref2), a, c);
+          a = exp2_approx(a);
+          c = exp2_approx(c);
+          l2 = add_f32x2(l2, pack_f32x2(a, c));
+          pk[i / 2] = pack16<kBf16>(a, c);
+        }
+        if (begun) {
+          // P's columns are free and O is whole
+          if (!wait(&st->pv_done[t], cnt - 1)) break;
+          if (move) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t x[16];
+              tmem_ld_32x32b_x16(to + c, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * corr);
+              tmem_st_x8(to + c, x);
+              tmem_st_x8(to + c + 8, x + 8);
+            }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < KT / 2; c += 8) tmem_st_x8(tp + c, pk + c);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&st->p_ready[t]);
+        ++cnt;
+        begun = true;
+      }
+      // ----------------------------------------------------------- output
+      if (!ok || (begun && !wait(&st->pv_done[t], cnt - 1))) break;
       float l0, l1;
       unpack_f32x2(l2, l0, l1);
       const float l = l0 + l1;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const bool mine = row < w.m;
-      T *orow = static_cast<T *>(P.o.p) + b * P.o.sb + h * P.o.sh + static_cast<int64_t>(row) * P.o.sl;
+      T *orow = static_cast<T *>(P.o.p) + w.b * P.o.sb + w.h * P.o.sh + static_cast<int64_t>(row) * P.o.sl;
       bool bad = false;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t x[32];
-        if (cnt > 0) {
+        if (begun) {
           tmem_ld_32x32b_x32(to + c, x);
           tmem_ld_wait();
+          if (c + 32 == D) {
+            // O is read: the next rows' products may begin
+            tc_fence_before();
+            mbar_arrive(&st->o_free[t]);
+          }
         }
         float y[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          y[i] = cnt > 0 ? __uint_as_float(x[i]) * inv : 0.f;
+          y[i] = begun ? __uint_as_float(x[i]) * inv : 0.f;
           bad |= !(fabsf(y[i]) < INFINITY);
         }
         if (mine) {
@@ -529,11 +582,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         todo &= todo - 1;
         const int rr = row - lane + r, pp = pos - lane + r;
         __syncwarp();
-        attention_row<T>(static_cast<const T *>(P.q.p) + b * P.q.sb + h * P.q.sh + static_cast<int64_t>(rr) * P.q.sl,
-                         static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh,
-                         static_cast<const T *>(P.v.p) + b * P.v.sb + hk * P.v.sh,
-                         static_cast<T *>(P.o.p) + b * P.o.sb + h * P.o.sh + static_cast<int64_t>(rr) * P.o.sl, P.k.sl,
-                         P.v.sl, P.D, pp, window_lo(P.mask, pp), w.sinks, sc);
+        attention_row<T>(
+            static_cast<const T *>(P.q.p) + w.b * P.q.sb + w.h * P.q.sh + static_cast<int64_t>(rr) * P.q.sl,
+            static_cast<const T *>(P.k.p) + w.b * P.k.sb + hk * P.k.sh,
+            static_cast<const T *>(P.v.p) + w.b * P.v.sb + hk * P.v.sh,
+            static_cast<T *>(P.o.p) + w.b * P.o.sb + w.h * P.o.sh + static_cast<int64_t>(rr) * P.o.sl, P.k.sl, P.v.sl,
+            P.D, pp, window_lo(P.mask, pp), w.sinks, sc);
       }
     }
   }
@@ -565,7 +619,8 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 enc, CUtensorMap *map, bool bf16, 
 }
 
 template <int D, bool kBf16>
-cudaError_t launch_tc(PFN_cuTensorMapEncodeTiled_v12000 enc, const AttnProblem &p, int *status, cudaStream_t stream) {
+cudaError_t launch_tc(PFN_cuTensorMapEncodeTiled_v12000 enc, const AttnProblem &p, int *status, int sm_count,
+                      cudaStream_t stream) {
   using C = Cfg<D>;
   TcMaps maps;
   TcArgs a = {};
@@ -585,7 +640,8 @@ cudaError_t launch_tc(PFN_cuTensorMapEncodeTiled_v12000 enc, const AttnProblem &
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.q_blocks) * p.B * p.H));
+  const int64_t items = static_cast<int64_t>(a.q_blocks) * p.B * p.H;
+  cfg.gridDim = dim3(static_cast<unsigned>(items < sm_count ? items : sm_count));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -607,15 +663,18 @@ bool window_tc_supported(const AttnProblem &p) {
   };
   return (p.dtype == LLK_DTYPE_BF16 || p.dtype == LLK_DTYPE_FP16) && p.D % 8 == 0 && p.D <= 128 && p.mask.Lk > 0 &&
          p.scale > 0.f && rows16(p.q, p.mask.Lq) && rows16(p.k, p.mask.Lk) && rows16(p.v, p.mask.Lk) &&
-         (static_cast<int64_t>(p.mask.Lq) + 255) / 256 * p.B * p.H <= INT32_MAX;
+         (static_cast<int64_t>(p.mask.Lq) + 255) / 256 * p.B * p.H <= INT32_MAX / 2;
 }
 
-cudaError_t window_tc_launch(void *encode_fn, const AttnProblem &p, int *status, cudaStream_t stream) {
+cudaError_t window_tc_launch(void *encode_fn, const AttnProblem &p, int *status, int sm_count, cudaStream_t stream) {
   if (p.B == 0 || p.H == 0 || p.mask.Lq == 0) return cudaSuccess;
   auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode_fn);
   const bool bf16 = p.dtype == LLK_DTYPE_BF16;
-  if (p.D <= 64) return bf16 ? launch_tc<64, true>(enc, p, status, stream) : launch_tc<64, false>(enc, p, status, stream);
-  return bf16 ? launch_tc<128, true>(enc, p, status, stream) : launch_tc<128, false>(enc, p, status, stream);
+  if (p.D <= 64)
+    return bf16 ? launch_tc<64, true>(enc, p, status, sm_count, stream)
+                : launch_tc<64, false>(enc, p, status, sm_count, stream);
+  return bf16 ? launch_tc<128, true>(enc, p, status, sm_count, stream)
+              : launch_tc<128, false>(enc, p, status, sm_count, stream);
 }
 
 }  // namespace llk_b200
