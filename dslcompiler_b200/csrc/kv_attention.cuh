@@ -1072,22 +1072,33 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
   }
 }
 
+// Dynamic shared memory of a CTA: the rings, or the warps' sums.
+constexpr int split_smem(int bits, int D, int G, int NT) {
+  const int rowb = D * bits / 8, block = kTok * (2 * rowb + (bits == 16 ? 0 : 8 * G));
+  const int stage = block * (D * bits <= 512 ? 2 : 1), rings = kWarps * (stage <= 2560 ? 4 : 3) * stage;
+  const int sums = kWarps * 8 * NT * (D + 2) * 4;
+  return rings > sums ? rings : sums;
+}
+
 // CTAs of 128 threads an SM holds: what the registers (accumulators, query
-// operand, a block's codes) and the rings leave.
+// operand, a block's codes) and 228 KB of shared memory leave.  Not to the
+// last KB: CTAs that come and go one by one leave gaps (measured: 6 of 148
+// SMs then held one less, and their work waited for a whole CTA's time).
 constexpr int ctas_per_sm(int bits, int D, int G, int NT) {
-  return D == 256   ? (bits == 16 ? 1 : 2)
-         : NT == 2  ? (D == 64 ? 3 : 2)
-         : bits == 16 ? (D == 128 ? 2 : 3)
-                      : (D == 128 && (bits == 8 || G > 1) ? 3 : 4);
+  const int by_regs = D == 256    ? (bits == 16 ? 1 : 2)
+                      : NT == 2   ? (D == 64 ? 3 : 2)
+                      : bits == 16 ? (D == 128 ? 2 : 3)
+                                   : (D == 128 && (bits == 8 || G > 1) ? 3 : 4);
+  const int fixed = 8 * NT * (2 * D + 8 + 4 * G + 4) + kWarps * 64 * NT + 1024;
+  const int by_smem = 224 * 1024 / (split_smem(bits, D, G, NT) + fixed);
+  return by_regs < by_smem ? by_regs : by_smem;
 }
 
 template <int BITS, int D, int G, bool kBf16, int NT>
 cudaError_t launch_split(const Params &a, cudaStream_t stream) {
   using X = Geo<BITS, D, G>;
-  constexpr int CTAS = ctas_per_sm(BITS, D, G, NT);
-  constexpr int sums = kWarps * 8 * NT * (D + 2) * static_cast<int>(sizeof(float));
-  constexpr int rings = kWarps * X::STAGES * X::STAGE;
-  constexpr int smem = sums > rings ? sums : rings;
+  constexpr int CTAS = ctas_per_sm(BITS, D, G, NT), smem = split_smem(BITS, D, G, NT);
+  static_assert(smem >= kWarps * X::STAGES * X::STAGE, "the rings' place");
   auto kern = split_kernel<BITS, D, G, kBf16, NT, CTAS>;
   auto join = combine_kernel<D, kBf16, BITS == 16>;
   // Once a device.  Both kernels ask for the largest shared memory: while one
