@@ -32,7 +32,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kCtas = 4;              // resident on an SM: 64 registers
 constexpr int kMaxTokens = 64;        // tokens of a writer's CTA
-constexpr int kBitmapWords = 1024;    // 32768 bits over the low bits of the CTA's slots
+constexpr int kBitmapWords = 1024;    // 32768 bits over the low bits of the CTA's slots, as many over a hash
 constexpr float kLargest = 65504.f;
 constexpr double kLeastScale = 0x1p-30;
 
@@ -348,11 +348,16 @@ struct Move {
   View4 k, v;
   const int64_t *slots;
   uint32_t n_tokens, L;  // B L, L
-  int tokens, shift;     // of a CTA, a power of two
+  int tokens;            // of a CTA
   int pairs;             // (tensor, head) pairs of a CTA
+  int step_pairs, step_tokens;  // rows of a round of the CTA: whole pairs and what is left
   int page_shift;        // log2 of the page, or -1
   int vec;
 };
+
+// A slot's bit of the second bitmap: the 15 upper bits of a product with 2^32
+// over the golden ratio.
+__device__ __forceinline__ uint32_t slot_hash(uint32_t s) { return s * 0x9e3779b1u >> 17; }
 
 // Where a CTA's tokens lie: rows of the dense tensors (element offsets at head
 // 0) and of the pool (at head 0; -1: nowhere).
@@ -373,19 +378,20 @@ __device__ __forceinline__ Place place(const Move &A, uint32_t n) {
 
 // Writer.  CTA: `tokens` tokens (blockIdx.x) of `pairs` pairs (blockIdx.y);
 // row = pair * tokens + token.  The same slot twice in a call: the CTA looks
-// through all later tokens' slots (a bitmap over its own slots rules nearly
-// all of them out) and leaves out its tokens that a later one overwrites, so a
+// through all later tokens' slots (two bitmaps over its own slots rule nearly
+// all of them out: one alone lets a token through for each of the CTA's when
+// the call has 2^15, and each costs a loop over the CTA's slots) and leaves out its tokens that a later one overwrites, so a
 // slot holds its last token whatever order the CTAs run in.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_constant__ Move A) {
   __shared__ Place at[kMaxTokens];
   __shared__ int64_t slot[kMaxTokens];
-  __shared__ uint32_t bitmap[kBitmapWords];
+  __shared__ uint32_t bitmap[2 * kBitmapWords];
   const KvPool &P = A.pool;
   const uint32_t n0 = blockIdx.x * A.tokens, n_tokens = A.n_tokens;
   const int cnt = n_tokens - n0 < static_cast<uint32_t>(A.tokens) ? static_cast<int>(n_tokens - n0) : A.tokens;
   if (n_tokens > 1)
-    for (int i = threadIdx.x; i < kBitmapWords; i += kThreads) bitmap[i] = 0;
+    for (int i = threadIdx.x; i < 2 * kBitmapWords; i += kThreads) bitmap[i] = 0;
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
@@ -394,22 +400,44 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_
     const int64_t s = p.row >= 0 ? A.slots[n0 + threadIdx.x] : -1;
     at[threadIdx.x] = p;
     slot[threadIdx.x] = s;
-    if (s >= 0 && n_tokens > 1) atomicOr(&bitmap[(s >> 5) & (kBitmapWords - 1)], 1u << (s & 31));
+    if (s >= 0 && n_tokens > 1) {
+      const uint32_t hash = slot_hash(static_cast<uint32_t>(s));
+      atomicOr(&bitmap[(s >> 5) & (kBitmapWords - 1)], 1u << (s & 31));
+      atomicOr(&bitmap[kBitmapWords + (hash >> 5)], 1u << (hash & 31));
+    }
   }
   __syncthreads();
   if (n_tokens > 1) {
-    // (a slot's low word decides for nearly all)
-    const uint32_t *low = reinterpret_cast<const uint32_t *>(A.slots);
-#pragma unroll 4
-    for (uint32_t n = n0 + 1 + threadIdx.x; n < n_tokens; n += kThreads) {
-      const uint32_t s = low[2 * static_cast<size_t>(n)];
-      if (bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1) {
-        const int64_t full = A.slots[n];
-        const int before = n - n0 < static_cast<uint32_t>(cnt) ? static_cast<int>(n - n0) : cnt;
-        for (int t = 0; t < before; ++t)
-          if (slot[t] == full) at[t].row = -1;  // (whoever finds it writes the same)
+    // A slot's low word decides for nearly all.
+    auto look = [&](uint32_t n, uint32_t s) {
+      if (!(bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1)) return;
+      const uint32_t hash = slot_hash(s);
+      if (!(bitmap[kBitmapWords + (hash >> 5)] >> (hash & 31) & 1)) return;
+      const int64_t full = A.slots[n];
+      const int before = n - n0 < static_cast<uint32_t>(cnt) ? static_cast<int>(n - n0) : cnt;
+      for (int t = 0; t < before; ++t)
+        if (slot[t] == full) at[t].row = -1;  // (whoever finds it writes the same)
+    };
+    // two a load, from a 16-byte boundary (token n0 itself does no harm), and
+    // several loads ahead: it is L2's latency that counts
+    constexpr int kAhead = 4;
+    const uint32_t i0 = n0 + 1 - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(A.slots + n0 + 1) >> 3 & 1);
+    const uint4 *two = reinterpret_cast<const uint4 *>(A.slots + i0);
+    const uint32_t twos = (n_tokens - i0) / 2;
+    for (uint32_t p = threadIdx.x; p < twos; p += kAhead * kThreads) {
+      uint4 v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (p + u * kThreads < twos) v[u] = two[p + u * kThreads];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t at2 = p + u * kThreads;
+        if (at2 >= twos) break;
+        look(i0 + 2 * at2, v[u].x);
+        look(i0 + 2 * at2 + 1, v[u].z);
       }
     }
+    if (threadIdx.x == 0 && (n_tokens - i0) % 2) look(n_tokens - 1, static_cast<uint32_t>(A.slots[n_tokens - 1]));
     __syncthreads();
   }
 
@@ -423,13 +451,23 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_
   Piece<T> x[kU], ahead[kU];
   int64_t row[kU], row_ahead[kU];
   bool is_v[kU], is_v_ahead[kU];
-  auto load = [&](int r0) {
+  const int end_pair = (blockIdx.y + 1) * A.pairs;
+  int next_pair = blockIdx.y * A.pairs + mine / A.tokens, next_t = mine % A.tokens;
+  auto next_row = [&]() {  // the thread's row of the next round
+    next_pair += A.step_pairs;
+    next_t += A.step_tokens;
+    if (next_t >= A.tokens) {
+      next_t -= A.tokens;
+      ++next_pair;
+    }
+  };
+  auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
+      const int t = next_t, pair = next_pair;
       is_v_ahead[u] = pair >= P.Hkv;
       const int h = is_v_ahead[u] ? pair - P.Hkv : pair;
-      row_ahead[u] = r < rows && t < cnt ? at[t].row : -1;
+      row_ahead[u] = pair < end_pair && t < cnt ? at[t].row : -1;
 #pragma unroll
       for (int i = 0; i < static_cast<int>(kN * sizeof(T) / 4); ++i) ahead[u].w[i] = 0;
       if (row_ahead[u] >= 0) {
@@ -438,9 +476,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_
                    ahead[u]);
         row_ahead[u] += static_cast<int64_t>(h) * P.page;
       }
+      next_row();
     }
   };
-  load(0);
+  load();
   for (int r0 = 0; r0 < rows; r0 += kU * step) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -448,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_
       row[u] = row_ahead[u];
       is_v[u] = is_v_ahead[u];
     }
-    if (r0 + kU * step < rows) load(r0 + kU * step);
+    if (r0 + kU * step < rows) load();
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       uint32_t param, words[kN * BITS / 32];
@@ -485,17 +524,28 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_read_kernel(const __grid_c
   const int step = kThreads / lpr, mine = threadIdx.x / lpr;
   uint32_t words[kU][kW], param[kU], words_ahead[kU][kW], param_ahead[kU];
   T *dst[kU], *dst_ahead[kU];
-  auto load = [&](int r0) {
+  const int end_pair = (blockIdx.y + 1) * A.pairs;
+  int next_pair = blockIdx.y * A.pairs + mine / A.tokens, next_t = mine % A.tokens;
+  auto next_row = [&]() {  // the thread's row of the next round
+    next_pair += A.step_pairs;
+    next_t += A.step_tokens;
+    if (next_t >= A.tokens) {
+      next_t -= A.tokens;
+      ++next_pair;
+    }
+  };
+  auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int r = r0 + u * step + mine, t = r & (A.tokens - 1), pair = blockIdx.y * A.pairs + (r >> A.shift);
+      const int t = next_t, pair = next_pair;
       const bool is_v = pair >= P.Hkv;
       const int h = is_v ? pair - P.Hkv : pair;
       dst_ahead[u] = nullptr;
       param_ahead[u] = 0;  // a slot outside the cache reads as zeros
 #pragma unroll
       for (int i = 0; i < kW; ++i) words_ahead[u][i] = 0;
-      if (r >= rows || t >= cnt) continue;
+      next_row();
+      if (pair >= end_pair || t >= cnt) continue;
       const View4 &out = is_v ? A.v : A.k;
       dst_ahead[u] = static_cast<T *>(out.p) + (is_v ? at[t].v : at[t].k) + h * out.sh + kN * l;
       if (at[t].row < 0) continue;
@@ -516,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_read_kernel(const __grid_c
       param_ahead[u] = static_cast<const uint32_t *>(is_v ? P.v_params : P.k_params)[row * groups + l / gl];
     }
   };
-  load(0);
+  load();
   for (int r0 = 0; r0 < rows; r0 += kU * step) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -525,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_read_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < kW; ++i) words[u][i] = words_ahead[u][i];
     }
-    if (r0 + kU * step < rows) load(r0 + kU * step);
+    if (r0 + kU * step < rows) load();
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       if (!dst[u]) continue;
@@ -567,32 +617,37 @@ cudaError_t move_t(bool write, const KvPool &p, const View4 &k, const View4 &v, 
     if (p.page == 1 << i) a.page_shift = i;
   // CTAs: tokens x a share of the heads.  A writer's CTA looks through all
   // later slots, so it should have many rows; but the SM with the most CTAs is
-  // the last to finish.  The least CTAs of an SM x instructions of their warps,
-  // as counted: ~400 for 16 elements of each lane, 12 for 32 slots looked
-  // through, 600 to begin with.
+  // the last to finish, and one CTA alone leaves it idle for a third of the
+  // time.  The least of an SM's CTAs x a CTA's cost, in the units of an
+  // instruction of all its warps, as measured: 500 for a round of 16 elements
+  // a lane, 0.1 for a slot looked through, 600 to begin with.
   const int64_t n = B * L;
+  const int lpr = p.D / kN;
   int ysplit = 1;
   double least = 0;
-  for (int shift = 6; shift >= 0; --shift)
-    for (int y = 1; 2 * p.Hkv % y == 0; y *= 2) {
-      const int64_t ctas = ((n + (1 << shift) - 1) >> shift) * y;
-      const double rounds = static_cast<double>((static_cast<int64_t>(2 * p.Hkv / y) << shift) * (p.D / kN) + kThreads - 1);
-      const double cost = static_cast<double>((ctas + sm_count - 1) / sm_count) *
-                          (600 + 400 * static_cast<double>(static_cast<int64_t>(rounds / kThreads)) +
-                           (write ? 12.0 / kThreads * static_cast<double>(n) / 2 : 0));
+  for (int y = 1; 2 * p.Hkv % y == 0; y *= 2)
+    for (int most = 1; most <= 3 * kCtas; ++most) {  // CTAs of an SM
+      int64_t tokens = (n * y + most * static_cast<int64_t>(sm_count) - 1) / (most * static_cast<int64_t>(sm_count));
+      if (tokens > kMaxTokens) tokens = kMaxTokens;
+      const int64_t ctas = (n + tokens - 1) / tokens * y;
+      const int64_t rounds = (tokens * (2 * p.Hkv / y) * lpr + kThreads - 1) / kThreads;
+      const double of_sm = static_cast<double>((ctas + sm_count - 1) / sm_count);
+      const double cost = (of_sm < 1.6 ? 1.6 : of_sm) *
+                          (600 + 500 * static_cast<double>(rounds) + (write ? 0.1 * static_cast<double>(n) / 2 : 0));
       if (least == 0 || cost < least) {
         least = cost;
-        a.shift = shift;
+        a.tokens = static_cast<int>(tokens);
         ysplit = y;
       }
     }
-  a.tokens = 1 << a.shift;
   a.pairs = 2 * p.Hkv / ysplit;
+  a.step_pairs = kThreads / lpr / a.tokens;
+  a.step_tokens = kThreads / lpr % a.tokens;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>((n + a.tokens - 1) >> a.shift), static_cast<unsigned>(ysplit));
+  cfg.gridDim = dim3(static_cast<unsigned>((n + a.tokens - 1) / a.tokens), static_cast<unsigned>(ysplit));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
