@@ -9,8 +9,13 @@
 //
 // A CTA owns 64 query rows of one head and sweeps the 64-key tiles that any
 // of them sees: the sinks' tiles, then the window's.  FMA-bound: 4 D FLOP a
-// pair.  Thread (ty, tx) of 16 x 16 owns a 4 x 4 block of scores and 4 rows x
-// 4 DP/64 columns of O; row reductions are shuffles over 16 lanes.
+// pair.  A warp owns 2 R neighbouring rows and skips the halves of tiles that
+// none of them sees; lane (tx, ty) has R rows x 4 keys of scores and R rows x
+// 4 DP/64 columns of O, so 16-byte loads from shared memory feed 2 R / 3 and
+// more packed f32 pairs each.  R = 8 with four warps, two CTAs an SM: one
+// CTA's loads and softmax run beside the other's products.  (R = 4 with eight
+// warps where DP = 256: R = 8 would need more than 255 registers.)  The
+// probabilities pass through the warp's own piece of shared memory.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -20,7 +25,7 @@ namespace llk_b200 {
 
 namespace {
 
-constexpr int kBQ = 64, kBK = 64, kThreads = 256, kPad = 4;
+constexpr int kBQ = 64, kBK = 64, kPad = 4;
 
 __device__ __forceinline__ void cp_async16_zfill(float *dst, const float *src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
@@ -40,14 +45,20 @@ __device__ __forceinline__ void load8(const T *src, float *x) {
 // [begin, end) and columns past D become zero (they are not read: what lies
 // there may be anything).  kVec: rows start on 16 bytes and D is a multiple
 // of the 16-byte piece.
-template <typename T, int DP, bool kVec>
+template <typename T, int DP, bool kVec, int kThreads>
 __device__ __forceinline__ void load_rows(float *dst, const T *src, int64_t sl, int row0, int begin, int end, int D) {
   constexpr int kLd = DP + kPad;
   if constexpr (kVec && sizeof(T) == 4) {
-    for (int e = threadIdx.x; e < kBQ * (DP / 4); e += kThreads) {
-      const int r = e / (DP / 4), c = 4 * (e % (DP / 4)), row = row0 + r;
+    constexpr int kRows = kThreads / (DP / 4);  // of a round
+    const int r0 = threadIdx.x / (DP / 4), c = 4 * (threadIdx.x % (DP / 4));
+    const T *from = src + (row0 + r0) * sl + c;
+    float *to = dst + r0 * kLd + c;
+#pragma unroll
+    for (int r = 0; r < kBQ; r += kRows) {
+      const int row = row0 + r0 + r;
       const bool in = row >= begin && row < end && c < D;
-      cp_async16_zfill(dst + r * kLd + c, reinterpret_cast<const float *>(in ? src + row * sl + c : src), in);
+      cp_async16_zfill(to + r * kLd, reinterpret_cast<const float *>(in ? from : src), in);
+      from += kRows * sl;
     }
   } else if constexpr (kVec) {
     for (int e = threadIdx.x; e < kBQ * (DP / 8); e += kThreads) {
@@ -66,16 +77,83 @@ __device__ __forceinline__ void load_rows(float *dst, const T *src, int64_t sl, 
   }
 }
 
-// kStages 2: the next tile's cp.async copies run while this one computes
-// (f32; D <= 128 leaves shared memory for it).
-template <typename T, int DP, bool kVec, int kStages>
-__global__ void __launch_bounds__(kThreads, 1) window_simt_kernel(const AttnProblem P, int q_tiles) {
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float x) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+
+// Scores (scaled) of a lane's R rows (2 apart) and the keys tx + 16 j, j0 <= j < j1.
+template <int R, int DP, int j0, int j1>
+__device__ __forceinline__ void dot_products(const float *q, const float *k, float scale, float (&s)[R][4]) {
+  constexpr int kLd = DP + kPad;
+  uint64_t acc[R][j1 - j0];  // sums of the even and of the odd d
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = j0; j < j1; ++j) acc[i][j - j0] = 0;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    ulonglong2 a[R], b[j1 - j0];
+#pragma unroll
+    for (int j = j0; j < j1; ++j) b[j - j0] = *reinterpret_cast<const ulonglong2 *>(k + 16 * j * kLd + d);
+#pragma unroll
+    for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const ulonglong2 *>(q + 2 * i * kLd + d);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < j1 - j0; ++j) acc[i][j] = fma2(a[i].x, b[j].x, acc[i][j]);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < j1 - j0; ++j) acc[i][j] = fma2(a[i].y, b[j].y, acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[i][j] = 0.f;
+      if (j >= j0 && j < j1) {
+        const float2 x = split2(acc[i][j - j0]);
+        s[i][j] = (x.x + x.y) * scale;
+      }
+    }
+}
+
+template <typename T, int DP>
+struct Simt {
+  static constexpr int R = DP > 128 ? 4 : 8;  // rows of a lane
+  static constexpr int kWarps = kBQ / (2 * R), kThreads = 32 * kWarps;
+  static constexpr int kCtas = DP > 128 ? 1 : 2;
+  static constexpr int kLdP = 2 * R + kPad;  // [key][row] of a half tile
+  static constexpr int kSmem = (3 * kBQ * (DP + kPad) + kWarps * kBK / 2 * kLdP) * static_cast<int>(sizeof(float));
+  static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory");
+};
+
+template <typename T, int DP, bool kVec>
+__global__ void __launch_bounds__(Simt<T, DP>::kThreads, Simt<T, DP>::kCtas)
+    window_simt_kernel(const AttnProblem P, int q_tiles) {
+  using G = Simt<T, DP>;
   extern __shared__ __align__(16) float sm[];
-  constexpr int kLd = DP + kPad, kOC = DP / 64;
-  float *Qs = sm;
-  float *KV = Qs + kBQ * kLd;                  // kStages x (K tile, V tile)
-  float *Pt = KV + kStages * 2 * kBK * kLd;    // [key][row]
-  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  constexpr int kLd = DP + kPad, kOC = DP / 64, R = G::R, kLdP = G::kLdP;
+  float *Qs = sm, *Ks = Qs + kBQ * kLd, *Vs = Ks + kBK * kLd;
+  const int warp = threadIdx.x >> 5, ty = threadIdx.x >> 4 & 1, tx = threadIdx.x & 15;
+  float *Pt = Vs + kBK * kLd + warp * (kBK / 2 * kLdP);
   // the last query tiles first: under the causal mask they have the most keys
   const int BH = P.B * P.H;
   const int b = (blockIdx.x % BH) / P.H, h = blockIdx.x % P.H;
@@ -103,164 +181,170 @@ __global__ void __launch_bounds__(kThreads, 1) window_simt_kernel(const AttnProb
   const int end_tile = hi > 0 ? (hi + kBK - 1) / kBK : 0;
   const int tiles = end_tile > w_first ? s_tiles + end_tile - w_first : 0;
   auto tile_row = [&](int t) { return (t < s_tiles ? t : w_first + t - s_tiles) * kBK; };
-  auto load_tile = [&](int t) {
-    float *Ks = KV + (t % kStages) * 2 * kBK * kLd;
+  auto load_tile = [&](float *dst, const T *src, int64_t sl, int t) {
     // a sinks' tile ends with the sinks (unless the window begins inside it)
     const int r0 = tile_row(t);
     const int begin = r0 >= s_keys ? lo : 0;
     const int end = t < s_tiles && r0 + kBK <= lo ? (s_keys < hi ? s_keys : hi) : hi;
-    load_rows<T, DP, kVec>(Ks, kb, P.k.sl, r0, begin, end, D);
-    load_rows<T, DP, kVec>(Ks + kBK * kLd, vb, P.v.sl, r0, begin, end, D);
+    load_rows<T, DP, kVec, G::kThreads>(dst, src, sl, r0, begin, end, D);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // the warp's rows: row(i) of the tile; the keys they see as lo and hi above
+  auto row = [&](int i) { return 2 * R * warp + 2 * i + ty; };
+  const int w0 = p0 + 2 * R * warp, w1 = w0 + 2 * R - 1 < last ? w0 + 2 * R - 1 : last;
+  const int warp_lo = window_lo(P.mask, w0), warp_hi = w1 >= w0 ? w1 + 1 : 0;
+  const float *q_rows = Qs + row(0) * kLd, *k_rows = Ks + tx * kLd;
 
-  load_rows<T, DP, kVec>(Qs, qb, P.q.sl, q0, 0, m_rows, D);
-  if (tiles > 0) load_tile(0);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  float m[4], l[4], acc[4][kOC][4];
+  load_rows<T, DP, kVec, G::kThreads>(Qs, qb, P.q.sl, q0, 0, m_rows, D);
+  if (tiles > 0) load_tile(Ks, kb, P.k.sl, 0);
+  float m[R], l[R];  // l: of this lane's keys alone
+  uint64_t acc[R][kOC][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < kOC; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+    for (int j = 0; j < kOC; ++j) acc[i][j][0] = acc[i][j][1] = 0;
   }
   const float sc = P.scale * kLog2e;
   for (int t = 0; t < tiles; ++t) {
-    if constexpr (kStages == 2) {
-      if (t + 1 < tiles) load_tile(t + 1);  // its buffer was last read by tile t-1, before the barrier that ended it
-      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 1;" ::: "memory");
-    } else {
-      if (t > 0) load_tile(t);
-      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-    }
-    __syncthreads();
-    const float *Ks = KV + (t % kStages) * 2 * kBK * kLd, *Vs = Ks + kBK * kLd;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // K is there, V is free
+    load_tile(Vs, vb, P.v.sl, t);
     const int k0 = tile_row(t);
-    float s[4][4];
+    bool sees[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int u = 0; u < 2; ++u) {
+      const int h0 = k0 + u * (kBK / 2);
+      sees[u] = h0 < warp_hi && (h0 + kBK / 2 > warp_lo || h0 < sinks);
+    }
+    float s[R][4];
+    if (sees[0] || sees[1]) {
+      if (sees[0] && sees[1])
+        dot_products<R, DP, 0, 4>(q_rows, k_rows, sc, s);
+      else if (sees[0])
+        dot_products<R, DP, 0, 2>(q_rows, k_rows, sc, s);
+      else
+        dot_products<R, DP, 2, 4>(q_rows, k_rows, sc, s);
+      // (all rows of the warp see the whole tile: nothing to mask)
+      const bool whole = k0 + kBK <= w0 + 1 && (k0 >= window_lo(P.mask, w0 + 2 * R - 1) || k0 + kBK <= sinks);
+      float mx[R];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-    float4 a[4], bb[4];
+      for (int i = 0; i < R; ++i) {
+        if (!whole) {
+          const int pos = p0 + row(i), row_lo = window_lo(P.mask, pos);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(&Qs[(4 * ty + i) * kLd]);
+          for (int j = 0; j < 4; ++j)
+            if (!key_visible(k0 + tx + 16 * j, pos, row_lo, sinks)) s[i][j] = -INFINITY;
+        }
+        mx[i] = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+      }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bb[j] = *reinterpret_cast<const float4 *>(&Ks[(tx + 16 * j) * kLd]);
-#pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
-      // the operands of step d + 4 load while step d computes
-      float4 an[4], bn[4];
-      const int dn = d + 4 < DP ? d + 4 : d;
+      for (int off = 8; off >= 1; off >>= 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) an[i] = *reinterpret_cast<const float4 *>(&Qs[(4 * ty + i) * kLd + dn]);
+        for (int i = 0; i < R; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], off));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bn[j] = *reinterpret_cast<const float4 *>(&Ks[(tx + 16 * j) * kLd + dn]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < R; ++i) {
+        const float m_new = fmaxf(m[i], mx[i]);
+        // exp2f, not the approximation: an f32 result keeps f32's accuracy
+        const float corr = m_new == -INFINITY ? 1.f : exp2f(m[i] - m_new), mm = m_new == -INFINITY ? 0.f : m_new;
+        float rsum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(a[i].x, bb[j].x, s[i][j]);
-          s[i][j] = fmaf(a[i].y, bb[j].y, s[i][j]);
-          s[i][j] = fmaf(a[i].z, bb[j].z, s[i][j]);
-          s[i][j] = fmaf(a[i].w, bb[j].w, s[i][j]);
+          s[i][j] = exp2f(s[i][j] - mm);
+          rsum += s[i][j];
         }
+        l[i] = fmaf(l[i], corr, rsum);
+        m[i] = m_new;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = an[i];
-        bb[i] = bn[i];
+        for (int jj = 0; jj < kOC; ++jj)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[i][jj][c] = mul2(acc[i][jj][c], twice(corr));
       }
     }
-    float p[4][4];
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // V is there, K is free
+    if (t + 1 < tiles) load_tile(Ks, kb, P.k.sl, t + 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pos = p0 + 4 * ty + i, row_lo = window_lo(P.mask, pos);
-      float rmax = -INFINITY;
+    for (int u = 0; u < 2; ++u) {
+      if (!sees[u]) continue;
+      __syncwarp();  // the other half's probabilities are read
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = key_visible(k0 + tx + 16 * j, pos, row_lo, sinks) ? s[i][j] * sc : -INFINITY;
-        rmax = fmaxf(rmax, s[i][j]);
-      }
+      for (int j = 2 * u; j < 2 * u + 2; ++j)
 #pragma unroll
-      for (int off = 8; off >= 1; off >>= 1) rmax = fmaxf(rmax, __shfl_xor_sync(0xffffffffu, rmax, off));
-      const float m_new = fmaxf(m[i], rmax);
-      // exp2f, not the approximation: an f32 result keeps f32's accuracy
-      const float corr = m_new == -INFINITY ? 1.f : exp2f(m[i] - m_new);
-      float rsum = 0.f;
+        for (int i = 0; i < R; i += 4)
+          *reinterpret_cast<float4 *>(&Pt[(tx + 16 * (j - 2 * u)) * kLdP + R * ty + i]) =
+              make_float4(s[i][j], s[i + 1][j], s[i + 2][j], s[i + 3][j]);
+      __syncwarp();
+      const int h0 = k0 + u * (kBK / 2);
+      int from = h0 < sinks ? 0 : warp_lo - h0, to = warp_hi - h0;  // (the rest's probabilities are 0)
+      from = from > 0 ? from & ~7 : 0;
+      to = to < kBK / 2 ? (to + 7) & ~7 : kBK / 2;
+      const float *v = Vs + u * (kBK / 2) * kLd + 4 * tx, *pr = Pt + R * ty;
+      for (int kk = from; kk < to; kk += 8)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[i][j] = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - m_new);
-        rsum += p[i][j];
-      }
+        for (int x = 0; x < 8; ++x) {
+          float4 pv[R / 4];
+          ulonglong2 vr[kOC];
 #pragma unroll
-      for (int off = 8; off >= 1; off >>= 1) rsum += __shfl_xor_sync(0xffffffffu, rsum, off);
-      l[i] = l[i] * corr + rsum;
-      m[i] = m_new;
+          for (int i = 0; i < R / 4; ++i) pv[i] = *reinterpret_cast<const float4 *>(pr + (kk + x) * kLdP + 4 * i);
 #pragma unroll
-      for (int jj = 0; jj < kOC; ++jj)
+          for (int jj = 0; jj < kOC; ++jj)
+            vr[jj] = *reinterpret_cast<const ulonglong2 *>(v + (kk + x) * kLd + 64 * jj);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][jj][c] *= corr;
-    }
+          for (int i = 0; i < R; ++i) {
+            const float4 f = pv[i / 4];
+            const uint64_t p2 = twice(i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4 *>(&Pt[(tx + 16 * j) * (kBQ + kPad) + 4 * ty]) =
-          make_float4(p[0][j], p[1][j], p[2][j], p[3][j]);
-    __syncthreads();
-    float4 pr = *reinterpret_cast<const float4 *>(&Pt[4 * ty]);
-    float4 vr[kOC];
-#pragma unroll
-    for (int jj = 0; jj < kOC; ++jj) vr[jj] = *reinterpret_cast<const float4 *>(&Vs[64 * jj + 4 * tx]);
-#pragma unroll 8
-    for (int kk = 0; kk < kBK; ++kk) {
-      const int kn = kk + 1 < kBK ? kk + 1 : kk;
-      const float4 prn = *reinterpret_cast<const float4 *>(&Pt[kn * (kBQ + kPad) + 4 * ty]);
-      float4 vrn[kOC];
-#pragma unroll
-      for (int jj = 0; jj < kOC; ++jj) vrn[jj] = *reinterpret_cast<const float4 *>(&Vs[kn * kLd + 64 * jj + 4 * tx]);
-      const float pv[4] = {pr.x, pr.y, pr.z, pr.w};
-#pragma unroll
-      for (int jj = 0; jj < kOC; ++jj) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[i][jj][0] = fmaf(pv[i], vr[jj].x, acc[i][jj][0]);
-          acc[i][jj][1] = fmaf(pv[i], vr[jj].y, acc[i][jj][1]);
-          acc[i][jj][2] = fmaf(pv[i], vr[jj].z, acc[i][jj][2]);
-          acc[i][jj][3] = fmaf(pv[i], vr[jj].w, acc[i][jj][3]);
+            for (int jj = 0; jj < kOC; ++jj) {
+              acc[i][jj][0] = fma2(p2, vr[jj].x, acc[i][jj][0]);
+              acc[i][jj][1] = fma2(p2, vr[jj].y, acc[i][jj][1]);
+            }
+          }
         }
-      }
-      pr = prn;
-#pragma unroll
-      for (int jj = 0; jj < kOC; ++jj) vr[jj] = vrn[jj];
     }
-    __syncthreads();  // Pt and this stage's K / V are free
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int r = q0 + row(i);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
     const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
     bool bad = false;
 #pragma unroll
-    for (int jj = 0; jj < kOC; ++jj)
+    for (int jj = 0; jj < kOC; ++jj) {
+      const float2 x01 = split2(acc[i][jj][0]), x23 = split2(acc[i][jj][1]);
+      const float x[4] = {x01.x * inv, x01.y * inv, x23.x * inv, x23.y * inv};
+      const int d = 64 * jj + 4 * tx;
+      if (r < m_rows && d < D) {
+        T out[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int d = 64 * jj + 4 * tx + c;
-        const float r = acc[i][jj][c] * inv;
-        if (row < m_rows && d < D) {
-          ob[row * P.o.sl + d] = from_f32<T>(r);
-          bad |= !isfinite(r);
+        for (int c = 0; c < 4; ++c) {
+          out[c] = from_f32<T>(x[c]);
+          bad |= d + c < D && !isfinite(x[c]);
+        }
+        T *to = ob + r * P.o.sl + d;
+        if constexpr (kVec && sizeof(T) == 4) {
+          *reinterpret_cast<float4 *>(to) = make_float4(x[0], x[1], x[2], x[3]);
+        } else if constexpr (kVec) {
+          *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(out);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (d + c < D) to[c] = out[c];
         }
       }
-    // rows 4 ty + i of the warp's two groups, redone by the whole warp
+    }
+    // rows i of the warp's two groups, redone by the whole warp
     const unsigned any = __ballot_sync(0xffffffffu, bad);
     if (any) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         if (any & (g ? 0xffff0000u : 0x0000ffffu)) {
-          const int r = q0 + 4 * ((ty & ~1) + g) + i, pos = n - m_rows + r;
+          const int rr = r - ty + g, pos = n - m_rows + rr;
           __syncwarp();
-          attention_row<T>(qb + r * P.q.sl, kb, vb, ob + r * P.o.sl, P.k.sl, P.v.sl, D, pos, window_lo(P.mask, pos),
+          attention_row<T>(qb + rr * P.q.sl, kb, vb, ob + rr * P.o.sl, P.k.sl, P.v.sl, D, pos, window_lo(P.mask, pos),
                            sinks, sc);
         }
       }
@@ -268,11 +352,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_simt_kernel(const AttnProb
   }
 }
 
-template <typename T, int DP, bool kVec, int kStages>
+template <typename T, int DP, bool kVec>
 cudaError_t launch_simt(const AttnProblem &p, cudaStream_t stream) {
-  const int smem = ((kBQ + 2 * kStages * kBK) * (DP + kPad) + kBK * (kBQ + kPad)) * static_cast<int>(sizeof(float));
-  auto kern = window_simt_kernel<T, DP, kVec, kStages>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  using G = Simt<T, DP>;
+  auto kern = window_simt_kernel<T, DP, kVec>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return e;
   const int q_tiles = (p.mask.Lq + kBQ - 1) / kBQ;
   cudaLaunchConfig_t cfg = {};
@@ -280,8 +366,8 @@ cudaError_t launch_simt(const AttnProblem &p, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(q_tiles) * p.B * p.H));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(G::kThreads);
+  cfg.dynamicSmemBytes = G::kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -291,10 +377,9 @@ cudaError_t launch_simt(const AttnProblem &p, cudaStream_t stream) {
 
 template <typename T, bool kVec>
 cudaError_t launch_simt_d(const AttnProblem &p, cudaStream_t stream) {
-  constexpr int kSt = kVec && sizeof(T) == 4 ? 2 : 1;
-  if (p.D <= 64) return launch_simt<T, 64, kVec, kSt>(p, stream);
-  if (p.D <= 128) return launch_simt<T, 128, kVec, kSt>(p, stream);
-  return launch_simt<T, 256, kVec, 1>(p, stream);
+  if (p.D <= 64) return launch_simt<T, 64, kVec>(p, stream);
+  if (p.D <= 128) return launch_simt<T, 128, kVec>(p, stream);
+  return launch_simt<T, 256, kVec>(p, stream);
 }
 
 bool rows_on_16_bytes(const View4 &v, int64_t el) {
@@ -306,7 +391,7 @@ template <typename T>
 cudaError_t launch_simt_t(const AttnProblem &p, cudaStream_t stream) {
   constexpr int64_t el = sizeof(T);
   const bool vec = p.D * el % 16 == 0 && rows_on_16_bytes(p.q, el) && rows_on_16_bytes(p.k, el) &&
-                   rows_on_16_bytes(p.v, el);
+                   rows_on_16_bytes(p.v, el) && rows_on_16_bytes(p.o, el);
   return vec ? launch_simt_d<T, true>(p, stream) : launch_simt_d<T, false>(p, stream);
 }
 
