@@ -10,7 +10,9 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
@@ -1067,10 +1069,17 @@ int view4(const llk_tensor4d &t, View4 *out) {
   return LLK_OK;
 }
 
-// An output's rows may not lie on one another.
+// An output's rows may not lie on one another: each dimension's stride is at
+// least what the dimensions of smaller strides reach over.
 bool rows_apart(const llk_tensor4d &t) {
-  for (int i = 0; i < 3; ++i)
-    if (t.dim[i] > 1 && t.stride[i] < t.dim[3]) return false;
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return t.stride[a] < t.stride[b]; });
+  int64_t reach = t.dim[3];
+  for (int i : order) {
+    if (t.dim[i] <= 1) continue;
+    if (t.stride[i] < reach || t.stride[i] > (INT64_MAX - reach) / (t.dim[i] - 1)) return false;
+    reach += t.stride[i] * (t.dim[i] - 1);
+  }
   return true;
 }
 
@@ -1105,9 +1114,31 @@ int attn_problem(const llk_tensor4d *q, int64_t Hkv, int64_t Lk, int dtype, int6
   return LLK_OK;
 }
 
-// Few query rows take the kernels that split the keys.
-bool use_split(const AttnProblem &P) {
-  return split_supported(P, nullptr) && static_cast<int64_t>(P.H / P.Hkv) * P.mask.Lq <= 64;
+// Whether a call takes the kernel that splits the keys, not one that has many
+// query rows of a head a CTA (256 on the tensor cores; those have no D above
+// 128, then 64 on the CUDA cores).  A block of 16 rows of a key head costs the
+// former as much of an SM's time a key (0.011 us at D = 128, less with fewer
+// d) as 256 rows the latter, which leaves SMs idle when there are few heads;
+// to begin and end takes as long as 900 keys (8 rows and fewer: 500) and 450.
+// Measured without a window, r = H / Hkv Lq rows, us split : not --
+//   B H Hkv = 16 32 8, L 4096, D 128:  r = 32 72 : 186, 64 176 : 187, 96 244 : 188
+//   1 32 8, L 8192, D 128:  r = 4 16 : 90, 128 44 : 90, 256 71 : 91, 512 126 : 92
+//   4 32 32, L 2048, D 128:  r = 4 28 : 30, 12 32 : 30, 32 46 : 30
+//   2 16 4, L 300, D 128:  r = 4 6.8 : 8.5, 16 9.9 : 8.4, 64 11.5 : 8.5
+//   1 8 8, L 500, D 64:  r = 8 7.0 : 10.4, 16 9.5 : 10.5, 64 12.1 : 10.5
+//   2 8 2, L 1024, D 256:  r = 64 15 : 157, 256 27 : 251, 4096 538 : 249
+bool use_split(const AttnProblem &P, int sm_count) {
+  if (!split_supported(P, nullptr)) return false;
+  const double Lq = P.mask.Lq, Lk = P.mask.Lk, g = P.H / P.Hkv;
+  auto keys = [&](double queries) {  // that so many neighbouring queries see
+    const double all = Lk - std::min(Lq, Lk) / 2;
+    return P.mask.window > 0 ? std::min(P.mask.window + P.mask.sinks + std::min(queries, Lq), all) : all;
+  };
+  const bool wide = P.D > 128;
+  const double blocks = P.B * std::ceil(g * Lq / 16) * P.Hkv, of_tile = wide ? 64 : 256;
+  const double split =
+      (g * Lq > 8 ? 900 : 500) + blocks / (0.94 * sm_count) * keys(std::ceil(16 / g)) * (wide ? 7 : P.D / 128.0);
+  return split <= 450 + std::ceil(P.B * std::ceil(Lq / of_tile) * P.H / sm_count) * keys(of_tile) * (wide ? 23 : 1);
 }
 
 int window_problem(const llk_tensor4d *q, const llk_tensor4d *k, int dtype, int64_t window, int64_t sinks, float scale,
@@ -1186,7 +1217,7 @@ int llk_window_attention_scratch(const llk_tensor4d *q, const llk_tensor4d *k, i
   DeviceState *ds;
   cudaStream_t stream;
   if ((rc = enter(gpu, nullptr, 0, &ds, &stream)) != LLK_OK) return rc;
-  if (use_split(P)) *bytes = static_cast<int64_t>(split_plan(P, nullptr, ds->sm_count).ws_bytes);
+  if (use_split(P, ds->sm_count)) *bytes = static_cast<int64_t>(split_plan(P, nullptr, ds->sm_count).ws_bytes);
   return LLK_OK;
 }
 
@@ -1215,7 +1246,7 @@ int llk_window_attention(const llk_tensor4d *q, const llk_tensor4d *k, const llk
   const bool keys = P.mask.Lk > 0;
   const void *ptrs[6] = {q->data, o->data, keys ? k->data : nullptr, keys ? v->data : nullptr, q_lens, kv_lens};
   if ((rc = enter(gpu, ptrs, 6, &ds, &stream)) != LLK_OK) return rc;
-  if (use_split(P)) {
+  if (use_split(P, ds->sm_count)) {
     std::lock_guard<std::mutex> lk(ds->mu);
     const SplitPlan plan = split_plan(P, nullptr, ds->sm_count);
     void *ws;
