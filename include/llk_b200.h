@@ -193,7 +193,9 @@ int llk_attention(const float *q, const float *k, const float *v, float *o, int6
  * (h' = h / (H / Hkv)).  A query that sees no key gives zeros; rows i >= m of
  * O are left as they were.  Keys and values that a query does not see do not
  * affect it, whatever they hold (infinities and NaN included).  O must not
- * overlap q, k or v. */
+ * overlap q, k or v.  The rows of an output must not overlap one another:
+ * each of its strides is at least what the dimensions of smaller strides
+ * reach over (else LLK_ERR_ALIGN). */
 
 /* [B, H, L, D]: strides in elements, stride[3] must be 1, none negative. */
 typedef struct llk_tensor4d {
