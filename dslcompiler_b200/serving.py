@@ -220,8 +220,11 @@ class QuantizedKVCache:
             raise TypeError("slots must be a torch.int64 CUDA tensor [B, L]")
         ps = _check_ints("slots", slots, torch.int64, tuple(slots.shape))
         if out is None:
-            shape = (slots.shape[0], self.kv_heads, slots.shape[1], self.head_dim)
-            k, v = torch.empty((2,) + shape, dtype=dtype or torch.bfloat16, device=self.device).unbind(0)
+            if dtype is not None and dtype not in _DTYPES:
+                raise TypeError(f"dtype must be one of {', '.join(str(d) for d in _DTYPES)}")
+            # (on the cache's device, where the slots have to be too)
+            k, v = self.k_params.new_empty((2, slots.shape[0], self.kv_heads, slots.shape[1], self.head_dim),
+                                           dtype=dtype).unbind(0)
             if stream is not None:
                 _used_on(k, stream)
                 _used_on(v, stream)
@@ -229,10 +232,10 @@ class QuantizedKVCache:
             k, v = out
             if dtype is not None and k.dtype != dtype:
                 raise TypeError(f"out must be {dtype}")
-        _check_data("k", k)
-        _check_data("v", v, dtype=k.dtype)
-        if (k.shape[0], k.shape[2]) != tuple(slots.shape):
-            raise ValueError("out must be [B, kv_heads, L, head_dim] with the slots' B and L")
+            _check_data("k", k)
+            _check_data("v", v, dtype=k.dtype)
+            if (k.shape[0], k.shape[2]) != tuple(slots.shape):
+                raise ValueError("out must be [B, kv_heads, L, head_dim] with the slots' B and L")
         g = gpu_context(self.device.index, _stream_of(slots, stream))
         rc = lib().llk_kv_cache_read(self._c, _tensor4d(k), _tensor4d(v, 1), _DTYPES[k.dtype], ps, g)
         if rc:
