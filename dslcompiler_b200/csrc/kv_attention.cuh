@@ -28,6 +28,20 @@
 // with s and m in f32 and p_t s_t rounded to f16.  The running reference of
 // the softmax is the maximum of score + log2(s of v), so p_t s_t is at most 1
 // whatever the scales are, and 11 bits of it are kept.
+//
+// The work is dealt by cost, not by sequence: every CTA gets the same number
+// of units of 128 tokens (a begun segment counts two more), whatever lengths
+// the sequences have, and segments that two CTAs share are joined by a second
+// small kernel.
+//
+// Measured: 4 x 64 heads over 8, D = 128, 4 bits, 131072 tokens: 125 us, 4.5
+// TB/s of codes, scales and minima (0.69 of the measured HBM rate; unpacking
+// and the softmax keep the issue slots busy, and SMs differ by 20 %); 32
+// sequences of 4096: 34 us for 14.5, 9 of them what a call over one sequence
+// of 517 tokens takes (find the segment 1, first loads 2, queries 1, sums and
+// output 2.5, the joining kernel 3).  Dense bf16, 16 x 32 heads over 8, 4096
+// of 8192 tokens: 48 us, 0.85 of the HBM rate.  Shifting by mul.hi instead of
+// by the ALU took 135 for then 124 us.
 #pragma once
 
 #include <atomic>
