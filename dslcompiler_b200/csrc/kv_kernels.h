@@ -50,6 +50,18 @@ struct KvPool {
 bool window_simt_supported(const AttnProblem &p);
 cudaError_t window_simt_launch(const AttnProblem &p, cudaStream_t stream);
 
+// f32, few query rows over many keys, split along the keys: rows of K and V
+// on 16 bytes, D a multiple of 4.
+struct RowsPlan {
+  int splits;       // shares of the keys
+  int rows;         // query rows of a block, 4 or 8
+  int row_blocks;   // blocks of query rows of one key head
+  size_t ws_bytes;  // device workspace the launch needs
+};
+bool rows_supported(const AttnProblem &p);
+RowsPlan rows_plan(const AttnProblem &p, int sm_count);
+cudaError_t rows_launch(const AttnProblem &p, const RowsPlan &plan, void *workspace, cudaStream_t stream);
+
 // Tensor-core kernel for prompts: bf16 / f16, D <= 128, rows on 16 bytes.
 // encode_fn: cuTensorMapEncodeTiled; status: the device's error word (a
 // bounded wait that gave up).

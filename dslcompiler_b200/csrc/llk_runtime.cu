@@ -1141,6 +1141,29 @@ bool use_split(const AttnProblem &P, int sm_count) {
   return split <= 450 + std::ceil(P.B * std::ceil(Lq / of_tile) * P.H / sm_count) * keys(of_tile) * (wide ? 23 : 1);
 }
 
+// The same choice in f32, in us: blocks of 8 rows of a key head that share
+// the keys out against tiles of 64 rows of a head, in the times a key that
+// were measured at D <= 64, 128 and 256.  Without a window, r = H / Hkv Lq
+// rows, us rows : tiles --
+//   B H Hkv = 16 32 8, L 4096, D 128:  r = 4 128 : 1049, 32 642 : 1049, 64 1125 : 1050
+//   1 32 8, L 8192, D 128:  r = 4 27 : 976, 256 643 : 999
+//   4 32 32, L 2048, D 128:  r = 16 182 : 254, 32 338 : 298
+//   1 8 8, L 500, D 64:  r = 1 9.5 : 38, 500 35 : 39
+//   2 8 2, L 1024, D 256:  r = 4 19 : 135, 256 116 : 231, 4096 770 : 233
+bool use_rows(const AttnProblem &P, int sm_count) {
+  if (!rows_supported(P)) return false;
+  const double Lq = P.mask.Lq, Lk = P.mask.Lk, g = P.H / P.Hkv;
+  const double row_us = P.D <= 64 ? 0.032 : P.D <= 128 ? 0.05 : 0.15, tile_us = P.D <= 64 ? 0.075 : P.D <= 128 ? 0.13 : 0.18;
+  const double blocks = P.B * std::ceil(g * Lq / 8) * P.Hkv;
+  const double waves = std::ceil(P.B * std::ceil(Lq / 64) * P.H / (sm_count * (P.D > 128 ? 1 : 2)));
+  auto keys = [&](double queries, double all) {  // that so many neighbouring queries see
+    return P.mask.window > 0 ? std::min(P.mask.window + P.mask.sinks + std::min(queries, Lq), all) : all;
+  };
+  const double mean = Lk - std::min(Lq, Lk) / 2;  // (one wave takes as long as its longest tile)
+  return 7 + blocks / sm_count * keys(std::ceil(8 / g), mean) * row_us <=
+         5 + waves * keys(64, waves > 1 ? mean : Lk) * tile_us;
+}
+
 int window_problem(const llk_tensor4d *q, const llk_tensor4d *k, int dtype, int64_t window, int64_t sinks, float scale,
                    AttnProblem *P) {
   int rc = attn_problem(q, k->dim[1], k->dim[2], dtype, window, sinks, scale, P);
@@ -1217,7 +1240,11 @@ int llk_window_attention_scratch(const llk_tensor4d *q, const llk_tensor4d *k, i
   DeviceState *ds;
   cudaStream_t stream;
   if ((rc = enter(gpu, nullptr, 0, &ds, &stream)) != LLK_OK) return rc;
-  if (use_split(P, ds->sm_count)) *bytes = static_cast<int64_t>(split_plan(P, nullptr, ds->sm_count).ws_bytes);
+  if (dtype == LLK_DTYPE_FP32) {
+    if (use_rows(P, ds->sm_count)) *bytes = static_cast<int64_t>(rows_plan(P, ds->sm_count).ws_bytes);
+  } else if (use_split(P, ds->sm_count)) {
+    *bytes = static_cast<int64_t>(split_plan(P, nullptr, ds->sm_count).ws_bytes);
+  }
   return LLK_OK;
 }
 
@@ -1252,6 +1279,13 @@ int llk_window_attention(const llk_tensor4d *q, const llk_tensor4d *k, const llk
     void *ws;
     if ((rc = split_workspace(*ds, plan.ws_bytes, ctx, stream, &ws)) != LLK_OK) return rc;
     return launched(split_launch(P, nullptr, nullptr, 0, plan, ws, stream));
+  }
+  if (use_rows(P, ds->sm_count)) {
+    std::lock_guard<std::mutex> lk(ds->mu);
+    const RowsPlan plan = rows_plan(P, ds->sm_count);
+    void *ws;
+    if ((rc = split_workspace(*ds, plan.ws_bytes, ctx, stream, &ws)) != LLK_OK) return rc;
+    return launched(rows_launch(P, plan, ws, stream));
   }
   if (window_tc_supported(P))
     return launched(window_tc_launch(reinterpret_cast<void *>(g_encode), P, ds->status, ds->sm_count, stream));

@@ -98,6 +98,36 @@ def test_window_attention_many_short_sequences(D, Hkv, g, Lq, L, window, sinks, 
     check(out, o, A, S, D, L, dtype, ref.HALF_STEP[dtype], ql, 7.0)
 
 
+@pytest.mark.parametrize("B,D,Hkv,g,Lq,L,window,sinks", [(50, 128, 8, 4, 1, 900, 0, 0), (2, 128, 2, 4, 3, 5000, 0, 0),
+                                                         (1, 64, 4, 1, 1, 4097, 0, 0), (3, 80, 2, 5, 2, 2000, 700, 33),
+                                                         (2, 256, 2, 9, 1, 3000, 0, 0), (4, 40, 3, 1, 20, 1111, 100, 7),
+                                                         (2, 4, 2, 2, 5, 600, 0, 0), (1, 128, 1, 16, 7, 2500, 17, 300),
+                                                         (9, 252, 4, 2, 1, 640, 64, 1)])
+def test_window_attention_f32_few_queries(B, D, Hkv, g, Lq, L, window, sinks):
+    q, k, v = rand(1, (B, Hkv * g, Lq, D), F32), rand(2, (B, Hkv, L, D), F32), rand(3, (B, Hkv, L, D), F32)
+    kv = lens_of(L, B, L, [L, 1, 0, 127])
+    ql = lens_of(Lq, B, Lq, [Lq, Lq, Lq, 0])
+    out = torch.full_like(q, 7.0)
+    llk.window_attention(q, k, v, window=window, sinks=sinks, q_lens=ints(ql), kv_lens=ints(kv), out=out)
+    o, A, S = plain(q, k, v, v.abs(), ql, kv, window, sinks)
+    check(out, o, A, S, D, L, F32, 0.0, ql, 7.0)
+    # infinities and NaN where no query looks, and in the last key of the first sequence
+    for b, n in enumerate(kv):
+        k[b, :, n:], v[b, :, n:] = math.nan, math.inf
+    if window and L > 2 * (window + Lq):
+        k[0, :, sinks : L - window - Lq - 20], v[0, :, sinks : L - window - Lq - 20] = math.inf, math.nan
+    again = torch.full_like(q, 7.0)
+    llk.window_attention(q, k, v, window=window, sinks=sinks, q_lens=ints(ql), kv_lens=ints(kv), out=again)
+    assert torch.equal(out, again)
+    v[0, :, L - 1] = math.inf
+    llk.window_attention(q, k, v, window=window, sinks=sinks, q_lens=ints(ql), kv_lens=ints(kv), out=again)
+    assert torch.equal(out[1:], again[1:])
+    assert not torch.isfinite(again[0, :, Lq - 1]).any()
+    before = out[0, :, : Lq - 1].double()  # the queries before the last do not see it
+    assert ((again[0, :, : Lq - 1].double() - before).abs() <= 2 * ref.bound(
+        o[0, :, : Lq - 1], A[0, :, : Lq - 1], S[0, :, : Lq - 1], D, L, F32, 0.0)).all()
+
+
 def pool_of(B, Hkv, L, D, bits, group, page):
     """A cache of random contents, its table, and (k, v, |s code| + |min| of v) in float64."""
     W = -(-L // page)
