@@ -26,7 +26,7 @@ LIB = os.path.join(OUT_DIR, "libllk_b200.so")
 
 SOURCES = ["swiglu_tc.cu", "swiglu_tc2.cu", "swiglu_decode.cu", "swiglu_simt.cu", "llk_runtime.cu", "swiglu_decode_noalloc.cu", "shard_gather.cu",
            "rope_attention.cu", "window_attention.cu", "window_attention_tc.cu", "window_attention_rows.cu",
-           "kv_cache.cu", "kv_attention.cu", "kv_attention_dense.cu"]
+           "kv_cache.cu", "kv_attention.cu", "kv_attention_f16.cu", "kv_attention_dense.cu"]
 HEADERS = ["sm100_ptx.cuh", "tc_kernels.h", "decode_kernels.h", "workspace.h",
            "attention_kernels.h", "kv_kernels.h", "attn_common.cuh", "kv_attention.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,5 +1,5 @@
-// kv_attention.cu -- attention over the quantised paged cache, and the plan
-// of the split kernels (kv_attention.cuh).
+// kv_attention.cu -- attention over the quantised paged cache in bf16, and the
+// plan of the split kernels (kv_attention.cuh).
 #include <type_traits>
 
 #include "kv_attention.cuh"
@@ -7,30 +7,6 @@
 namespace llk_b200 {
 
 using namespace split_attn;
-
-namespace {
-
-template <int BITS, int D, int G>
-cudaError_t launch_nt(const Params &a, cudaStream_t stream) {
-  if constexpr (row_tiles(16, D) == 2)
-    if (row_tiles(a.p.H / a.p.Hkv * a.p.mask.Lq, D) == 2) return launch_split<BITS, D, G, false, 2>(a, stream);
-  return launch_split<BITS, D, G, false, 1>(a, stream);
-}
-
-template <int BITS>
-cudaError_t launch_bits(const Params &a, cudaStream_t stream) {
-  const int groups = a.p.D / a.pool.group;
-  if (a.p.D == 64) return groups == 1 ? launch_nt<BITS, 64, 1>(a, stream) : launch_nt<BITS, 64, 2>(a, stream);
-  if (a.p.D == 128)
-    return groups == 1   ? launch_nt<BITS, 128, 1>(a, stream)
-           : groups == 2 ? launch_nt<BITS, 128, 2>(a, stream)
-                         : launch_nt<BITS, 128, 4>(a, stream);
-  return groups == 2   ? launch_nt<BITS, 256, 2>(a, stream)
-         : groups == 4 ? launch_nt<BITS, 256, 4>(a, stream)
-                       : launch_nt<BITS, 256, 8>(a, stream);
-}
-
-}  // namespace
 
 bool split_supported(const AttnProblem &p, const KvPool *pool) {
   const int64_t g = p.Hkv > 0 ? p.H / p.Hkv : 0, rows = g * p.mask.Lq;
@@ -63,8 +39,9 @@ SplitPlan split_plan(const AttnProblem &p, const KvPool *pool, int sm_count) {
   }
   const int64_t segments = static_cast<int64_t>(p.B) * p.Hkv * s.row_blocks;
   const int64_t units = segments * (keys > kSpan ? (keys + kSpan - 1) / kSpan : 1), cost = units + segments * kStart;
+  const bool two = pool && p.dtype == LLK_DTYPE_FP16;
   const int64_t room = static_cast<int64_t>(sm_count) *
-                       ctas_per_sm(pool ? pool->bits : 16, p.D, pool ? p.D / pool->group : 1, nt);
+                       ctas_per_sm(pool ? pool->bits : 16, p.D, pool ? p.D / pool->group : 1, nt, two);
   s.workers = static_cast<int>(cost < room ? cost : room);
   s.ws_bytes = 0;
   if (units > segments)  // else no segment has more than one unit: none is cut
@@ -92,7 +69,8 @@ cudaError_t split_launch(const AttnProblem &p, const KvPool *pool, const int *bl
     a.part_o = reinterpret_cast<float *>(a.part_ml + 2 * static_cast<size_t>(plan.workers) * 8 * nt);
   }
   if (!pool) return launch_dense(a, stream);
-  return pool->bits == 4 ? launch_bits<4>(a, stream) : launch_bits<8>(a, stream);
+  if (p.dtype == LLK_DTYPE_FP16) return launch_cache_f16(a, stream);
+  return pool->bits == 4 ? launch_bits<4, false>(a, stream) : launch_bits<8, false>(a, stream);
 }
 
 }  // namespace llk_b200

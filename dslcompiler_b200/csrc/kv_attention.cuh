@@ -1,6 +1,7 @@
 // kv_attention.cuh -- attention of few query rows over many keys, split along
 // the keys: over the quantised paged cache (4 or 8 bits) and over dense 16-bit
-// keys and values.  Instantiated by kv_attention.cu and kv_attention_dense.cu.
+// keys and values.  Instantiated by kv_attention.cu (cache, bf16),
+// kv_attention_f16.cu (cache, f16) and kv_attention_dense.cu.
 //
 // HBM-bound: every key and value byte is read once.  A warp works on blocks
 // of 16 tokens of its own: cp.async copies them into its ring of stages in
@@ -25,7 +26,10 @@
 // a shift per four).  A group's scale and minimum never touch the codes:
 //   score(t) = s_t (q . c_t) + m_t sum(q),
 //   O        = sum_t (p_t s_t) c_t + sum_t p_t m_t,
-// with s and m in f32 and p_t s_t rounded to f16.  The running reference of
+// with s and m in f32 and p_t s_t rounded to f16, or to the sum of two f16
+// (kTwo) where the output is f16: one rounding moves values that are small
+// against s c and m, of which they are the difference, by more than the
+// output's own (measured: 5.0e-4 of the result for 2.1e-4).  The running reference of
 // the softmax is the maximum of score + log2(s of v), so p_t s_t is at most 1
 // whatever the scales are, and 11 bits of it are kept.
 //
@@ -340,7 +344,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // A block that does not exist, or whose page is not in the pool.
 constexpr uint32_t kNoBlock = 0xffffffffu;
 
-template <int BITS, int D, int G, bool kBf16, int NT, int CTAS>
+template <int BITS, int D, int G, bool kBf16, bool kTwo, int NT, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_constant__ Params A) {
   using X = Geo<BITS, D, G>;
   constexpr int E = X::E, WK = X::WK, VW = X::VW, NU = X::NU, UR = X::UR, UT = X::UT;
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
             }
           }
         }
-        constexpr int kLo = kBf16 ? 2 : 1;  // bf16 weights as a sum of two, so that their rounding does not show
+        constexpr int kLo = kTwo ? 2 : 1;  // weights as a sum of two, so that their rounding does not show
         uint32_t bw[kQuant ? G : 1][NT][2][kLo];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -876,9 +880,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
               }
               const uint32_t hi = pack2<kBf16>(w0, w1);
               bw[gi][nt][i][0] = movmatrix_trans(hi);
-              if constexpr (kBf16) {
-                const float2 back = unpack2<true>(hi);
-                bw[gi][nt][i][1] = movmatrix_trans(pack2<true>(w0 - back.x, w1 - back.y));
+              if constexpr (kTwo) {
+                const float2 back = unpack2<kBf16>(hi);
+                bw[gi][nt][i][1] = movmatrix_trans(pack2<kBf16>(w0 - back.x, w1 - back.y));
               }
             }
           }
@@ -908,8 +912,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
                   const int tile = u * UT + 2 * w + hf;
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt)
-                    mma16816<false>(acc[tile][nt], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, d & 0x00ff00ffu,
-                                    (d >> 8) & 0x00ff00ffu, bw[gi][nt][0][0], bw[gi][nt][1][0]);
+#pragma unroll
+                    for (int q = 0; q < kLo; ++q)
+                      mma16816<false>(acc[tile][nt], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, d & 0x00ff00ffu,
+                                      (d >> 8) & 0x00ff00ffu, bw[gi][nt][0][q], bw[gi][nt][1][q]);
                 } else {
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {
@@ -917,8 +923,10 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
                     const int tile = u * UT + 4 * w + 2 * hf + k;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                      mma16816<false>(acc[tile][nt], as & 0x000f000fu, as & 0x00f000f0u, ds & 0x000f000fu,
-                                      ds & 0x00f000f0u, bw[gi][nt][0][0], bw[gi][nt][1][0]);
+#pragma unroll
+                      for (int q = 0; q < kLo; ++q)
+                        mma16816<false>(acc[tile][nt], as & 0x000f000fu, as & 0x00f000f0u, ds & 0x000f000fu,
+                                        ds & 0x00f000f0u, bw[gi][nt][0][q], bw[gi][nt][1][q]);
                   }
                 }
               }
@@ -1098,8 +1106,10 @@ constexpr int split_smem(int bits, int D, int G, int NT) {
 // operand, a block's codes) and 228 KB of shared memory leave.  Not to the
 // last KB: CTAs that come and go one by one leave gaps (measured: 6 of 148
 // SMs then held one less, and their work waited for a whole CTA's time).
-constexpr int ctas_per_sm(int bits, int D, int G, int NT) {
-  const int by_regs = D == 256    ? (bits == 16 ? 1 : 2)
+// With weights of two parts no more than without: llk_kv_cache_attention_scratch
+// does not know the type.
+constexpr int ctas_per_sm(int bits, int D, int G, int NT, bool two) {
+  const int by_regs = bits < 16 && two && D < 256 ? (NT == 2 ? 2 : D == 64 && G == 1 ? 4 : 3) : D == 256    ? (bits == 16 ? 1 : 2)
                       : NT == 2   ? (D == 64 ? 3 : 2)
                       : bits == 16 ? (D == 128 ? 2 : 3)
                                    : (D == 128 && (bits == 8 || G > 1) ? 3 : 4);
@@ -1108,12 +1118,12 @@ constexpr int ctas_per_sm(int bits, int D, int G, int NT) {
   return by_regs < by_smem ? by_regs : by_smem;
 }
 
-template <int BITS, int D, int G, bool kBf16, int NT>
+template <int BITS, int D, int G, bool kBf16, bool kTwo, int NT>
 cudaError_t launch_split(const Params &a, cudaStream_t stream) {
   using X = Geo<BITS, D, G>;
-  constexpr int CTAS = ctas_per_sm(BITS, D, G, NT), smem = split_smem(BITS, D, G, NT);
+  constexpr int CTAS = ctas_per_sm(BITS, D, G, NT, kTwo), smem = split_smem(BITS, D, G, NT);
   static_assert(smem >= kWarps * X::STAGES * X::STAGE, "the rings' place");
-  auto kern = split_kernel<BITS, D, G, kBf16, NT, CTAS>;
+  auto kern = split_kernel<BITS, D, G, kBf16, kTwo, NT, CTAS>;
   auto join = combine_kernel<D, kBf16, BITS == 16>;
   // Once a device.  Both kernels ask for the largest shared memory: while one
   // drains and the next one's CTAs move in, an SM cannot change its split of
@@ -1153,7 +1163,28 @@ cudaError_t launch_split(const Params &a, cudaStream_t stream) {
 // rows than that and the accumulators leave registers for it.
 constexpr int row_tiles(int rows, int D) { return rows > 8 && D <= 128 ? 2 : 1; }
 
-cudaError_t launch_dense(const Params &a, cudaStream_t stream);  // kv_attention_dense.cu
+template <int BITS, int D, int G, bool kTwo>
+cudaError_t launch_cache_nt(const Params &a, cudaStream_t stream) {
+  if constexpr (row_tiles(16, D) == 2)
+    if (row_tiles(a.p.H / a.p.Hkv * a.p.mask.Lq, D) == 2) return launch_split<BITS, D, G, false, kTwo, 2>(a, stream);
+  return launch_split<BITS, D, G, false, kTwo, 1>(a, stream);
+}
+
+template <int BITS, bool kTwo>
+cudaError_t launch_bits(const Params &a, cudaStream_t stream) {
+  const int groups = a.p.D / a.pool.group;
+  if (a.p.D == 64) return groups == 1 ? launch_cache_nt<BITS, 64, 1, kTwo>(a, stream) : launch_cache_nt<BITS, 64, 2, kTwo>(a, stream);
+  if (a.p.D == 128)
+    return groups == 1   ? launch_cache_nt<BITS, 128, 1, kTwo>(a, stream)
+           : groups == 2 ? launch_cache_nt<BITS, 128, 2, kTwo>(a, stream)
+                         : launch_cache_nt<BITS, 128, 4, kTwo>(a, stream);
+  return groups == 2   ? launch_cache_nt<BITS, 256, 2, kTwo>(a, stream)
+         : groups == 4 ? launch_cache_nt<BITS, 256, 4, kTwo>(a, stream)
+                       : launch_cache_nt<BITS, 256, 8, kTwo>(a, stream);
+}
+
+cudaError_t launch_dense(const Params &a, cudaStream_t stream);      // kv_attention_dense.cu
+cudaError_t launch_cache_f16(const Params &a, cudaStream_t stream);  // kv_attention_f16.cu
 
 }  // namespace split_attn
 }  // namespace llk_b200

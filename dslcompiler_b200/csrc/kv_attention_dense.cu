@@ -12,8 +12,8 @@ namespace {
 template <bool kBf16, int D>
 cudaError_t launch_nt(const Params &a, cudaStream_t stream) {
   if constexpr (row_tiles(16, D) == 2)
-    if (row_tiles(a.p.H / a.p.Hkv * a.p.mask.Lq, D) == 2) return launch_split<16, D, 1, kBf16, 2>(a, stream);
-  return launch_split<16, D, 1, kBf16, 1>(a, stream);
+    if (row_tiles(a.p.H / a.p.Hkv * a.p.mask.Lq, D) == 2) return launch_split<16, D, 1, kBf16, kBf16, 2>(a, stream);
+  return launch_split<16, D, 1, kBf16, kBf16, 1>(a, stream);
 }
 
 template <bool kBf16>

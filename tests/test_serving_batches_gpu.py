@@ -173,6 +173,21 @@ def test_cache_attention_many_short_sequences(bits, D, group, Hkv, g, Lq, L, win
         assert (got[b, :, : ql[b]] == 0).all() and (got[b, :, ql[b] :] == 7.0).all()
 
 
+@pytest.mark.parametrize("bits,D,group,Lq", [(4, 64, 64, 1), (4, 64, 32, 3), (4, 128, 128, 1), (4, 128, 64, 1),
+                                             (4, 128, 32, 4), (4, 256, 64, 1), (8, 64, 32, 2), (8, 128, 32, 1),
+                                             (8, 128, 128, 5), (8, 256, 128, 1)])
+def test_cache_attention_f16_keeps_its_precision(bits, D, group, Lq):
+    """In f16 the weights are sums of two f16: 2^-22 of each, and of a small one 2^-25 of the largest."""
+    B, Hkv, g, L = 3, 4, 4, 333
+    cache, table, k, v, slack = pool_of(B, Hkv, L, D, bits, group, 16)
+    lens = [L, 3, 40]
+    q = rand(1, (B, Hkv * g, Lq, D), F16)
+    out = cache.attention(q, table, ints(lens))
+    o, A, S = plain(q, k, v, slack, [Lq] * B, lens, 0, 0)
+    tol = ref.bound(o, A, S, D, L, F16, 2.0**-22) + L * 2.0**-24 * slack.amax()
+    assert ((out.double() - o).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("dtype,bits", [(BF16, 4), (F16, 8), (F32, 4)])
 @pytest.mark.parametrize("B,L,Hkv,D", [(1, 1, 1, 64), (3, 5, 7, 64), (1, 149, 3, 128), (2, 4097, 1, 64),
                                        (5, 1111, 2, 256), (1, 9001, 4, 128)])
