@@ -4,7 +4,9 @@ with its writer, reader and attention (``llk_kv_cache_*``).
 
 Tensors are torch CUDA tensors, [B, H, L, D] in any order of strides (unit
 stride along D); calls run asynchronously on the current torch stream of
-their device, or on ``stream``.  There is no CPU path and no host staging.
+their device, or on ``stream``: the caller orders that stream behind what made
+the inputs, and its own use of the result behind that stream.  There is no CPU
+path and no host staging.
 """
 from __future__ import annotations
 
@@ -75,9 +77,29 @@ def _ranges(window, sinks):
     return min(window, 2**62), min(sinks, 2**62)
 
 
-def _new_out(q, q_lens):
+def _made_on(stream, device, make):
+    """make()'s tensor, taken from the allocator and filled on the stream that the call runs on: nothing orders work
+    queued on torch's current stream (a fill, or the last use of a block that the allocator hands out again) before a
+    kernel on another one."""
+    if stream is None:
+        return make()
+    s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device)
+    with torch.cuda.stream(s):
+        return make()
+
+
+def _new_out(make, device, stream):
+    """An output that the caller gets: it may be used on the current stream too, so its memory is handed out again
+    only behind the work queued there by then."""
+    out = _made_on(stream, device, make)
+    if stream is not None:
+        out.record_stream(torch.cuda.current_stream(device))
+    return out
+
+
+def _out_like(q, q_lens, stream):
     # rows behind a sequence's queries are not written: they read as zeros
-    return torch.empty_like(q) if q_lens is None else torch.zeros_like(q)
+    return _new_out(lambda: torch.empty_like(q) if q_lens is None else torch.zeros_like(q), q.device, stream)
 
 
 def _scratch(nbytes, like, stream):
@@ -85,16 +107,8 @@ def _scratch(nbytes, like, stream):
     share it."""
     if not nbytes:
         return None, None
-    buf = like.new_empty((nbytes + 1) // 2)
-    if stream is not None:
-        _used_on(buf, stream)
+    buf = _made_on(stream, like.device, lambda: like.new_empty((nbytes + 1) // 2))
     return buf, KernelContext(buf.data_ptr(), nbytes)
-
-
-def _used_on(t, stream):
-    """The allocator hands t's memory out again only behind the work now queued on `stream`."""
-    s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=t.device)
-    t.record_stream(s)
 
 
 # How much scratch a call needs follows from its sizes.
@@ -128,17 +142,14 @@ def window_attention(q, k, v, *, window=0, sinks: int = 0, scale: float | None =
     B, D = q.shape[0], q.shape[3]
     pq = None if q_lens is None else _check_ints("q_lens", q_lens, torch.int32, (B,))
     pk = None if kv_lens is None else _check_ints("kv_lens", kv_lens, torch.int32, (B,))
-    made = out is None
-    if made:
-        out = _new_out(q, q_lens)
+    if out is None:
+        out = _out_like(q, q_lens, stream)
     else:
         _check_data("out", out, dtype=q.dtype)
     dtype = _DTYPES[q.dtype]
     need = _window_scratch(tuple(q.shape), tuple(k.shape), k.stride(), k.data_ptr() % 16 == 0, dtype, window, sinks,
                            q.device.index)
     buf, ctx = _scratch(need, q, stream)
-    if made and stream is not None:
-        _used_on(out, stream)
     g = gpu_context(q.device.index, _stream_of(q, stream))
     rc = lib().llk_window_attention(_tensor4d(q), _tensor4d(k, 1), _tensor4d(v, 2), _tensor4d(out, 3), dtype, pq, pk,
                                     window, sinks, 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale), ctx, g)
@@ -223,11 +234,8 @@ class QuantizedKVCache:
             if dtype is not None and dtype not in _DTYPES:
                 raise TypeError(f"dtype must be one of {', '.join(str(d) for d in _DTYPES)}")
             # (on the cache's device, where the slots have to be too)
-            k, v = self.k_params.new_empty((2, slots.shape[0], self.kv_heads, slots.shape[1], self.head_dim),
-                                           dtype=dtype).unbind(0)
-            if stream is not None:
-                _used_on(k, stream)
-                _used_on(v, stream)
+            shape = (2, slots.shape[0], self.kv_heads, slots.shape[1], self.head_dim)
+            k, v = _new_out(lambda: self.k_params.new_empty(shape, dtype=dtype), self.device, stream).unbind(0)
         else:
             k, v = out
             if dtype is not None and k.dtype != dtype:
@@ -257,16 +265,13 @@ class QuantizedKVCache:
             raise ValueError("block_table must be [B, pages a sequence] with unit stride along its rows")
         pk = _check_ints("kv_lens", kv_lens, torch.int32, (B,))
         pq = None if q_lens is None else _check_ints("q_lens", q_lens, torch.int32, (B,))
-        made = out is None
-        if made:
-            out = _new_out(q, q_lens)
+        if out is None:
+            out = _out_like(q, q_lens, stream)
         else:
             _check_data("out", out, dtype=q.dtype)
         W = block_table.shape[1]
         buf, ctx = _scratch(_cache_scratch(tuple(q.shape), self.page_size, self.kv_heads, self.head_dim, self.bits,
                                            self.group_size, W, window, sinks, q.device.index), q, stream)
-        if made and stream is not None:
-            _used_on(out, stream)
         g = gpu_context(self.device.index, _stream_of(q, stream))
         rc = lib().llk_kv_cache_attention(_tensor4d(q), self._c, block_table.data_ptr(), W,
                                           block_table.stride(0) if B > 1 else W, pq, pk, _tensor4d(out, 1),
