@@ -247,9 +247,11 @@ __device__ __forceinline__ void quantise_in(const Piece<T> &raw, float2 range, u
     const uint64_t d = add2(f32x2(x(e), x(e + 4)), m2);
     uint64_t q = mul2(d, inv2);
     q = fma2(fma2(q, s2, d), inv2, q);
-    // (a lower bound only where m may lie above the smallest element, an upper
-    // one only where the scale's rounding can push the largest past the top)
-    constexpr bool kLow = !std::is_same<T, __nv_bfloat16>::value, kHigh = BITS == 8;
+    // (a lower bound only where m may lie above the smallest element: bf16
+    // elements are their own bf16 minimum, but a saturated one, 65504, is not a
+    // bf16; an upper one only where the scale's rounding can push the largest
+    // past the top)
+    constexpr bool kLow = kWild || !std::is_same<T, __nv_bfloat16>::value, kHigh = BITS == 8;
     if constexpr (kLow || kHigh) {
       float2 c = split2(q);
       if constexpr (kLow) c = make_float2(fmaxf(c.x, 0.f), fmaxf(c.y, 0.f));
