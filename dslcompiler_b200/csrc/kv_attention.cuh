@@ -30,7 +30,7 @@
 // (kTwo) where the output is f16: one rounding moves values that are small
 // against s c and m, of which they are the difference, by more than the
 // output's own (measured: 5.0e-4 of the result for 2.1e-4).  The running reference of
-// the softmax is the maximum of score + log2(s of v), so p_t s_t is at most 1
+// the softmax is the maximum of score + log2(|s of v|), so p_t s_t is at most 1
 // whatever the scales are, and 11 bits of it are kept.
 //
 // The work is dealt by cost, not by sequence: every CTA gets the same number
@@ -38,8 +38,8 @@
 // the sequences have, and segments that two CTAs share are joined by a second
 // small kernel.
 //
-// Measured: 4 x 64 heads over 8, D = 128, 4 bits, 131072 tokens: 125 us, 4.5
-// TB/s of codes, scales and minima (0.69 of the measured HBM rate; unpacking
+// Measured: 4 x 64 heads over 8, D = 128, 4 bits, 131072 tokens: 128 us, 4.4
+// TB/s of codes, scales and minima (0.67 of the measured HBM rate; unpacking
 // and the softmax keep the issue slots busy, and SMs differ by 20 %); 32
 // sequences of 4096: 34 us for 14.5, 9 of them what a call over one sequence
 // of 517 tokens takes (find the segment 1, first loads 2, queries 1, sums and
@@ -66,6 +66,16 @@ constexpr float kSlack = 8.f;
 // The reference before any token: below every score, and finite, so that a
 // masked score (-inf) less it is -inf.
 constexpr float kNoRef = -1e38f;
+// A weight carries the magnitude of its token's largest value scale, and each
+// group's ratio to it follows, its sign with it: a caller's pool may hold
+// negative scales, and zeros (slots never written, constant rows of another
+// writer).  The magnitude counts as kLeastScale at least: far below any scale
+// in use, so that a zero leaves the other tokens' weights their bits, and large
+// enough that a token's own weight is not lost below 2^-126.  (The ratio costs
+// a multiplication a weight also where a row is one group: 125 to 128 us at
+// 131072 tokens.  A branch around it, taken by a vote on the block's scales,
+// took 132.)
+constexpr float kLeastScale = 0x1p-60f;
 
 struct Params {
   AttnProblem p;
@@ -772,17 +782,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
           float lg = 0.f;
           rs[hv][i] = 1.f;
           if constexpr (kQuant) {
-            float mx = 0.f;
+            float mx = kLeastScale;
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
               sr[hv][i][gi] = __uint_as_float(par[i][G + gi] << 16);
-              mx = gi == 0 ? sr[hv][i][gi] : fmaxf(mx, sr[hv][i][gi]);
+              mx = fmaxf(mx, fabsf(sr[hv][i][gi]));
             }
             lg = lg2_approx(mx);
             rs[hv][i] = rcp_approx(mx);
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
-              if constexpr (G > 1) sr[hv][i][gi] *= rs[hv][i];
+              sr[hv][i][gi] *= rs[hv][i];
               mr[hv][i][gi] = __uint_as_float(par[i][G + gi] & 0xffff0000u) * rs[hv][i];
             }
           }
@@ -873,10 +883,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
               if constexpr (kQuant) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) pm[nt][gi][j] = fmaf(wt[j], mr[hv][i][gi], pm[nt][gi][j]);
-                if constexpr (G > 1) {
-                  w0 *= sr[hv][i][gi];
-                  w1 *= sr[hv][i][gi];
-                }
+                w0 *= sr[hv][i][gi];
+                w1 *= sr[hv][i][gi];
               }
               const uint32_t hi = pack2<kBf16>(w0, w1);
               bw[gi][nt][i][0] = movmatrix_trans(hi);

@@ -165,7 +165,7 @@ class QuantizedKVCache:
       (4 bits: element 2j in the low nibble of byte j),
     * k_params, v_params bf16 [num_pages, kv_heads, page_size, head_dim / group_size, 2]: (scale, min),
 
-    an element standing for scale * code + min.  head_dim 64, 128 or 256;
+    an element standing for scale * code + min (a zero-filled slot for zeros).  head_dim 64, 128 or 256;
     group_size 32, 64 or 128; page_size a multiple of 16.  Slot number =
     page * page_size + offset; token t of a sequence lies in page
     block_table[b, t // page_size] at offset t % page_size."""
