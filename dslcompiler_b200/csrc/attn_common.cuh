@@ -1,7 +1,7 @@
 // attn_common.cuh -- device helpers the serving attention kernels share: the
 // element types, a sequence's visible key ranges, and the row-by-row form of
-// the operator that a kernel falls back on for a row whose result is not
-// finite.
+// the operator that a kernel falls back on for a row whose result a value that
+// it does not see may have made non-finite.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -56,15 +56,133 @@ __device__ __forceinline__ bool key_visible(int j, int p, int lo, int sinks) {
   return j <= p && (j >= lo || j < sinks);
 }
 
+// ---- Rows whose result is not finite.  The tiled kernels multiply a masked
+// weight 0 with the value row of its tile, which is wrong where that row holds
+// an infinity or NaN.  They find it by the non-finite result; but a row that
+// sees such a value itself, or has a NaN among its own scores, is not finite by
+// right, and there can be as many of those as there are queries.  So a row is
+// redone (attention_row) only where one of the keys that it does not see and
+// its tiles hold has a value that is not finite: those keys lie behind its
+// position or in front of its window, and there are no more of them than a tile
+// has queries (and keys).
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(T x, bool inf) {  // inf: only infinities
+  const float f = fabsf(to_f32(x));
+  return inf ? f == INFINITY : !(f < INFINITY);
+}
+
+// The first of the rows from, from + step, .. (count of them, step 1 or -1) of
+// v that holds a value that is not finite (inf: an infinity), or -1.  By one
+// warp.  `tick` (as in attention_row) may be null.
+template <typename T>
+__device__ __noinline__ int bad_row(const T *v, int64_t v_sl, int D, int from, int count, int step, bool inf,
+                                    int *tick) {
+  constexpr int kAt = 8, kVec = 16 / sizeof(T), kNone = 0x7fffffff;
+  const int lane = threadIdx.x & 31;
+  // pieces of a row, 16 bytes where rows start there, and rows of a round of kAt pieces a lane
+  const bool vec = ((reinterpret_cast<uintptr_t>(v) | v_sl * sizeof(T) | D * sizeof(T)) & 15) == 0;
+  const int pieces = vec ? D / kVec : D, rows = 32 * kAt / pieces;  // (D <= 256: a row at least)
+  int row[kAt];
+  const T *at[kAt];
+#pragma unroll
+  for (int u = 0; u < kAt; ++u) {
+    const int c = lane + 32 * u;
+    row[u] = c / pieces < rows ? c / pieces : kNone;
+    at[u] = v + static_cast<int64_t>(from + (row[u] < rows ? row[u] : 0) * step) * v_sl + c % pieces * (vec ? kVec : 1);
+  }
+  for (int j = 0; j < count; j += rows) {
+    int found = kNone;
+    uint4 x[kAt];
+#pragma unroll
+    for (int u = 0; u < kAt; ++u) {
+      x[u] = make_uint4(0, 0, 0, 0);
+      if (row[u] < count - j) {
+        if (vec) {
+          x[u] = *reinterpret_cast<const uint4 *>(at[u]);
+        } else {
+          *reinterpret_cast<T *>(&x[u]) = *at[u];
+        }
+      }
+      at[u] += static_cast<int64_t>(rows) * step * v_sl;
+    }
+#pragma unroll
+    for (int u = 0; u < kAt; ++u) {
+      const T *e = reinterpret_cast<const T *>(&x[u]);
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) bad |= not_finite(e[i], inf);
+      if (bad && j + row[u] < found) found = j + row[u];
+    }
+    found = __reduce_min_sync(0xffffffffu, found);
+    if (found != kNone) return from + found * step;
+    if (tick && lane == 0) atomicAdd(tick, 1);
+  }
+  return -1;
+}
+
+// What of the values hidden from a warp's rows is not finite: the last of the
+// keys behind the first row's position p0 (before hi), and the first of those
+// from `from` to before the last row's window, last_lo; -1 for none.
+struct HiddenBad {
+  int late, early;
+  // whether a row at position p with its window from lo may have met one
+  __device__ __forceinline__ bool meets(int p, int lo) const { return (late >= 0 && late > p) || (early >= 0 && early < lo); }
+};
+template <typename T>
+__device__ __forceinline__ HiddenBad hidden_bad(const T *v, int64_t v_sl, int D, int p0, int hi, int from, int last_lo,
+                                                int *tick = nullptr) {
+  const int first = p0 + 1 > 0 ? p0 + 1 : 0;
+  HiddenBad b;
+  b.late = hi > first ? bad_row(v, v_sl, D, hi - 1, hi - first, -1, false, tick) : -1;
+  b.early = last_lo > from ? bad_row(v, v_sl, D, from, last_lo - from, 1, false, tick) : -1;
+  return b;
+}
+
+// The same for one row at position p of a sequence of n keys and m queries whose
+// window begins at lo: whether it is to be redone.  k16: the tiles' weights were
+// one f16 or a sum of two numbers, and one that is 0 there (or a sum of either
+// sign) times an infinity that the row does see is NaN, not so by the
+// definition.
+template <typename T, bool k16>
+__device__ __forceinline__ bool redo_row(const T *v, int64_t v_sl, const AttnMask &mk, int D, int n, int m, int p,
+                                         int lo, bool nan) {
+  const int first = window_lo(mk, n - m);
+  if (hidden_bad<T>(v, v_sl, D, p, n, first > mk.sinks ? first : mk.sinks, lo).meets(p, lo)) return true;
+  if (!k16 || !nan) return false;
+  const int s_end = mk.sinks < lo ? mk.sinks : lo, end = p + 1 > 0 ? p + 1 : 0;
+  return bad_row<T>(v, v_sl, D, 0, s_end < end ? s_end : end, 1, true, nullptr) >= 0 ||
+         bad_row<T>(v, v_sl, D, lo, end - lo, 1, true, nullptr) >= 0;
+}
+
+// Score of key row k (16 bytes at a time where rows start there).
+template <typename T>
+__device__ __forceinline__ float dot_row(const T *q, const T *k, int D, bool vec) {
+  constexpr int kVec = 16 / sizeof(T);
+  float s = 0.f;
+  if (vec) {
+#pragma unroll 4
+    for (int d = 0; d < D; d += kVec) {
+      const uint4 a = *reinterpret_cast<const uint4 *>(q + d), b = *reinterpret_cast<const uint4 *>(k + d);
+      const T *x = reinterpret_cast<const T *>(&a), *y = reinterpret_cast<const T *>(&b);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) s = fmaf(to_f32(x[i]), to_f32(y[i]), s);
+    }
+  } else {
+    for (int d = 0; d < D; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
+  }
+  return s;
+}
+
 // One query row, one warp, straight from the definition; keys that the row
-// does not see are not touched.  The tiled kernels multiply a masked weight 0
-// with the value row of its tile, which is wrong only where that row holds an
-// infinity or NaN: they find it by the non-finite result and redo the row
-// here.  D <= 256.
+// does not see are not touched.  D <= 256.  `tick`, where it is not null, is
+// counted up as the row proceeds, for those who wait for this warp with a limit.
 template <typename T>
 __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T *o, int64_t k_sl, int64_t v_sl, int D,
-                                           int p, int lo, int sinks, float scale_log2) {
+                                           int p, int lo, int sinks, float scale_log2, int *tick = nullptr) {
   const int lane = threadIdx.x & 31;
+  const bool vec = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | k_sl * sizeof(T) |
+                     D * sizeof(T)) & 15) == 0;
   float acc[8], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -75,11 +193,7 @@ __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T
     for (int j0 = first; j0 < end; j0 += 32) {
       const int j = j0 + lane;
       float s = -INFINITY;
-      if (j < end) {
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = fmaf(to_f32(q[d]), to_f32(k[j * k_sl + d]), s);
-        s *= scale_log2;
-      }
+      if (j < end) s = dot_row(q, k + j * k_sl, D, vec) * scale_log2;
       float mx = s;
 #pragma unroll
       for (int off = 16; off >= 1; off >>= 1) {
@@ -93,6 +207,7 @@ __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] *= corr;
       const int cnt = end - j0 < 32 ? end - j0 : 32;
+#pragma unroll 4
       for (int t = 0; t < cnt; ++t) {
         const float pt = __shfl_sync(0xffffffffu, pj, t);
         l += pt;
@@ -103,6 +218,7 @@ __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T
         }
       }
       m = m_new;
+      if (tick && lane == 0) atomicAdd(tick, 1);
     }
   }
 #pragma unroll

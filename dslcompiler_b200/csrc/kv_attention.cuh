@@ -990,7 +990,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int64_t o_at = row_at(P.o, b_now, hk, g, R);
-      bool bad = false;
+      bool bad = false, nan = false;
       for (int d = lane; d < D; d += 32) {
         float x = 0.f;
 #pragma unroll
@@ -998,6 +998,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
         if (whole) {
           x *= inv;
           bad |= !isfinite(x);
+          nan |= x != x;
           store_o(P.o.p, o_at + d, P.dtype, x);
         } else {
           A.part_o[(slot * 8 * NT + col) * D + d] = x;
@@ -1005,15 +1006,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
       }
       if (!whole && lane == 0) A.part_ml[slot * 8 * NT + col] = make_float2(ref, sum);
       if constexpr (!kQuant) {
-        // several queries: a value row of another query's range may hold an infinity or NaN
-        if (rg.m > 1 && __any_sync(0xffffffffu, bad)) {
+        // a value that the row does not see may be the cause (its own scores are not: see the sum)
+        if (sum == sum && __any_sync(0xffffffffu, bad)) {
           using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-          const int pos = rg.p_first + R / g;
-          __syncwarp();
-          attention_row<T>(static_cast<const T *>(P.q.p) + row_at(P.q, b_now, hk, g, R),
-                           reinterpret_cast<const T *>(kbase), reinterpret_cast<const T *>(vbase),
-                           static_cast<T *>(P.o.p) + o_at, P.k.sl, P.v.sl, D, pos, window_lo(P.mask, pos),
-                           P.mask.sinks, P.scale * kLog2e);
+          const int pos = rg.p_first + R / g, lo = window_lo(P.mask, pos);
+          const T *v = reinterpret_cast<const T *>(vbase);
+          if (redo_row<T, true>(v, P.v.sl, P.mask, D, rg.n, rg.m, pos, lo, __any_sync(0xffffffffu, nan))) {
+            __syncwarp();
+            attention_row<T>(static_cast<const T *>(P.q.p) + row_at(P.q, b_now, hk, g, R),
+                             reinterpret_cast<const T *>(kbase), v, static_cast<T *>(P.o.p) + o_at, P.k.sl, P.v.sl, D,
+                             pos, lo, P.mask.sinks, P.scale * kLog2e);
+          }
         }
       }
     }
@@ -1081,23 +1084,26 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t at = row_at(P.o, b, hk, g, R);
-  bool bad = false;
+  bool bad = false, nan = false;
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
     if (lane + 32 * i < D) {
       const float x = acc[i] * inv;
       bad |= !isfinite(x);
+      nan |= x != x;
       store_o(P.o.p, at + lane + 32 * i, P.dtype, x);
     }
   if constexpr (kDense) {
-    if (m > 1 && __any_sync(0xffffffffu, bad)) {
+    if (sum == sum && __any_sync(0xffffffffu, bad)) {
       using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-      const int pos = n - m + R / g;
-      __syncwarp();
-      attention_row<T>(static_cast<const T *>(P.q.p) + row_at(P.q, b, hk, g, R),
-                       static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh,
-                       static_cast<const T *>(P.v.p) + b * P.v.sb + hk * P.v.sh, static_cast<T *>(P.o.p) + at, P.k.sl,
-                       P.v.sl, D, pos, window_lo(P.mask, pos), P.mask.sinks, P.scale * kLog2e);
+      const int pos = n - m + R / g, lo = window_lo(P.mask, pos);
+      const T *v = static_cast<const T *>(P.v.p) + b * P.v.sb + hk * P.v.sh;
+      if (redo_row<T, true>(v, P.v.sl, P.mask, D, n, m, pos, lo, __any_sync(0xffffffffu, nan))) {
+        __syncwarp();
+        attention_row<T>(static_cast<const T *>(P.q.p) + row_at(P.q, b, hk, g, R),
+                         static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh, v, static_cast<T *>(P.o.p) + at,
+                         P.k.sl, P.v.sl, D, pos, lo, P.mask.sinks, P.scale * kLog2e);
+      }
     }
   }
 }

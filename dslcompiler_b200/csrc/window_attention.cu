@@ -312,6 +312,8 @@ __global__ void __launch_bounds__(Simt<T, DP>::kThreads, Simt<T, DP>::kCtas)
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  HiddenBad hidden = {-1, -1};
+  bool looked = false;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = q0 + row(i);
@@ -343,12 +345,20 @@ __global__ void __launch_bounds__(Simt<T, DP>::kThreads, Simt<T, DP>::kCtas)
         }
       }
     }
-    // rows i of the warp's two groups, redone by the whole warp
-    const unsigned any = __ballot_sync(0xffffffffu, bad);
+    // rows i of the warp's two groups, redone by the whole warp where a value
+    // that the row does not see may be the cause (not its own scores: see l)
+    const unsigned any = __ballot_sync(0xffffffffu, bad && l[i] == l[i]);
     if (any) {
+      if (!looked) {
+        // (the tile in which the window begins holds keys in front of it too)
+        const int front = w_first * kBK > sinks ? w_first * kBK : sinks;
+        hidden = hidden_bad<T>(vb, P.v.sl, D, w0, hi, front, window_lo(P.mask, w1));
+        looked = true;
+      }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        if (any & (g ? 0xffff0000u : 0x0000ffffu)) {
+        const int at = p0 + row(i) - ty + g;
+        if ((any & (g ? 0xffff0000u : 0x0000ffffu)) && hidden.meets(at, window_lo(P.mask, at))) {
           const int rr = r - ty + g, pos = n - m_rows + rr;
           __syncwarp();
           attention_row<T>(qb + rr * P.q.sl, kb, vb, ob + rr * P.o.sl, P.k.sl, P.v.sl, D, pos, window_lo(P.mask, pos),

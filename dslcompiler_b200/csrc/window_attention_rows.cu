@@ -66,10 +66,11 @@ __device__ __forceinline__ Row row_of(const AttnProblem &P, int b, int hk, int a
   return w;
 }
 
-// Writes one row from its sums x over all shares (lane: columns lane + 32 i);
-// a row that is not finite is redone key by key.
+// Writes one row, of a sequence of n keys and m queries, from its sums x over all
+// shares (lane: columns lane + 32 i); one that a value it does not see may have
+// made non-finite is redone key by key.
 template <int DP>
-__device__ __forceinline__ void write_row(const AttnProblem &P, int b, int hk, const Row &w,
+__device__ __forceinline__ void write_row(const AttnProblem &P, int b, int hk, int n, int m, const Row &w,
                                           const float (&x)[DP / 32], float l) {
   const int lane = threadIdx.x & 31;
   float *o = static_cast<float *>(P.o.p) + w.o;
@@ -83,12 +84,15 @@ __device__ __forceinline__ void write_row(const AttnProblem &P, int b, int hk, c
       bad |= !isfinite(x[i] * inv);
     }
   }
-  if (__any_sync(0xffffffffu, bad)) {
-    __syncwarp();
-    attention_row<float>(static_cast<const float *>(P.q.p) + w.q,
-                         static_cast<const float *>(P.k.p) + b * P.k.sb + hk * P.k.sh,
-                         static_cast<const float *>(P.v.p) + b * P.v.sb + hk * P.v.sh, o, P.k.sl, P.v.sl, P.D, w.pos,
-                         window_lo(P.mask, w.pos), P.mask.sinks, P.scale * kLog2e);
+  if (l == l && __any_sync(0xffffffffu, bad)) {
+    const float *v = static_cast<const float *>(P.v.p) + b * P.v.sb + hk * P.v.sh;
+    const int lo = window_lo(P.mask, w.pos);
+    if (redo_row<float, false>(v, P.v.sl, P.mask, P.D, n, m, w.pos, lo, false)) {
+      __syncwarp();
+      attention_row<float>(static_cast<const float *>(P.q.p) + w.q,
+                           static_cast<const float *>(P.k.p) + b * P.k.sb + hk * P.k.sh, v, o, P.k.sl, P.v.sl, P.D,
+                           w.pos, lo, P.mask.sinks, P.scale * kLog2e);
+    }
   }
 }
 
@@ -266,7 +270,7 @@ __global__ void __launch_bounds__(32 * Geo<DP, R>::kWarps, Geo<DP, R>::kCtas) ro
       for (int c = 0; c < DP / 32; ++c) x[c] = fmaf(f, part[r * DP + lane + 32 * c], x[c]);
     }
     if (A.splits == 1) {
-      write_row<DP>(P, b, hk, w, x, sum);
+      write_row<DP>(P, b, hk, n, m, w, x, sum);
     } else {
       const int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + r;
       if (lane == 0) A.part_ml[at] = make_float2(top, sum);
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(32 * R) combine_kernel(const Params A) {
     for (int c = 0; c < DP / 32; ++c) x[c] = fmaf(f, A.part_o[(at + s * kRows) * DP + lane + 32 * c], x[c]);
   }
   // (a share whose scores are all NaN keeps the maximum -inf, but 0 * NaN is NaN)
-  write_row<DP>(P, b, hk, w, x, sum);
+  write_row<DP>(P, b, hk, n, m, w, x, sum);
 }
 
 template <int DP, int R>

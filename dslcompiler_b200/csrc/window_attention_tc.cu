@@ -41,9 +41,6 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
-#include <algorithm>
-#include <atomic>
-
 #include "attn_common.cuh"
 
 namespace llk_b200 {
@@ -52,7 +49,7 @@ namespace {
 
 constexpr int kBM = 128;                // rows of a query tile
 constexpr int kThreads = 352;
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;
 // The reference m may lag a row's maximum by up to this power of two before O
 // is rescaled: P stays below 2^8, far inside f16, its relative rounding is
 // the same, and the f32 sums do not mind.
@@ -86,7 +83,33 @@ struct Tail {
   uint64_t q_full[2], q_empty[2], o_free[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], landed, mma_done;
   uint32_t tmem;
   int abort;
+  int tick;  // counts on while a warp redoes rows
 };
+
+// mbar_wait_bounded, for waits on warps that may be redoing rows: it gives up
+// after one to two limits without any progress there.  (A row of 2^20 keys takes
+// a warp some tens of milliseconds, and it may have 32 of them.)
+__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, Tail *st) {
+  volatile int *abort = &st->abort, *tick = &st->tick;
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = global_timer_ns();
+  int seen = -1;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0) {
+      if (*abort != 0) return false;
+      if (global_timer_ns() - t0 > kWaitLimitNs) {
+        const int now = *tick;
+        if (now == seen) {
+          *abort = LLK_ERR_TIMEOUT;
+          return false;
+        }
+        seen = now;
+        t0 = global_timer_ns();
+      }
+    }
+  }
+}
 
 __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
   uint64_t r;
@@ -189,6 +212,43 @@ struct Ring {
   }
 };
 
+// A warp's rows that are not finite (bad: this lane's, written already, at
+// position pos): those that a value they do not see may have made so are redone
+// from the definition.
+template <typename T>
+__device__ __noinline__ void redo_rows(const AttnProblem &P, bool bad, int b, int h, int row, int pos, int *tick) {
+  const int lane = threadIdx.x & 31, hk = h / (P.H / P.Hkv), sinks = P.mask.sinks;
+  const T *v = static_cast<const T *>(P.v.p) + b * P.v.sb + hk * P.v.sh;
+  T *o = static_cast<T *>(P.o.p) + b * P.o.sb + h * P.o.sh;
+  // the keys that the CTA sweeps for these rows, as in the kernel's plan
+  int n, m;
+  seq_lens(P.mask, b, n, m);
+  const int q0 = row & ~(2 * kBM - 1), p0 = n - m + q0, hi = p0 + (m - q0 < 2 * kBM ? m - q0 : 2 * kBM);
+  const int lo = window_lo(P.mask, p0), s_keys = sinks < lo ? sinks : lo;
+  const int warp_last = pos - lane + 31 < hi - 1 ? pos - lane + 31 : hi - 1;
+  const HiddenBad hidden = hidden_bad<T>(v, P.v.sl, P.D, pos - lane, hi, lo > sinks ? lo : sinks,
+                                         window_lo(P.mask, warp_last), tick);
+  bool again = bad && hidden.meets(pos, window_lo(P.mask, pos));
+  if constexpr (std::is_same<T, __half>::value) {
+    // a weight below f16's least times an infinity that the row does see: NaN here, not by the definition
+    bool nan = false;
+    if (bad && !again)
+      for (int d = 0; d < P.D; ++d) nan |= __hisnan(o[row * P.o.sl + d]);
+    if (__any_sync(0xffffffffu, nan)) {
+      const bool some = bad_row<T>(v, P.v.sl, P.D, 0, s_keys, 1, true, tick) >= 0 ||
+                        bad_row<T>(v, P.v.sl, P.D, lo, hi - lo, 1, true, tick) >= 0;
+      again |= nan && some;
+    }
+  }
+  for (unsigned todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
+    const int r = __ffs(todo) - 1 - lane;
+    __syncwarp();
+    attention_row<T>(static_cast<const T *>(P.q.p) + b * P.q.sb + h * P.q.sh + (row + r) * P.q.sl,
+                     static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh, v, o + (row + r) * P.o.sl, P.k.sl,
+                     P.v.sl, P.D, pos + r, window_lo(P.mask, pos + r), sinks, P.scale * kLog2e, tick);
+  }
+}
+
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
     window_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs A) {
@@ -217,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&st->landed, 1);
     mbar_init(&st->mma_done, 2);
     st->abort = 0;
+    st->tick = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.k);
@@ -232,7 +293,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t tmem = st->tmem;
-  volatile int *abort = &st->abort;
 
   // This CTA's blocks of rows: the last ones of the sequences, which have the
   // most keys, first, and every other round of them in reverse.
@@ -286,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int issued = 0;
     uint32_t landings = 0, queries[2] = {0, 0};
     auto wait = [&](uint64_t *bar, uint32_t phase) {
-      const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+      const bool r = wait_bounded(bar, phase & 1, st);
       return static_cast<bool>(__all_sync(0xffffffffu, r));
     };
     for (int round = 0; ok && item_of(round) < items; ++round) {
@@ -376,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       Ring<ST> ring;
       auto wait = [&](uint64_t *bar, uint32_t phase) {
-        if (!mbar_try_wait(bar, phase & 1)) ok = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+        if (!mbar_try_wait(bar, phase & 1)) ok = wait_bounded(bar, phase & 1, st);
         tc_fence_after();
         return ok;
       };
@@ -447,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       const bool r = mbar_try_wait(bar, phase & 1) ||
-                     mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
+                     wait_bounded(bar, phase & 1, st);
       ok = __all_sync(0xffffffffu, r);
       tc_fence_after();
       return ok;
@@ -455,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int round = 0; ok && item_of(round) < items; ++round) {
       const Sweep w = plan(item_of(round));
       if (w.rows <= kBM * t) continue;  // no query of this tile: nothing is written
-      const int n = w.tiles, hk = w.h / g;
+      const int n = w.tiles;
       const int row = w.q0 + kBM * t + row_in, pos = w.p0 + kBM * t + row_in;
       const int row_lo = window_lo(P.mask, pos);
       const int first = w.p0 + kBM * t;  // of the tile's rows that exist, the first and the last position
@@ -587,20 +647,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // a non-finite row: redone from the definition, by the whole warp
-      unsigned todo = __ballot_sync(0xffffffffu, mine && bad);
-      while (todo) {
-        const int r = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const int rr = row - lane + r, pp = pos - lane + r;
-        __syncwarp();
-        attention_row<T>(
-            static_cast<const T *>(P.q.p) + w.b * P.q.sb + w.h * P.q.sh + static_cast<int64_t>(rr) * P.q.sl,
-            static_cast<const T *>(P.k.p) + w.b * P.k.sb + hk * P.k.sh,
-            static_cast<const T *>(P.v.p) + w.b * P.v.sb + hk * P.v.sh,
-            static_cast<T *>(P.o.p) + w.b * P.o.sb + w.h * P.o.sh + static_cast<int64_t>(rr) * P.o.sl, P.k.sl, P.v.sl,
-            P.D, pp, window_lo(P.mask, pp), w.sinks, sc);
-      }
+      // (where its own scores are not finite, which l shows, it is right)
+      if (__any_sync(0xffffffffu, mine && bad && l == l))
+        redo_rows<T>(P, mine && bad && l == l, w.b, w.h, row, pos, &st->tick);
     }
   }
   tc_fence_before();
