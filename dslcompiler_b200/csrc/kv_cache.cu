@@ -38,6 +38,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kCtas = 4;              // resident on an SM: 64 registers
 constexpr int kMaxTokens = 64;        // tokens of a writer's CTA
+// Tokens of a writer's launch: the look for repeated slots is 7 of 74 us there
+// (8 heads of 128), what splitting further would save goes into more launches.
+constexpr int64_t kMaxLaunch = 32768;
 constexpr int kBitmapWords = 1024;    // 32768 bits over the low bits of the CTA's slots, as many over a hash
 constexpr float kLargest = 65504.f;
 constexpr double kLeastScale = 0x1p-30;
@@ -355,7 +358,7 @@ struct Move {
   KvPool pool;
   View4 k, v;
   const int64_t *slots;
-  uint32_t n_tokens, L;  // B L, L
+  uint32_t first, n_tokens, L;  // the launch's tokens [first, n_tokens) of the call's B L; L
   int tokens;            // of a CTA
   int pairs;             // (tensor, head) pairs of a CTA
   int step_pairs, step_tokens;  // rows of a round of the CTA: whole pairs and what is left
@@ -389,16 +392,19 @@ __device__ __forceinline__ Place place(const Move &A, uint32_t n) {
 // through all later tokens' slots (two bitmaps over its own slots rule nearly
 // all of them out: one alone lets a token through for each of the CTA's when
 // the call has 2^15, and each costs a loop over the CTA's slots) and leaves out its tokens that a later one overwrites, so a
-// slot holds its last token whatever order the CTAs run in.
+// slot holds its last token whatever order the CTAs run in.  That look grows
+// with the square of the tokens, so a launch takes kMaxLaunch of them at most,
+// and the launches of a longer call follow one another: a later one overwrites.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_constant__ Move A) {
   __shared__ Place at[kMaxTokens];
   __shared__ int64_t slot[kMaxTokens];
   __shared__ uint32_t bitmap[2 * kBitmapWords];
   const KvPool &P = A.pool;
-  const uint32_t n0 = blockIdx.x * A.tokens, n_tokens = A.n_tokens;
+  const uint32_t n0 = A.first + blockIdx.x * A.tokens, n_tokens = A.n_tokens;
+  const bool several = n_tokens - A.first > 1;
   const int cnt = n_tokens - n0 < static_cast<uint32_t>(A.tokens) ? static_cast<int>(n_tokens - n0) : A.tokens;
-  if (n_tokens > 1)
+  if (several)
     for (int i = threadIdx.x; i < 2 * kBitmapWords; i += kThreads) bitmap[i] = 0;
   __syncthreads();
   pdl_wait();
@@ -408,14 +414,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_
     const int64_t s = p.row >= 0 ? A.slots[n0 + threadIdx.x] : -1;
     at[threadIdx.x] = p;
     slot[threadIdx.x] = s;
-    if (s >= 0 && n_tokens > 1) {
+    if (s >= 0 && several) {
       const uint32_t hash = slot_hash(static_cast<uint32_t>(s));
       atomicOr(&bitmap[(s >> 5) & (kBitmapWords - 1)], 1u << (s & 31));
       atomicOr(&bitmap[kBitmapWords + (hash >> 5)], 1u << (hash & 31));
     }
   }
   __syncthreads();
-  if (n_tokens > 1) {
+  if (several) {
     // A slot's low word decides for nearly all.
     auto look = [&](uint32_t n, uint32_t s) {
       if (!(bitmap[(s >> 5) & (kBitmapWords - 1)] >> (s & 31) & 1)) return;
@@ -617,7 +623,6 @@ cudaError_t move_t(bool write, const KvPool &p, const View4 &k, const View4 &v, 
   a.k = k;
   a.v = v;
   a.slots = slots;
-  a.n_tokens = static_cast<uint32_t>(B * L);
   a.L = static_cast<uint32_t>(L);
   a.vec = rows_on_16_bytes(k, sizeof(T)) && rows_on_16_bytes(v, sizeof(T));
   a.page_shift = -1;
@@ -629,7 +634,8 @@ cudaError_t move_t(bool write, const KvPool &p, const View4 &k, const View4 &v, 
   // time.  The least of an SM's CTAs x a CTA's cost, in the units of an
   // instruction of all its warps, as measured: 500 for a round of 16 elements
   // a lane, 0.1 for a slot looked through, 600 to begin with.
-  const int64_t n = B * L;
+  const int64_t all = B * L, launches = write ? (all + kMaxLaunch - 1) / kMaxLaunch : 1;
+  const int64_t n = (all + launches - 1) / launches;  // tokens of a launch
   const int lpr = p.D / kN;
   int ysplit = 1;
   double least = 0;
@@ -655,15 +661,21 @@ cudaError_t move_t(bool write, const KvPool &p, const View4 &k, const View4 &v, 
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>((n + a.tokens - 1) / a.tokens), static_cast<unsigned>(ysplit));
+  cfg.gridDim.y = static_cast<unsigned>(ysplit);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e =
-      write ? cudaLaunchKernelEx(&cfg, p.bits == 4 ? kv_write_kernel<T, 4> : kv_write_kernel<T, 8>, a)
-            : cudaLaunchKernelEx(&cfg, p.bits == 4 ? kv_read_kernel<T, 4> : kv_read_kernel<T, 8>, a);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  for (int64_t first = 0; first < all; first += n) {
+    a.first = static_cast<uint32_t>(first);
+    a.n_tokens = static_cast<uint32_t>(first + n < all ? first + n : all);
+    cfg.gridDim.x = (a.n_tokens - a.first + a.tokens - 1) / a.tokens;
+    const cudaError_t e =
+        write ? cudaLaunchKernelEx(&cfg, p.bits == 4 ? kv_write_kernel<T, 4> : kv_write_kernel<T, 8>, a)
+              : cudaLaunchKernelEx(&cfg, p.bits == 4 ? kv_read_kernel<T, 4> : kv_read_kernel<T, 8>, a);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaGetLastError();
 }
 
 cudaError_t move(bool write, const KvPool &p, const View4 &k, const View4 &v, int dtype, int64_t B, int64_t L,
