@@ -545,7 +545,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
 #pragma unroll 1
     for (int i = 0; i < kRows; ++i) {
       const int row = warp + kWarps * i;
-      float x[kPairs][2], up = 1.f;
+      float x[kPairs][2];
+      int k2 = 0;
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
         uint32_t w = qraw[0][k];
@@ -567,8 +568,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
         for (int k = 0; k < kPairs; ++k) top = fmaxf(top, fmaxf(fabsf(x[k][0]), fabsf(x[k][1])));
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // floor(log2 top)
-        const int k2 = top > 0.f && ex < 128 ? 9 - ex : 0;
-        up = k2 > 126 ? 0x1p126f : __uint_as_float(static_cast<uint32_t>(127 + (k2 < -126 ? -126 : k2)) << 23);
+        k2 = top > 0.f && ex < 128 ? 9 - ex : 0;  // -118 at least
+        k2 = k2 > 126 ? 126 : k2;
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + k2) << 23);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {
           x[k][0] *= up;
@@ -586,7 +588,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
           if (lane == 0) qsum[row][gi] = sum * 0x1p-24f;
         }
       }
-      if (lane == 0) qfac[row] = P.scale * kLog2e * (kQuant ? 0x1p24f / up : 1.f);
+      if constexpr (kQuant) {
+        // (the largest bf16 queries, from 2^113 on: a factor that is finite still tells their scores apart)
+        const float f = scalbnf(P.scale * kLog2e, 24 - k2);
+        if (lane == 0) qfac[row] = fminf(fmaxf(f, -0x1.fffffep127f), 0x1.fffffep127f);
+      } else if (lane == 0) {
+        qfac[row] = P.scale * kLog2e;
+      }
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
         const int e = 2 * (lane + 32 * k);  // even, so e and e + 1 lie in one word

@@ -227,10 +227,9 @@ int llk_window_attention_scratch(const llk_tensor4d *q, const llk_tensor4d *k, i
  *                      (4 bits: element 2j in the low nibble of byte j);
  *   k_params, v_params [num_pages, kv_heads, page_size, head_dim / group_size]
  *                      pairs (scale, min) of bf16, scale first.
- * An element stands for scale * code + min, whatever the (finite) scale:
- * zeros, as in slots that were never written, and negative ones too.
- * head_dim 64, 128 or 256; bits 4
- * or 8; group_size 32, 64 or 128, dividing head_dim; page_size a multiple of
+ * An element stands for scale * code + min, of either sign and zero (as in
+ * slots that were never written), up to 2^60 in magnitude.  head_dim 64, 128
+ * or 256; bits 4 or 8; group_size 32, 64 or 128, dividing head_dim; page_size a multiple of
  * 16; all four pointers 16-byte aligned.  Token t of a sequence lies in page
  * block_table[b][t / page_size] at offset t % page_size; slot number = page *
  * page_size + offset. */

@@ -139,3 +139,23 @@ def test_zero_scales_in_a_long_context():
     dense = llk.window_attention(q.float(), k, v, kv_lens=lens)
     got = cache.attention(q, table, lens)
     assert ((got.float() - dense).abs() <= 2.0**-7 * dense.abs() + 2.0**-10 * v.abs().amax()).all()
+
+
+@pytest.mark.parametrize("bits,D,group,page", [(4, 64, 32, 16), (4, 128, 128, 64), (8, 256, 64, 16)])
+def test_queries_of_any_magnitude(bits, D, group, page):
+    """From the least to the largest bf16: with a scale to match, an ordinary result; with the usual one, the largest
+    score takes all."""
+    B, Hkv, g, L = 1, 2, 3, 90
+    cache, table, gen = pool(B, Hkv, L, D, bits, group, page, D)
+    q = torch.randn((B, g * Hkv, 2, D), generator=gen).to(BF16)
+    for e in (-120, -60, 60, 100):
+        check(cache, table, (q * 2.0**e).cuda(), [L], L, scale=D**-0.5 * 2.0**-e)
+    k, v, slack = held(cache, table, L)
+    for e in (40, 100, 112, 115, 119):
+        big = (q * 2.0**e).to(BF16)
+        got = cache.attention(big.cuda(), table, ints([L])).cpu().double()
+        s = big.double() @ k.repeat_interleave(g, 1).transpose(2, 3)
+        s.masked_fill_(~ref.visible(2, L, L, 2, 0, 0), -float("inf"))
+        want = torch.gather(v.repeat_interleave(g, 1), 2, s.argmax(-1, keepdim=True).expand(-1, -1, -1, D))
+        a = torch.gather(slack.repeat_interleave(g, 1), 2, s.argmax(-1, keepdim=True).expand(-1, -1, -1, D))
+        assert ((got - want).abs() <= ref.HALF_STEP[BF16] * want.abs() + (2.0**-11 + L * 2.0**-22) * a).all(), e
