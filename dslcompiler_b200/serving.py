@@ -71,10 +71,12 @@ def _check_ints(what, t, dtype, shape):
 
 
 def _ranges(window, sinks):
-    window, sinks = int(window or 0), int(sinks)
-    if window < 0 or sinks < 0:
+    w, s = int(window or 0), int(sinks)
+    if w != (window or 0) or s != sinks:  # (a fraction would be cut to another window)
+        raise ValueError("window and sinks must be whole numbers")
+    if w < 0 or s < 0:
         raise ValueError("window and sinks must not be negative")
-    return min(window, 2**62), min(sinks, 2**62)
+    return min(w, 2**62), min(s, 2**62)
 
 
 def _made_on(stream, device, make):

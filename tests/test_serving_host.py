@@ -39,3 +39,14 @@ def test_what_a_call_makes_is_made_on_its_stream(monkeypatch):
     seen = []
     serving._made_on(s, q.device, lambda: seen.append(current[-1]))
     assert seen == [s] and current == ["torch's"]
+
+
+def test_window_and_sinks_are_whole_numbers():
+    assert serving._ranges(None, 0) == (0, 0)
+    assert serving._ranges(7, 3) == (7, 3)
+    assert serving._ranges(torch.tensor(7), True) == (7, 1)
+    assert serving._ranges(2**70, 2**70) == (2**62, 2**62)
+    assert serving._ranges(100.0, 2.0) == (100, 2)
+    for window, sinks in ((-1, 0), (0, -1), (0.5, 0), (99.9, 0), (4, 1.5), ("4", 0)):
+        with pytest.raises(ValueError):
+            serving._ranges(window, sinks)
