@@ -14,7 +14,7 @@ import numpy as np
 
 from . import capi
 from .capi import check, lib
-from .swiglu import _device_of, _is_torch, _stream_of, gpu_context
+from .swiglu import _device_of, _is_torch, _out_on, _stream_of, gpu_context
 
 try:
     import torch
@@ -42,10 +42,11 @@ def _check(t, dtype_torch, dtype_np, what):
         raise TypeError(f"{what} must be a {np.dtype(dtype_np).name} array")
 
 
-def _like(t, shape=None):
+def _like(t, zeros, stream):
     if _is_torch(t):
-        return torch.empty(shape or t.shape, dtype=t.dtype, device=t.device)
-    return np.empty(shape or t.shape, t.dtype)
+        make = torch.zeros if zeros else torch.empty
+        return _out_on(stream if t.is_cuda else None, t.device, lambda: make(t.shape, dtype=t.dtype, device=t.device))
+    return (np.zeros if zeros else np.empty)(t.shape, t.dtype)
 
 
 def rope(x, position_ids, *, theta: float = 10000.0, out=None, math_mode: str = "strict", stream=None,
@@ -60,7 +61,7 @@ def rope(x, position_ids, *, theta: float = 10000.0, out=None, math_mode: str = 
     if tuple(position_ids.shape) != (L,):
         raise ValueError(f"position_ids must be [{L}]")
     if out is None:
-        out = _like(x)
+        out = _like(x, False, stream)
     g = gpu_context(_device_of(x, device), _stream_of(x, stream), math_mode=math_mode)
     check(lib().llk_rope(_ptr(x), _ptr(position_ids), _ptr(out), B, H, L, D, float(theta), ctypes.byref(g)),
           "llk_rope")
@@ -84,7 +85,7 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, out=
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if _is_torch(q) else np.zeros(q.shape, np.float32)
+        out = _like(q, True, stream)
     g = gpu_context(_device_of(q, device), _stream_of(q, stream), math_mode=math_mode)
     check(lib().llk_attention(_ptr(q), _ptr(k), _ptr(v), _ptr(out), B, H, Lq, Lk, D, float(scale), int(bool(causal)),
                               ctypes.byref(g)), "llk_attention")

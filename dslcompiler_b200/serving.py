@@ -17,7 +17,7 @@ import threading
 
 from . import capi
 from .capi import KernelContext, KvCache, Tensor4D, check, lib
-from .swiglu import _is_torch, _stream_of, gpu_context
+from .swiglu import _is_torch, _made_on, _out_on, _stream_of, gpu_context
 
 try:
     import torch
@@ -79,29 +79,9 @@ def _ranges(window, sinks):
     return min(w, 2**62), min(s, 2**62)
 
 
-def _made_on(stream, device, make):
-    """make()'s tensor, taken from the allocator and filled on the stream that the call runs on: nothing orders work
-    queued on torch's current stream (a fill, or the last use of a block that the allocator hands out again) before a
-    kernel on another one."""
-    if stream is None:
-        return make()
-    s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device)
-    with torch.cuda.stream(s):
-        return make()
-
-
-def _new_out(make, device, stream):
-    """An output that the caller gets: it may be used on the current stream too, so its memory is handed out again
-    only behind the work queued there by then."""
-    out = _made_on(stream, device, make)
-    if stream is not None:
-        out.record_stream(torch.cuda.current_stream(device))
-    return out
-
-
 def _out_like(q, q_lens, stream):
     # rows behind a sequence's queries are not written: they read as zeros
-    return _new_out(lambda: torch.empty_like(q) if q_lens is None else torch.zeros_like(q), q.device, stream)
+    return _out_on(stream, q.device, lambda: torch.empty_like(q) if q_lens is None else torch.zeros_like(q))
 
 
 def _scratch(nbytes, like, stream):
@@ -237,7 +217,7 @@ class QuantizedKVCache:
                 raise TypeError(f"dtype must be one of {', '.join(str(d) for d in _DTYPES)}")
             # (on the cache's device, where the slots have to be too)
             shape = (2, slots.shape[0], self.kv_heads, slots.shape[1], self.head_dim)
-            k, v = _new_out(lambda: self.k_params.new_empty(shape, dtype=dtype), self.device, stream).unbind(0)
+            k, v = _out_on(stream, self.device, lambda: self.k_params.new_empty(shape, dtype=dtype)).unbind(0)
         else:
             k, v = out
             if dtype is not None and k.dtype != dtype:

@@ -62,6 +62,26 @@ def _current_raw_stream(index):
     return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
+def _made_on(stream, device, make):
+    """make()'s tensor, taken from the allocator and filled on the stream that the call runs on: nothing orders work
+    queued on torch's current stream (a fill, or the last use of a block that the allocator hands out again) before a
+    kernel on another one."""
+    if stream is None:
+        return make()
+    s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=device)
+    with torch.cuda.stream(s):
+        return make()
+
+
+def _out_on(stream, device, make):
+    """An output that the caller gets: it may be used on the current stream too, so its memory is handed out again
+    only behind the work queued there by then."""
+    out = _made_on(stream, device, make)
+    if stream is not None:
+        out.record_stream(torch.cuda.current_stream(device))
+    return out
+
+
 def _device_of(t, device):
     if device is not None:
         return int(device)
@@ -95,10 +115,11 @@ def _check_bf16(*ts):
                 raise TypeError("numpy operands must hold bf16 bit patterns (uint16)")
 
 
-def _new_out(like, rows, cols, f32: bool):
+def _new_out(like, rows, cols, f32: bool, stream=None):
     if _is_torch(like):
         dt = torch.float32 if f32 else torch.bfloat16
-        return torch.empty((rows, cols), dtype=dt, device=like.device)
+        return _out_on(stream if like.is_cuda else None, like.device,
+                       lambda: torch.empty((rows, cols), dtype=dt, device=like.device))
     return np.empty((rows, cols), np.float32 if f32 else np.uint16)
 
 
@@ -111,7 +132,7 @@ def fused_swiglu(x, wg, wu, *, out=None, out_dtype: str = "bf16", variant: str =
     _check_bf16(x, wg, wu)
     f32 = out_dtype in ("f32", "fp32", "float32")
     if out is None:
-        out = _new_out(x, x.shape[0], wg.shape[1], f32)
+        out = _new_out(x, x.shape[0], wg.shape[1], f32, stream)
     tx, tg, tu, ty = tensor2d(x), tensor2d(wg), tensor2d(wu), tensor2d(out)
     ctx = None  # no scratch: the library's own workspace
     if scratch is not None:
@@ -130,7 +151,7 @@ def matmul(a, b, c=None, *, accumulate: bool = False, variant: str = "auto", str
     if c is None:
         if accumulate:
             raise ValueError("accumulate=True needs c")
-        c = _new_out(a, a.shape[0], b.shape[1], True)
+        c = _new_out(a, a.shape[0], b.shape[1], True, stream)
     ta, tb, tc = tensor2d(a), tensor2d(b), tensor2d(c)
     g = gpu_context(_device_of(a, device), _stream_of(a, stream), capi.LLK_DTYPE_FP32, variant)
     check(lib().llk_matmul(ctypes.byref(ta), ctypes.byref(tb), ctypes.byref(tc), int(accumulate), None,
@@ -212,7 +233,7 @@ class PackedWeights:
         _check_bf16(x)
         f32 = out_dtype in ("f32", "fp32", "float32")
         if out is None:
-            out = _new_out(x, x.shape[0], self.N, f32)
+            out = _new_out(x, x.shape[0], self.N, f32, stream)
         tx, ty = tensor2d(x), tensor2d(out)
         g = gpu_context(-1, _stream_of(x, stream), capi.LLK_DTYPE_FP32 if f32 else capi.LLK_DTYPE_BF16, variant,
                         math_mode)

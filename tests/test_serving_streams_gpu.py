@@ -129,3 +129,33 @@ def test_a_result_given_back_early_waits_for_the_current_stream():
         torch.cuda.synchronize()
         assert torch.equal(copy, want)
         del others
+
+
+def test_other_operators_results_stand_when_the_current_stream_is_late():
+    """llk.rope, llk.attention (whose output starts from zeros), fused_swiglu, matmul, PackedWeights likewise."""
+    q, k, v = (rand(s, (1, 4, 96, 64)).float() for s in (1, 2, 3))
+    pos = torch.arange(96, device="cuda")
+    x, wg, wu = rand(4, (64, 128)), rand(5, (128, 256)), rand(6, (128, 256))
+    pw = llk.PackedWeights(wg, wu)
+    side = torch.cuda.Stream()
+    for name, call in (("attention", lambda s: llk.attention(q, k, v, causal=True, stream=s)),
+                       ("rope", lambda s: llk.rope(q, pos, stream=s)),
+                       ("swiglu", lambda s: llk.fused_swiglu(x, wg, wu, stream=s)),
+                       ("matmul", lambda s: llk.matmul(x, wg, stream=s)),
+                       ("packed", lambda s: pw(x, stream=s))):
+        want = call(None)
+        torch.cuda.synchronize()
+        blocks = [torch.full_like(want, i + 1.0) for i in range(4)]
+        copies = [torch.zeros_like(want) for _ in blocks]
+        torch.cuda.synchronize()
+        torch.cuda._sleep(BUSY)
+        for c, b in zip(copies, blocks):
+            c.copy_(b)
+        del blocks, b
+        got = call(side)
+        with torch.cuda.stream(side):
+            early = got.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(early, want) and torch.equal(got, want), name
+        for i, c in enumerate(copies):
+            assert (c == i + 1.0).all(), (name, i)
