@@ -458,65 +458,50 @@ __global__ void __launch_bounds__(kThreads, kCtas) kv_write_kernel(const __grid_
   const int lpr = P.D / kN, l = threadIdx.x & (lpr - 1);  // lanes a row
   const int rows = A.tokens * A.pairs;
   const int gl = P.group / kN, groups = P.D / P.group;
-  constexpr int kU = 1;  // rows in flight a thread, and as many ahead
   const int step = kThreads / lpr, mine = threadIdx.x / lpr;
   // every lane runs every round (the group's shuffles take the whole warp);
-  // the next round's rows load while this one's are worked on
-  Piece<T> x[kU], ahead[kU];
-  int64_t row[kU], row_ahead[kU];
-  bool is_v[kU], is_v_ahead[kU];
+  // the next round's row loads while this one's is worked on
+  Piece<T> x, ahead;
+  int64_t row, row_ahead;
+  bool is_v, is_v_ahead;
   const int end_pair = (blockIdx.y + 1) * A.pairs;
   int next_pair = blockIdx.y * A.pairs + mine / A.tokens, next_t = mine % A.tokens;
-  auto next_row = [&]() {  // the thread's row of the next round
-    next_pair += A.step_pairs;
+  auto load = [&]() {
+    const int t = next_t, pair = next_pair;
+    is_v_ahead = pair >= P.Hkv;
+    const int h = is_v_ahead ? pair - P.Hkv : pair;
+    row_ahead = pair < end_pair && t < cnt ? at[t].row : -1;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(kN * sizeof(T) / 4); ++i) ahead.w[i] = 0;
+    if (row_ahead >= 0) {
+      const View4 &src = is_v_ahead ? A.v : A.k;
+      load_piece(static_cast<const T *>(src.p) + (is_v_ahead ? at[t].v : at[t].k) + h * src.sh + kN * l, A.vec, ahead);
+      row_ahead += static_cast<int64_t>(h) * P.page;
+    }
+    next_pair += A.step_pairs;  // the thread's row of the next round
     next_t += A.step_tokens;
     if (next_t >= A.tokens) {
       next_t -= A.tokens;
       ++next_pair;
     }
   };
-  auto load = [&]() {
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int t = next_t, pair = next_pair;
-      is_v_ahead[u] = pair >= P.Hkv;
-      const int h = is_v_ahead[u] ? pair - P.Hkv : pair;
-      row_ahead[u] = pair < end_pair && t < cnt ? at[t].row : -1;
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(kN * sizeof(T) / 4); ++i) ahead[u].w[i] = 0;
-      if (row_ahead[u] >= 0) {
-        const View4 &src = is_v_ahead[u] ? A.v : A.k;
-        load_piece(static_cast<const T *>(src.p) + (is_v_ahead[u] ? at[t].v : at[t].k) + h * src.sh + kN * l, A.vec,
-                   ahead[u]);
-        row_ahead[u] += static_cast<int64_t>(h) * P.page;
-      }
-      next_row();
-    }
-  };
   load();
-  for (int r0 = 0; r0 < rows; r0 += kU * step) {
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      x[u] = ahead[u];
-      row[u] = row_ahead[u];
-      is_v[u] = is_v_ahead[u];
+  for (int r0 = 0; r0 < rows; r0 += step) {
+    x = ahead;
+    row = row_ahead;
+    is_v = is_v_ahead;
+    if (r0 + step < rows) load();
+    uint32_t param, words[kN * BITS / 32];
+    quantise<T, BITS>(x, gl, words, &param);
+    if (row < 0) continue;
+    uint8_t *dst = static_cast<uint8_t *>(is_v ? P.v_codes : P.k_codes) + row * (P.D * BITS / 8) + kN * BITS / 8 * l;
+    if constexpr (BITS == 4) {
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(words[0], words[1]);
+    } else {
+      *reinterpret_cast<uint4 *>(dst) = make_uint4(words[0], words[1], words[2], words[3]);
     }
-    if (r0 + kU * step < rows) load();
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      uint32_t param, words[kN * BITS / 32];
-      quantise<T, BITS>(x[u], gl, words, &param);
-      if (row[u] < 0) continue;
-      uint8_t *dst =
-          static_cast<uint8_t *>(is_v[u] ? P.v_codes : P.k_codes) + row[u] * (P.D * BITS / 8) + kN * BITS / 8 * l;
-      if constexpr (BITS == 4) {
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(words[0], words[1]);
-      } else {
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(words[0], words[1], words[2], words[3]);
-      }
-      if ((l & (gl - 1)) == 0)
-        static_cast<uint32_t *>(is_v[u] ? P.v_params : P.k_params)[row[u] * groups + l / gl] = param;
-    }
+    if ((l & (gl - 1)) == 0)
+      static_cast<uint32_t *>(is_v ? P.v_params : P.k_params)[row * groups + l / gl] = param;
   }
 }
 
