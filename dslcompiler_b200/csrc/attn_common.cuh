@@ -39,6 +39,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// A mean of finite f16 values by weights that were rounded to 16 bits: not past
+// the largest f16, which rounding would make an infinity.
+__device__ __forceinline__ float within_f16(float x) {
+  return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+}
+
 // Keys n and queries m of sequence b, clamped to the tensors.
 __device__ __forceinline__ void seq_lens(const AttnMask &mk, int b, int &n, int &m) {
   n = mk.kv_lens ? mk.kv_lens[b] : mk.Lk;

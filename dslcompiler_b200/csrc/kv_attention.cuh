@@ -1007,6 +1007,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) split_kernel(const __grid_cons
           x *= inv;
           bad |= !isfinite(x);
           nan |= x != x;
+          if constexpr (!kQuant && !kBf16) x = within_f16(x);
           store_o(P.o.p, o_at + d, P.dtype, x);
         } else {
           A.part_o[(slot * 8 * NT + col) * D + d] = x;
@@ -1096,9 +1097,10 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
     if (lane + 32 * i < D) {
-      const float x = acc[i] * inv;
+      float x = acc[i] * inv;
       bad |= !isfinite(x);
       nan |= x != x;
+      if constexpr (kDense && !kBf16) x = within_f16(x);
       store_o(P.o.p, at + lane + 32 * i, P.dtype, x);
     }
   if constexpr (kDense) {

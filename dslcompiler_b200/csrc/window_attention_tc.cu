@@ -632,6 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 32; ++i) {
           y[i] = begun ? __uint_as_float(x[i]) * inv : 0.f;
           bad |= !(fabsf(y[i]) < INFINITY);
+          if constexpr (!kBf16) y[i] = within_f16(y[i]);
         }
         if (mine) {
           if (A.vec_o && c + 32 <= P.D) {

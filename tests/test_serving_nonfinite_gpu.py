@@ -141,3 +141,23 @@ def test_one_nan_does_not_make_a_prompt_slow(dtype, D):
         t = timed(lambda: llk.window_attention(q, k2, v2))
         print(f"{what} {dtype} D {D}: {plain:.3f} ms clean, {t:.3f} ms with one NaN")
         assert t < 5 * plain + 0.2, (what, t, plain)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,D,window,sinks", [(1, 8, 2, 700, 700, 64, 0, 0), (1, 8, 2, 600, 600, 128, 9, 2),
+                                                          (1, 4, 2, 300, 300, 256, 5, 0), (2, 8, 2, 3, 900, 128, 0, 0),
+                                                          (8, 8, 2, 1, 40, 64, 3, 0)])
+def test_values_at_the_largest_f16_stay_finite(B, H, Hkv, Lq, Lk, D, window, sinks):
+    """A weighted mean of finite values is finite: the weights' rounding does not push it over the type's largest."""
+    q, k = rand(1, (B, H, Lq, D), F16), rand(2, (B, Hkv, Lk, D), F16)
+    v = torch.full((B, Hkv, Lk, D), 65504.0, dtype=F16, device="cuda")
+    v[..., 1::2] *= -1
+    lens = torch.full((B,), Lk, dtype=torch.int32, device="cuda")
+    got = llk.window_attention(q, k, v, window=window, sinks=sinks, kv_lens=lens)
+    assert torch.isfinite(got).all()
+    # half a step of the result and of each weight
+    assert ((got.double().abs() - 65504).abs() <= 65504 * 2 * ref.HALF_STEP[F16]).all()
+    v[0, 0, Lk // 2, 0] = math.inf
+    got = llk.window_attention(q, k, v, window=window, sinks=sinks, kv_lens=lens)
+    see = ref.visible(Lq, Lk, Lk, Lq, window, sinks)[:, Lk // 2].cuda()
+    assert (got[0, :H // Hkv, see, 0] == math.inf).all()
+    assert torch.isfinite(got[0, :H // Hkv, ~see]).all() and torch.isfinite(got[0, H // Hkv:]).all()
