@@ -208,7 +208,8 @@ class QuantizedKVCache:
 
     def read(self, slots, *, dtype=None, out=None, stream=None):
         """(k, v) [B, kv_heads, L, head_dim] of the slots [B, L] in ``dtype`` (default bf16), or into the pair
-        ``out``.  A slot outside the cache reads as zeros."""
+        ``out``.  A slot outside the cache reads as zeros.  What was written within 2^-8 of +-65504, or saturated to
+        it, may stand for more than f16 holds (-65504 for -65536) and read as an infinity there; bf16 and f32 hold it."""
         if not _is_torch(slots) or slots.dim() != 2:
             raise TypeError("slots must be a torch.int64 CUDA tensor [B, L]")
         ps = _check_ints("slots", slots, torch.int64, tuple(slots.shape))

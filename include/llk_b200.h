@@ -250,7 +250,12 @@ int llk_kv_cache_write(const llk_kv_cache *cache, const llk_tensor4d *k, const l
                        const int64_t *slots, const llk_gpu_context *gpu);
 
 /* Reads slots [B, L] back into k, v [B, kv_heads, L, head_dim]; a slot
- * outside the cache reads as zeros. */
+ * outside the cache reads as zeros.  What an element stands for, scale * code +
+ * min, is rounded to dtype once.  By the roundings of min and scale it may lie
+ * a little outside what was written: where that came within 2^-8 of +-65504 (a
+ * -65504 or -infinity stands for -65536), FP16 reads it as an infinity.  Read
+ * such tokens as BF16 or FP32; llk_kv_cache_attention is not concerned, it
+ * works on them in f32. */
 int llk_kv_cache_read(const llk_kv_cache *cache, const llk_tensor4d *k, const llk_tensor4d *v, int dtype,
                       const int64_t *slots, const llk_gpu_context *gpu);
 

@@ -159,3 +159,20 @@ def test_queries_of_any_magnitude(bits, D, group, page):
         want = torch.gather(v.repeat_interleave(g, 1), 2, s.argmax(-1, keepdim=True).expand(-1, -1, -1, D))
         a = torch.gather(slack.repeat_interleave(g, 1), 2, s.argmax(-1, keepdim=True).expand(-1, -1, -1, D))
         assert ((got - want).abs() <= ref.HALF_STEP[BF16] * want.abs() + (2.0**-11 + L * 2.0**-22) * a).all(), e
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_tokens_at_the_ends_of_the_held_range(bits):
+    """Infinities and +-65504 are held as up to +-65536, which bf16 and f32 read back; attention works on that."""
+    B, Hkv, g, L, D = 1, 2, 3, 60, 64
+    cache, table, gen = pool(B, Hkv, L, D, bits, 32, 16, 1)
+    k, v = (torch.randn((B, Hkv, L, D), generator=gen) for _ in range(2))
+    v[:, :, 3], v[:, :, 9, ::2], v[:, :, 20, 5], v[:, :, 31] = -65504.0, float("inf"), -float("inf"), 65504.0
+    t = torch.arange(L, device="cuda")
+    slots = (table.long()[:, t // 16] * 16 + t % 16).contiguous()
+    cache.write(k.cuda(), v.cuda(), slots)
+    for dtype in (BF16, F32):
+        back = cache.read(slots, dtype=dtype)[1]
+        assert torch.isfinite(back).all() and (back.abs() <= 65536 + 256).all()
+        assert torch.equal(back.cpu(), held(cache, table, L)[1].float().to(dtype))
+    check(cache, table, torch.randn((B, Hkv * g, 2, D), generator=gen).to(BF16).cuda(), [L], L)
