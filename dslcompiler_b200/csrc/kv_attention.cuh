@@ -29,23 +29,24 @@
 // with s and m in f32 and p_t s_t rounded to f16, or to the sum of two f16
 // (kTwo) where the output is f16: one rounding moves values that are small
 // against s c and m, of which they are the difference, by more than the
-// output's own (measured: 5.0e-4 of the result for 2.1e-4).  The running reference of
-// the softmax is the maximum of score + log2(|s of v|), so p_t s_t is at most 1
-// whatever the scales are, and 11 bits of it are kept.
+// output's own (measured: 5.0e-4 of the result for 2.1e-4).  Over dense keys a
+// bf16 weight is the sum of two (one alone has 8 bits), an f16 weight one f16.
+// The running reference of the softmax is the maximum of score + log2(|s of v|),
+// so p_t s_t is at most 1 whatever the scales are, and 11 bits of it are kept.
 //
 // The work is dealt by cost, not by sequence: every CTA gets the same number
 // of units of 128 tokens (a begun segment counts two more), whatever lengths
 // the sequences have, and segments that two CTAs share are joined by a second
 // small kernel.
 //
-// Measured: 4 x 64 heads over 8, D = 128, 4 bits, 131072 tokens: 128 us, 4.4
-// TB/s of codes, scales and minima (0.67 of the measured HBM rate; unpacking
-// and the softmax keep the issue slots busy, and SMs differ by 20 %); 32
-// sequences of 4096: 34 us for 14.5, 9 of them what a call over one sequence
-// of 517 tokens takes (find the segment 1, first loads 2, queries 1, sums and
-// output 2.5, the joining kernel 3).  Dense bf16, 16 x 32 heads over 8, 4096
-// of 8192 tokens: 48 us, 0.85 of the HBM rate.  Shifting by mul.hi instead of
-// by the ALU took 135 for then 124 us.
+// Measured at 1965 MHz: 4 x 64 heads over 8, D = 128, 4 bits, 131072 tokens:
+// 127 us, 4.4 TB/s of codes, scales and minima (0.68 of the measured HBM rate:
+// an instruction issues in 57 % of the clocks, four warps a scheduler that wait
+// for fixed latencies and the ALU); 32 sequences of 4096: 34 to 35 us for 14.5,
+// 9 of them what a call over one sequence of 517 tokens takes (find the segment 1,
+// first loads 2, queries 1, sums and output 2.5, the joining kernel 3).  Dense
+// bf16, 16 x 32 heads over 8, 4096 of 8192 tokens: 47 us, 0.86 of the HBM rate.
+// Shifting by mul.hi instead of by the ALU took 135 for then 124 us.
 #pragma once
 
 #include <atomic>

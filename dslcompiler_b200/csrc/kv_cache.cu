@@ -9,9 +9,9 @@
 //
 // HBM-bound both ways; what there is to save is instructions.  A thread owns
 // 16 elements of a row, a row is D / 16 neighbouring lanes.  A CTA first works
-// out where its tokens lie, once for all heads.  Writing: the group's minimum and maximum are packed 16-bit
-// operations and shuffles of the pair (min, -max); the quotient (x - m) / s is
-// a product with 1 / s and one correction by its remainder, which makes it
+// out where its tokens lie, once for all heads.  Writing: the group's minimum
+// and maximum are packed 16-bit operations and shuffles of the pair (min, -max);
+// the quotient (x - m) / s is a product with 1 / s and one correction by its remainder, which makes it
 // exact wherever the quotient is a tie between two codes (the remainder is
 // exact, and so is the corrected quotient when it is representable), so
 // rounding to even by adding 1.5 * 2^23 settles the ties of 16-bit inputs;
@@ -21,11 +21,11 @@
 // masked into the mantissa of 2^23 where it lies, so that a subtraction makes
 // it code * 16^i, and one fused multiply-add with scale / 16^i the value.
 //
-// Measured, 4 x 8191 bf16 tokens of 8 heads, D = 128, 4 bits: write 74 us (7 of
-// them the look for repeated slots), read 34 us, each 170 MB, 26 us at the
-// measured HBM rate.  The write issues an instruction in 71 % of the clocks:
-// 420 of them a warp for 16 elements a lane.  32 tokens: 3.4 and 2.1 us, a
-// launch.  2000 f32 tokens of 32 heads, D = 64, 8 bits: 15 and 7 us.
+// Measured at 1965 MHz, 4 x 8191 bf16 tokens of 8 heads, D = 128, 4 bits: write
+// 78 us (7 of them the look for repeated slots), read 34 us, each 170 MB, 26 us
+// at the measured HBM rate.  The write issues an instruction in 70 % of the
+// clocks: 420 of them a warp for 16 elements a lane.  32 tokens: 3.2 and 2.2 us,
+// a launch.  2000 f32 tokens of 32 heads, D = 64, 8 bits: 16 and 8 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -38,7 +38,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kCtas = 4;              // resident on an SM: 64 registers
 constexpr int kMaxTokens = 64;        // tokens of a writer's CTA
-// Tokens of a writer's launch: the look for repeated slots is 7 of 74 us there
+// Tokens of a writer's launch: the look for repeated slots is 7 of 78 us there
 // (8 heads of 128), what splitting further would save goes into more launches.
 constexpr int64_t kMaxLaunch = 32768;
 constexpr int kBitmapWords = 1024;    // 32768 bits over the low bits of the CTA's slots, as many over a hash

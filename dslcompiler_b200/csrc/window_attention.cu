@@ -17,12 +17,12 @@
 // warps where DP = 256: R = 8 would need more than 255 registers.)  The
 // probabilities pass through the warp's own piece of shared memory.
 //
-// Measured (f32, D = 128): 32 heads, 1000 tokens, window 333: 156 us for 61 at
-// the nominal FMA rate, 1.45 times the pairs being computed where tiles are
-// cut by the window's ends; 4096 tokens without a window 2.93 ms, 0.64 of the
-// rate (the FMA pipe works 54 % of the clocks at 8 warps an SM, stalls are
-// fixed latencies and the pipe itself).  One CTA of 256 threads with 4 x 4
-// scores a thread took 204 us.
+// Measured (f32, D = 128, 1965 MHz): 32 heads, 1000 tokens, window 333: 156 us
+// for 61 at the nominal FMA rate, 1.45 times the pairs being computed where
+// tiles are cut by the window's ends (the FMA pipe works 58 % of the clocks at 8
+// warps an SM, stalls are fixed latencies, the pipe itself and the CTA's
+// barriers); 4096 tokens without a window 2.96 ms, 0.63 of the rate.  One CTA of
+// 256 threads with 4 x 4 scores a thread took 204 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -4,16 +4,15 @@
 // The same sums as window_attention.cu's, all in f32 on the CUDA cores.  What
 // bounds it is reading K and V once, so a CTA takes up to 8 rows that share a
 // key head (query heads of its group times queries; 4 where there are no more)
-// and a share of the blocks
-// of 16 keys that any of them sees; its warps take blocks in turn, each with
-// its own two stages of cp.async copies and its own running maximum and sum,
-// and no barrier until they join.  Scores: a lane has one key and half of d
+// and a share of the blocks of 16 keys that any of them sees; its warps take
+// blocks in turn, each with its own two stages of cp.async copies and its own
+// running maximum and sum, and no barrier until they join.  Scores: a lane has one key and half of d
 // (rows of K pitched by 4 banks, so the 16 rows' pieces do not collide).
 // Output: a lane has DP / 32 columns, the probabilities come back through
 // shared memory.  Shares of a block of rows are joined by combine_kernel.
 //
-// Measured (D = 128): 16 x 32 heads over 8, one token over 4096 keys: 128 us,
-// 537 MB at 0.64 of the measured HBM rate; with 8 rows 183 us, the FMA and
+// Measured (D = 128): 16 x 32 heads over 8, one token over 4096 keys: 127 us,
+// 537 MB at 0.65 of the measured HBM rate; with 8 rows 183 us, the FMA and
 // shared-memory instructions of one warp a scheduler and a half.  One sequence
 // of 8192 keys: 27 us.  (Tiles of 64 rows: 1049 and 977 us.)
 #include <cuda.h>

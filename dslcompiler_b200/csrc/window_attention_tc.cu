@@ -24,19 +24,25 @@
 //
 // 4 D FLOP and one exponential a pair: at D = 128 the tensor core (8192 FLOP
 // a clock and SM) and the exponential unit (16 a clock and SM) need the same
-// 512 clocks for 128 x 64 pairs.  Neither is what bounds it: a key tile of
-// both query tiles takes 2000 to 2300 clocks, of which the tensor core works
-// 1560, and a softmax warp's chain (wait, TMEM load, maximum, exponentials,
-// TMEM store, arrive) is as long as that.
+// 512 clocks for 128 x 64 pairs.  Neither is what bounds it: under a window of
+// 1024 the tensor core works 44 % of the clocks and an instruction issues in
+// 39 %; a key tile of both query tiles takes 2000 to 2300 clocks, and a softmax
+// warp's chain (wait, TMEM load, maximum, exponentials, TMEM store, arrive) is
+// as long as that.
+//
+// P is rounded to the inputs' 16 bits, as the tensor core takes it, and its sum
+// is not: the error against 64 bits is 0.0018 (bf16) and 0.00023 (f16) of the
+// result's size, where rounding the result alone makes 0.0017 and 0.00021.
 //
 // Measured (bf16, D = 128): 32 heads over 8 of keys, 8192 tokens, window 4096
-// and 4 sinks: 369 us, 0.68 of the time of the products at the measured bf16
-// rate, 251 us; 32 heads, 4096 tokens, window 1024: 85 us for 37 (512 items on
-// 148 SMs: four rounds are paid, 3.46 worked).  Tried and
-// slower: key tiles of 64 (569 for then 497 us), one commit for several
-// products (107 for 92), exponentials partly by a polynomial on the FMA pipe
-// (95 to 91 for 87), registers moved from the MMA warps to the softmax (85 for
-// 86: no difference).
+// and 4 sinks: 372 us at 1965 MHz, 0.67 of the time of the products at the
+// measured bf16 rate, 251 us; called for seconds the power limit sets the clock,
+// 437 us at 1670 MHz.  32 heads, 4096 tokens, window 1024: 87 us for 37, for
+// seconds 98 us at 1730 MHz (512 items on 148 SMs: four rounds are paid, 3.46
+// worked).  Tried and slower: key tiles of 64 (569 for then 497 us), one commit
+// for several products (107 for 92), exponentials partly by a polynomial on the
+// FMA pipe (95 to 91 for 87), registers moved from the MMA warps to the softmax
+// (85 for 86: no difference).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
