@@ -159,3 +159,35 @@ def test_other_operators_results_stand_when_the_current_stream_is_late():
         assert torch.equal(early, want) and torch.equal(got, want), name
         for i, c in enumerate(copies):
             assert (c == i + 1.0).all(), (name, i)
+
+
+def test_calls_on_a_forked_stream_of_a_captured_graph():
+    """stream= names a stream that the capture has forked to: what the call makes belongs to the graph, and replays
+    do not need the memory that eager calls take in between."""
+    B, H, Hkv, D, L, page = 2, 8, 2, 64, 600, 16
+    q, k, v = rand(1, (B, H, 2, D)), rand(3, (B, Hkv, L, D)), rand(4, (B, Hkv, L, D))
+    cache = llk.QuantizedKVCache.empty(B * 40, page, Hkv, D)
+    table = torch.arange(B * 40, device="cuda", dtype=torch.int32).reshape(B, 40)
+    slots = (torch.arange(B, device="cuda")[:, None] * 640 + torch.arange(L, device="cuda")[None]).contiguous()
+    kv, few = ints([L, 450]), ints([2, 1])
+    cache.write(k, v, slots)
+
+    def run(s):
+        return (llk.window_attention(q, k, v, kv_lens=kv, q_lens=few, stream=s),
+                cache.attention(q, table, kv, q_lens=few, stream=s), *cache.read(slots, stream=s))
+
+    run(None)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        got = run(side)
+        main.wait_stream(side)
+    for seed in (5, 6):
+        q.copy_(rand(seed, q.shape))
+        graph.replay()
+        want = run(None)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
