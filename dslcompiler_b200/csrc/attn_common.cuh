@@ -79,11 +79,9 @@ __device__ __forceinline__ bool not_finite(T x, bool inf) {  // inf: only infini
 }
 
 // The first of the rows from, from + step, .. (count of them, step 1 or -1) of
-// v that holds a value that is not finite (inf: an infinity), or -1.  By one
-// warp.  `tick` (as in attention_row) may be null.
+// v that holds a value that is not finite (inf: an infinity), or -1.  By one warp.
 template <typename T>
-__device__ __noinline__ int bad_row(const T *v, int64_t v_sl, int D, int from, int count, int step, bool inf,
-                                    int *tick) {
+__device__ __noinline__ int bad_row(const T *v, int64_t v_sl, int D, int from, int count, int step, bool inf) {
   constexpr int kAt = 8, kVec = 16 / sizeof(T), kNone = 0x7fffffff;
   const int lane = threadIdx.x & 31;
   // pieces of a row, 16 bytes where rows start there, and rows of a round of kAt pieces a lane
@@ -122,7 +120,6 @@ __device__ __noinline__ int bad_row(const T *v, int64_t v_sl, int D, int from, i
     }
     found = __reduce_min_sync(0xffffffffu, found);
     if (found != kNone) return from + found * step;
-    if (tick && lane == 0) atomicAdd(tick, 1);
   }
   return -1;
 }
@@ -133,15 +130,17 @@ __device__ __noinline__ int bad_row(const T *v, int64_t v_sl, int D, int from, i
 struct HiddenBad {
   int late, early;
   // whether a row at position p with its window from lo may have met one
-  __device__ __forceinline__ bool meets(int p, int lo) const { return (late >= 0 && late > p) || (early >= 0 && early < lo); }
+  __device__ __forceinline__ bool meets(int p, int lo) const {
+    return (late >= 0 && late > p) || (early >= 0 && early < lo);
+  }
 };
 template <typename T>
-__device__ __forceinline__ HiddenBad hidden_bad(const T *v, int64_t v_sl, int D, int p0, int hi, int from, int last_lo,
-                                                int *tick = nullptr) {
+__device__ __forceinline__ HiddenBad hidden_bad(const T *v, int64_t v_sl, int D, int p0, int hi, int from,
+                                                int last_lo) {
   const int first = p0 + 1 > 0 ? p0 + 1 : 0;
   HiddenBad b;
-  b.late = hi > first ? bad_row(v, v_sl, D, hi - 1, hi - first, -1, false, tick) : -1;
-  b.early = last_lo > from ? bad_row(v, v_sl, D, from, last_lo - from, 1, false, tick) : -1;
+  b.late = hi > first ? bad_row(v, v_sl, D, hi - 1, hi - first, -1, false) : -1;
+  b.early = last_lo > from ? bad_row(v, v_sl, D, from, last_lo - from, 1, false) : -1;
   return b;
 }
 
@@ -157,38 +156,41 @@ __device__ __forceinline__ bool redo_row(const T *v, int64_t v_sl, const AttnMas
   if (hidden_bad<T>(v, v_sl, D, p, n, first > mk.sinks ? first : mk.sinks, lo).meets(p, lo)) return true;
   if (!k16 || !nan) return false;
   const int s_end = mk.sinks < lo ? mk.sinks : lo, end = p + 1 > 0 ? p + 1 : 0;
-  return bad_row<T>(v, v_sl, D, 0, s_end < end ? s_end : end, 1, true, nullptr) >= 0 ||
-         bad_row<T>(v, v_sl, D, lo, end - lo, 1, true, nullptr) >= 0;
+  return bad_row<T>(v, v_sl, D, 0, s_end < end ? s_end : end, 1, true) >= 0 ||
+         bad_row<T>(v, v_sl, D, lo, end - lo, 1, true) >= 0;
 }
 
-// Score of key row k (16 bytes at a time where rows start there).
+// A 16-byte piece as f32.
 template <typename T>
-__device__ __forceinline__ float dot_row(const T *q, const T *k, int D, bool vec) {
-  constexpr int kVec = 16 / sizeof(T);
-  float s = 0.f;
-  if (vec) {
-#pragma unroll 4
-    for (int d = 0; d < D; d += kVec) {
-      const uint4 a = *reinterpret_cast<const uint4 *>(q + d), b = *reinterpret_cast<const uint4 *>(k + d);
-      const T *x = reinterpret_cast<const T *>(&a), *y = reinterpret_cast<const T *>(&b);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) s = fmaf(to_f32(x[i]), to_f32(y[i]), s);
-    }
-  } else {
-    for (int d = 0; d < D; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-  }
-  return s;
+__device__ __forceinline__ float piece_at(const uint4 &x, int i) {
+  return to_f32(reinterpret_cast<const T *>(&x)[i]);
 }
 
 // One query row, one warp, straight from the definition; keys that the row
-// does not see are not touched.  D <= 256.  `tick`, where it is not null, is
-// counted up as the row proceeds, for those who wait for this warp with a limit.
+// does not see are not touched.  D <= 256.  o holds the tiles' result: where all
+// of it that is not finite is NaN by the row's own token, it stands (values that
+// are NaN throughout would have every row redone).
+//
+// 32 keys at a time: a lane has the score of one, then a 16-byte piece of every
+// (32 / pieces)-th value row; what rows are not made of such pieces goes element
+// by element.  Latency is all there is to it (a warp alone, many loads ahead).
 template <typename T>
 __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T *o, int64_t k_sl, int64_t v_sl, int D,
-                                           int p, int lo, int sinks, float scale_log2, int *tick = nullptr) {
+                                           int p, int lo, int sinks, float scale_log2) {
+  constexpr int kVec = 16 / sizeof(T), kAt = 8;
   const int lane = threadIdx.x & 31;
-  const bool vec = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | k_sl * sizeof(T) |
-                     D * sizeof(T)) & 15) == 0;
+  bool needed = p < 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    if (p >= 0 && d < D && not_finite(o[d], false)) needed |= !isnan(to_f32(v[p * v_sl + d]));
+  }
+  if (!__any_sync(0xffffffffu, needed)) return;
+  const int pieces = D / kVec;
+  const bool vec = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                     k_sl * sizeof(T) | v_sl * sizeof(T) | D * sizeof(T)) & 15) == 0 && pieces <= 32;
+  // a lane's piece, and its first row of the rows that the warp reads at once
+  const int at_once = vec ? 32 / pieces : 1, mine = vec ? lane % pieces : 0, row0 = vec ? lane / pieces : 0;
   float acc[8], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -197,9 +199,42 @@ __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T
   for (int part = 0; part < 2; ++part) {
     const int first = part == 0 ? 0 : lo, end = part == 0 ? (s_end < p + 1 ? s_end : p + 1) : p + 1;
     for (int j0 = first; j0 < end; j0 += 32) {
-      const int j = j0 + lane;
+      const int j = j0 + lane, cnt = end - j0 < 32 ? end - j0 : 32;
+      auto value_rows = [&](int t0, uint4 (&x)[kAt]) {  // kAt of this lane's value rows, from the t0-th on
+#pragma unroll
+        for (int u = 0; u < kAt; ++u) {
+          const int t = (t0 + u) * at_once + row0;
+          x[u] = make_uint4(0, 0, 0, 0);
+          if (row0 < at_once && t < cnt)
+            x[u] = *reinterpret_cast<const uint4 *>(v + static_cast<int64_t>(j0 + t) * v_sl + mine * kVec);
+        }
+      };
+      uint4 vx[kAt];
+      if (vec) value_rows(0, vx);
       float s = -INFINITY;
-      if (j < end) s = dot_row(q, k + j * k_sl, D, vec) * scale_log2;
+      if (j < end) {
+        const T *kr = k + static_cast<int64_t>(j) * k_sl;
+        s = 0.f;
+        if (vec) {
+          for (int c0 = 0; c0 < pieces; c0 += kAt) {
+            uint4 x[kAt], y[kAt];
+#pragma unroll
+            for (int u = 0; u < kAt; ++u) {
+              const int c = c0 + u < pieces ? c0 + u : c0;
+              x[u] = *reinterpret_cast<const uint4 *>(q + c * kVec);
+              y[u] = *reinterpret_cast<const uint4 *>(kr + c * kVec);
+            }
+#pragma unroll
+            for (int u = 0; u < kAt; ++u)
+              if (c0 + u < pieces)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) s = fmaf(piece_at<T>(x[u], i), piece_at<T>(y[u], i), s);
+          }
+        } else {
+          for (int d = 0; d < D; ++d) s = fmaf(to_f32(q[d]), to_f32(kr[d]), s);
+        }
+        s *= scale_log2;
+      }
       float mx = s;
 #pragma unroll
       for (int off = 16; off >= 1; off >>= 1) {
@@ -209,28 +244,53 @@ __device__ __noinline__ void attention_row(const T *q, const T *k, const T *v, T
       const float m_new = (mx != mx || m != m) ? NAN : fmaxf(m, mx);
       const float corr = m == -INFINITY ? 0.f : exp2f(m - m_new);
       const float pj = s == -INFINITY ? 0.f : exp2f(s - m_new);
-      l = l * corr;
+      l = fmaf(l, corr, pj);  // of this lane's keys
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] *= corr;
-      const int cnt = end - j0 < 32 ? end - j0 : 32;
-#pragma unroll 4
-      for (int t = 0; t < cnt; ++t) {
-        const float pt = __shfl_sync(0xffffffffu, pj, t);
-        l += pt;
+      if (vec) {
+        for (int t0 = 0; t0 * at_once < cnt; t0 += kAt) {
+          if (t0 > 0) value_rows(t0, vx);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = lane + 32 * i;
-          if (d < D) acc[i] = fmaf(pt, to_f32(v[(j0 + t) * v_sl + d]), acc[i]);
+          for (int u = 0; u < kAt; ++u) {
+            const int t = (t0 + u) * at_once + row0;
+            const float pt = __shfl_sync(0xffffffffu, pj, t & 31);
+            if (row0 < at_once && t < cnt)
+#pragma unroll
+              for (int i = 0; i < kVec; ++i) acc[i] = fmaf(pt, piece_at<T>(vx[u], i), acc[i]);
+          }
+        }
+      } else {
+        for (int t = 0; t < cnt; ++t) {
+          const float pt = __shfl_sync(0xffffffffu, pj, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int d = lane + 32 * i;
+            if (d < D) acc[i] = fmaf(pt, to_f32(v[static_cast<int64_t>(j0 + t) * v_sl + d]), acc[i]);
+          }
         }
       }
       m = m_new;
-      if (tick && lane == 0) atomicAdd(tick, 1);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    if (d < D) o[d] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+  for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (vec) {
+    // the lanes that share a piece, in order of their rows
+    for (int r = 1; r < at_once; ++r)
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const float x = __shfl_sync(0xffffffffu, acc[i], (mine + r * pieces) & 31);
+        if (row0 == 0) acc[i] += x;
+      }
+    if (row0 == 0)
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) o[mine * kVec + i] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = lane + 32 * i;
+      if (d < D) o[d] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+    }
   }
 }
 

@@ -6,8 +6,9 @@
 // key head (query heads of its group times queries; 4 where there are no more)
 // and a share of the blocks of 16 keys that any of them sees; its warps take
 // blocks in turn, each with its own two stages of cp.async copies and its own
-// running maximum and sum, and no barrier until they join.  Scores: a lane has one key and half of d
-// (rows of K pitched by 4 banks, so the 16 rows' pieces do not collide).
+// running maximum and sum, and no barrier until they join.  Scores: a lane has
+// one key and half of d (rows of K pitched by 4 banks, so the 16 rows' pieces do
+// not collide).
 // Output: a lane has DP / 32 columns, the probabilities come back through
 // shared memory.  Shares of a block of rows are joined by combine_kernel.
 //

@@ -35,9 +35,9 @@
 // result's size, where rounding the result alone makes 0.0017 and 0.00021.
 //
 // Measured (bf16, D = 128): 32 heads over 8 of keys, 8192 tokens, window 4096
-// and 4 sinks: 372 us at 1965 MHz, 0.67 of the time of the products at the
+// and 4 sinks: 371 us at 1965 MHz, 0.68 of the time of the products at the
 // measured bf16 rate, 251 us; called for seconds the power limit sets the clock,
-// 437 us at 1670 MHz.  32 heads, 4096 tokens, window 1024: 87 us for 37, for
+// 437 us at 1670 MHz.  32 heads, 4096 tokens, window 1024: 86 us for 37, for
 // seconds 98 us at 1730 MHz (512 items on 148 SMs: four rounds are paid, 3.46
 // worked).  Tried and slower: key tiles of 64 (569 for then 497 us), one commit
 // for several products (107 for 92), exponentials partly by a polynomial on the
@@ -55,7 +55,7 @@ namespace {
 
 constexpr int kBM = 128;                // rows of a query tile
 constexpr int kThreads = 352;
-constexpr uint64_t kWaitLimitNs = 1000000000ull;
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
 // The reference m may lag a row's maximum by up to this power of two before O
 // is rescaled: P stays below 2^8, far inside f16, its relative rounding is
 // the same, and the f32 sums do not mind.
@@ -89,33 +89,8 @@ struct Tail {
   uint64_t q_full[2], q_empty[2], o_free[2], kv_full[8], kv_empty[8], s_full[2], s_empty[2], p_ready[2], pv_done[2], landed, mma_done;
   uint32_t tmem;
   int abort;
-  int tick;  // counts on while a warp redoes rows
+  int bad;  // some row of the CTA is not finite
 };
-
-// mbar_wait_bounded, for waits on warps that may be redoing rows: it gives up
-// after one to two limits without any progress there.  (A row of 2^20 keys takes
-// a warp some tens of milliseconds, and it may have 32 of them.)
-__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, Tail *st) {
-  volatile int *abort = &st->abort, *tick = &st->tick;
-  if (mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = global_timer_ns();
-  int seen = -1;
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 0) {
-      if (*abort != 0) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
-        const int now = *tick;
-        if (now == seen) {
-          *abort = LLK_ERR_TIMEOUT;
-          return false;
-        }
-        seen = now;
-        t0 = global_timer_ns();
-      }
-    }
-  }
-}
 
 __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
   uint64_t r;
@@ -218,40 +193,54 @@ struct Ring {
   }
 };
 
-// A warp's rows that are not finite (bad: this lane's, written already, at
-// position pos): those that a value they do not see may have made so are redone
-// from the definition.
+// The rows of one item (256 from q0 on) whose written result is not finite:
+// those that a value they do not see may have made so are redone from the
+// definition.  By all warps of the CTA, 8 rows at a time, when its last item is
+// done: nobody waits for it with a limit, however many rows and keys there are.
 template <typename T>
-__device__ __noinline__ void redo_rows(const AttnProblem &P, bool bad, int b, int h, int row, int pos, int *tick) {
-  const int lane = threadIdx.x & 31, hk = h / (P.H / P.Hkv), sinks = P.mask.sinks;
+__device__ __noinline__ void redo_item(const AttnProblem &P, int b, int h, int q0) {
+  constexpr int kRows = 8;
+  const int lane = threadIdx.x & 31, hk = h / (P.H / P.Hkv), sinks = P.mask.sinks, D = P.D;
   const T *v = static_cast<const T *>(P.v.p) + b * P.v.sb + hk * P.v.sh;
   T *o = static_cast<T *>(P.o.p) + b * P.o.sb + h * P.o.sh;
-  // the keys that the CTA sweeps for these rows, as in the kernel's plan
   int n, m;
   seq_lens(P.mask, b, n, m);
-  const int q0 = row & ~(2 * kBM - 1), p0 = n - m + q0, hi = p0 + (m - q0 < 2 * kBM ? m - q0 : 2 * kBM);
+  // the keys that the CTA swept for these rows, as in the kernel's plan
+  const int end = m < q0 + 2 * kBM ? m : q0 + 2 * kBM, p0 = n - m + q0, hi = n - m + end;
   const int lo = window_lo(P.mask, p0), s_keys = sinks < lo ? sinks : lo;
-  const int warp_last = pos - lane + 31 < hi - 1 ? pos - lane + 31 : hi - 1;
-  const HiddenBad hidden = hidden_bad<T>(v, P.v.sl, P.D, pos - lane, hi, lo > sinks ? lo : sinks,
-                                         window_lo(P.mask, warp_last), tick);
-  bool again = bad && hidden.meets(pos, window_lo(P.mask, pos));
-  if constexpr (std::is_same<T, __half>::value) {
-    // a weight below f16's least times an infinity that the row does see: NaN here, not by the definition
-    bool nan = false;
-    if (bad && !again)
-      for (int d = 0; d < P.D; ++d) nan |= __hisnan(o[row * P.o.sl + d]);
-    if (__any_sync(0xffffffffu, nan)) {
-      const bool some = bad_row<T>(v, P.v.sl, P.D, 0, s_keys, 1, true, tick) >= 0 ||
-                        bad_row<T>(v, P.v.sl, P.D, lo, hi - lo, 1, true, tick) >= 0;
-      again |= nan && some;
+  int infinities = -1;  // among all values of the sweep (not looked yet)
+  for (int row = q0 + kRows * (threadIdx.x >> 5); row < end; row += kRows * (kThreads / 32)) {
+    const int rows = end - row < kRows ? end - row : kRows, pos = n - m + row;
+    unsigned bad = 0, nan = 0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int d = lane; d < 128; d += 32) {
+        const float x = r < rows && d < D ? to_f32(o[static_cast<int64_t>(row + r) * P.o.sl + d]) : 0.f;
+        bad |= (fabsf(x) < INFINITY ? 0u : 1u) << r;
+        nan |= (x != x ? 1u : 0u) << r;
+      }
+    bad = __reduce_or_sync(0xffffffffu, bad);
+    if (!bad) continue;
+    nan = __reduce_or_sync(0xffffffffu, nan);
+    const HiddenBad hidden = hidden_bad<T>(v, P.v.sl, D, pos, hi, lo > sinks ? lo : sinks,
+                                           window_lo(P.mask, pos + rows - 1));
+    for (; bad; bad &= bad - 1) {
+      const int r = __ffs(bad) - 1, p = pos + r, row_lo = window_lo(P.mask, p);
+      bool again = hidden.meets(p, row_lo);
+      if (std::is_same<T, __half>::value && !again && (nan >> r & 1)) {
+        // a weight below f16's least times an infinity that the row does see: NaN here, not by the definition
+        if (infinities < 0)
+          infinities = bad_row<T>(v, P.v.sl, D, 0, s_keys, 1, true) >= 0 ||
+                       bad_row<T>(v, P.v.sl, D, lo, hi - lo, 1, true) >= 0;
+        again = infinities > 0;
+      }
+      if (again)
+        attention_row<T>(
+            static_cast<const T *>(P.q.p) + b * P.q.sb + h * P.q.sh + static_cast<int64_t>(row + r) * P.q.sl,
+            static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh, v, o + static_cast<int64_t>(row + r) * P.o.sl,
+            P.k.sl, P.v.sl, D, p, row_lo, sinks, P.scale * kLog2e);
     }
-  }
-  for (unsigned todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
-    const int r = __ffs(todo) - 1 - lane;
-    __syncwarp();
-    attention_row<T>(static_cast<const T *>(P.q.p) + b * P.q.sb + h * P.q.sh + (row + r) * P.q.sl,
-                     static_cast<const T *>(P.k.p) + b * P.k.sb + hk * P.k.sh, v, o + (row + r) * P.o.sl, P.k.sl,
-                     P.v.sl, P.D, pos + r, window_lo(P.mask, pos + r), sinks, P.scale * kLog2e, tick);
   }
 }
 
@@ -283,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&st->landed, 1);
     mbar_init(&st->mma_done, 2);
     st->abort = 0;
-    st->tick = 0;
+    st->bad = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.k);
@@ -299,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t tmem = st->tmem;
+  volatile int *abort = &st->abort;
 
   // This CTA's blocks of rows: the last ones of the sequences, which have the
   // most keys, first, and every other round of them in reverse.
@@ -352,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int issued = 0;
     uint32_t landings = 0, queries[2] = {0, 0};
     auto wait = [&](uint64_t *bar, uint32_t phase) {
-      const bool r = wait_bounded(bar, phase & 1, st);
+      const bool r = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
       return static_cast<bool>(__all_sync(0xffffffffu, r));
     };
     for (int round = 0; ok && item_of(round) < items; ++round) {
@@ -442,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       Ring<ST> ring;
       auto wait = [&](uint64_t *bar, uint32_t phase) {
-        if (!mbar_try_wait(bar, phase & 1)) ok = wait_bounded(bar, phase & 1, st);
+        if (!mbar_try_wait(bar, phase & 1)) ok = mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
         tc_fence_after();
         return ok;
       };
@@ -513,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       const bool r = mbar_try_wait(bar, phase & 1) ||
-                     wait_bounded(bar, phase & 1, st);
+                     mbar_wait_bounded(bar, phase & 1, abort, LLK_ERR_TIMEOUT, kWaitLimitNs);
       ok = __all_sync(0xffffffffu, r);
       tc_fence_after();
       return ok;
@@ -654,9 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // (where its own scores are not finite, which l shows, it is right)
-      if (__any_sync(0xffffffffu, mine && bad && l == l))
-        redo_rows<T>(P, mine && bad && l == l, w.b, w.h, row, pos, &st->tick);
+      if (mine && bad) st->bad = 1;
     }
   }
   tc_fence_before();
@@ -666,6 +654,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, C::kCols);
   }
   if (threadIdx.x == 0 && st->abort != 0) atomicExch(A.status, st->abort);
+  if (st->bad && !st->abort)
+    for (int round = 0; item_of(round) < items; ++round) {
+      const int item = item_of(round), bh = item % BH;
+      redo_item<typename std::conditional<kBf16, __nv_bfloat16, __half>::type>(
+          P, bh / P.H, bh % P.H, (A.q_blocks - 1 - item / BH) * 2 * kBM);
+    }
 }
 
 // {D, L, H, B} map of a view with a box of 64 x rows; a broadcast or size-1

@@ -161,3 +161,30 @@ def test_values_at_the_largest_f16_stay_finite(B, H, Hkv, Lq, Lk, D, window, sin
     see = ref.visible(Lq, Lk, Lk, Lq, window, sinks)[:, Lk // 2].cuda()
     assert (got[0, :H // Hkv, see, 0] == math.inf).all()
     assert torch.isfinite(got[0, :H // Hkv, ~see]).all() and torch.isfinite(got[0, H // Hkv:]).all()
+
+
+@pytest.mark.parametrize("dtype,D,window", [(BF16, 128, 0), (F16, 64, 700), (F32, 64, 0)])
+def test_values_that_are_nan_from_some_token_on(dtype, D, window):
+    """The later half of a head's values all NaN, its keys not: each query has such values in front of it and behind;
+    those before the half are finite, and the call takes its usual time but for the tiles at the border."""
+    L, H = 8192 if dtype != F32 else 4096, 8
+    q, k, v = rand(1, (1, H, L, D), dtype), rand(2, (1, 2, L, D), dtype), rand(3, (1, 2, L, D), dtype)
+    kw = dict(window=window, sinks=2)
+    clean = llk.window_attention(q, k, v, **kw)
+    plain = timed(lambda: llk.window_attention(q, k, v, **kw))
+    cut = L // 2 + 37  # inside a tile
+    v[0, 1, cut:] = math.nan
+    got = llk.window_attention(q, k, v, **kw)
+    assert torch.equal(got[:, :H // 2], clean[:, :H // 2])
+    assert torch.isnan(got[0, H // 2:, cut:]).all()
+    before, want = got[0, H // 2:, :cut], clean[0, H // 2:, :cut]
+    assert torch.isfinite(before).all()
+    step = ref.HALF_STEP[dtype] if dtype != F32 else 2.0**-18  # (the rows at the border: by another order of sums)
+    assert ((before.double() - want.double()).abs() <= 4 * step * clean.abs().amax().double()).all()
+    t = timed(lambda: llk.window_attention(q, k, v, **kw))
+    v[0, 1] = math.nan
+    assert torch.isnan(llk.window_attention(q, k, v, **kw)[0, H // 2:]).all()
+    t_all = timed(lambda: llk.window_attention(q, k, v, **kw))
+    print(f"{dtype} D {D}: {plain:.3f} ms clean, {t:.3f} ms half NaN, {t_all:.3f} ms all NaN")
+    # the border's tiles: some rows of a warp, one after another, over half of the keys
+    assert t < 5 * plain + 15.0 and t_all < 5 * plain + 0.4
