@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (mine && bad) st->bad = 1;
+      if (mine && bad) st->bad = 1;  // (redo_item looks at it when the CTA's items are done)
     }
   }
   tc_fence_before();
